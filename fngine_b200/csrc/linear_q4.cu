@@ -1,0 +1,447 @@
+// Projections with 4-bit weights and group scales at decode width (T <= 16).
+//
+//   acc[t][r] = sum over groups g of  s[r][g] * sum_{i in g} (c[r][i] - z[r][g]) * x[t][i],   then the epilogue.
+//
+// c - z is a whole number of magnitude <= 15, exact in bf16, and so is x: the tensor core forms the inner sums of a group
+// from exact products in fp32, and one multiply-add per group and output applies the scale. Nothing is rounded but sums.
+//
+// The weights are the only large operand, so the kernel is built around their stream. A warp takes 16 MT rows (the M
+// side of mma.sync m16n8k16, the tokens are the N side) through K in steps of 128: its own ring of cp.async stages in
+// shared memory, no barrier between warps. ldmatrix gives lane (g, t) of a quad eight consecutive codes of row g, of
+// which every second MMA operand pair is one AND-OR: the nibbles of 0x000f000f under the bf16 exponent of 128, minus
+// 128 + z. The activations lie in shared memory in the order (0 4 1 5 2 6 3 7) that those pairs come in. S warps share
+// the K steps of a row tile and add their tiles in shared memory in warp order, so results do not depend on timing.
+#include "common.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace fb {
+namespace {
+
+constexpr int kQ4Warps = 16;
+constexpr int kQ4Threads = 32 * kQ4Warps;
+constexpr int kQ4Step = 128;    // K values per step of a warp: 64 bytes of a row
+constexpr int kQ4MaxTok = 16;
+constexpr int kQ4SmemLimit = 227 * 1024;
+
+struct Q4Args {
+  const __nv_bfloat16* x;
+  const uint8_t* codes;
+  const void* scales;
+  const uint8_t* zeros;
+  void* out;
+  const float* inj;
+  const float* gate_logit;
+  int n, k, tokens, kind, gate_stride;
+  int scale_f16;   // 16-bit scales: fp16 instead of bf16
+  int units;       // row tiles
+  int split;       // warps per row tile
+  int chunk;       // K steps whose activations are in shared memory at a time
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two codes (bits 0-3 and 16-19 of w) minus their zero point, as a bf16 pair: 128 + c is exact, and so is the difference.
+__device__ __forceinline__ uint32_t codes_to_bf16(uint32_t w, uint32_t zero) {
+  uint32_t v, r;
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(v) : "r"(w));  // (w & mask) | 128.0
+  asm("sub.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(zero));
+  return r;
+}
+
+// Stages of a warp's ring. One more costs 16 or 32 KB of the activations' room.
+template <int MT>
+constexpr int kQ4Stages = MT == 1 ? 6 : 3;
+template <int MT>
+constexpr int kQ4RowPitch = 16 * MT + 4;  // floats between tokens of a partial tile: lanes of a fragment in 32 banks
+template <int MT, int NT>
+constexpr int q4_fixed_smem() {
+  return kQ4Warps * (kQ4Stages<MT> * MT * 1024 + 8 * NT * kQ4RowPitch<MT> * 4);
+}
+
+template <int MT, int NT, int GROUP, bool SF32>
+__global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
+  constexpr int kStages = kQ4Stages<MT>;
+  constexpr int kGroups = kQ4Step / GROUP;                           // groups per step
+  constexpr int kScaleWords = SF32 ? kGroups : (kGroups + 1) / 2;    // 32-bit words of a row's scales per step
+  constexpr int kPitch = kQ4RowPitch<MT>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* ring = smem + warp * (kStages * MT * 1024);
+  float* tile = reinterpret_cast<float*>(smem + kQ4Warps * kStages * MT * 1024) + warp * (8 * NT * kPitch);
+  uint8_t* xs = smem + q4_fixed_smem<MT, NT>();
+  const int split = a.split, per_cta = kQ4Warps / split;
+  const int wk = warp % split, wu = warp / split;
+  const int ksteps = a.k / kQ4Step;
+  const int half = a.n >> 1;
+  const bool swiglu = a.kind == FB_EPI_SWIGLU;
+  const int first = blockIdx.x * per_cta + wu, stride = gridDim.x * per_cta;
+  const size_t row_bytes = size_t(a.k) >> 1;
+  const int row_groups = a.k / GROUP;
+
+  // Row r of a row tile; rows behind the last one repeat it and are not stored. SwiGlu: 16 gate rows, then their up rows.
+  auto row_of = [&](int unit, int r) {
+    if (swiglu) {
+      const int j = unit * 16 + (r & 15);
+      return (j < half ? j : half - 1) + (r >> 4) * half;
+    }
+    const int j = unit * (16 * MT) + r;
+    return j < a.n ? j : a.n - 1;
+  };
+
+  // Cursor of the code copies: kStages - 1 steps ahead of the products.
+  int pu = first, ps = wk;
+  const uint8_t* src[2 * MT];
+  auto seek = [&] {
+    if (pu < a.units) {
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) src[i] = a.codes + size_t(row_of(pu, 8 * i + g)) * row_bytes + t * 16;
+    }
+  };
+  const uint32_t ring_addr = smem_u32(ring);
+  // 16-byte chunk c of row r lies at r * 64 + (c ^ (r / 2 % 4)) * 16: eight rows of a chunk in eight bank groups.
+  const uint32_t put = uint32_t(g * 64 + ((t ^ ((g >> 1) & 3)) << 4));
+  int put_stage = 0;
+  auto copy_step = [&] {
+    if (pu < a.units) {
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i)
+        cp_async16(ring_addr + put_stage * (MT * 1024) + i * 512 + put, src[i] + size_t(ps) * 64);
+      ps += split;
+      if (ps >= ksteps) {
+        ps = wk;
+        pu += stride;
+        seek();
+      }
+    }
+    cp_async_commit();
+    put_stage = put_stage + 1 == kStages ? 0 : put_stage + 1;
+  };
+
+  // Scales and zero points of the step after the current one.
+  uint32_t s_raw[2 * MT][kScaleWords], z_raw[2 * MT];
+  int su = first, ss = wk;
+  auto load_scales = [&] {
+    if (su >= a.units) return;
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) {
+      const size_t at = size_t(row_of(su, 8 * i + g)) * row_groups + ss * kGroups;
+      if (SF32) {
+        const float* p = static_cast<const float*>(a.scales) + at;
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) s_raw[i][j] = __float_as_uint(p[j]);
+      } else {
+        const uint16_t* p = static_cast<const uint16_t*>(a.scales) + at;
+        if (kGroups == 1) {
+          s_raw[i][0] = *p;
+        } else {
+#pragma unroll
+          for (int j = 0; j < kScaleWords; ++j) s_raw[i][j] = reinterpret_cast<const uint32_t*>(p)[j];
+        }
+      }
+      if (a.zeros) {
+        const uint8_t* z = a.zeros + at;
+        z_raw[i] = kGroups == 1 ? *z : kGroups == 2 ? *reinterpret_cast<const uint16_t*>(z) : *reinterpret_cast<const uint32_t*>(z);
+        z_raw[i] &= 0x0f0f0f0fu;
+      }
+    }
+    ss += split;
+    if (ss >= ksteps) {
+      ss = wk;
+      su += stride;
+    }
+  };
+
+  seek();
+  pdl_wait_prior();
+  pdl_launch_dependents();
+#pragma unroll
+  for (int i = 0; i < 2 * MT; ++i) z_raw[i] = 0x08080808u;
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) copy_step();
+  load_scales();
+
+  const int x_pitch = a.chunk * (kQ4Step * 2) + 64;  // 64 modulo 128: two tokens' 64-byte blocks in different banks
+  const uint32_t xs_addr = smem_u32(xs);
+  uint32_t x_row[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {  // token columns behind the last one read its values and are not stored
+    const int tok = nt * 8 + g;
+    x_row[nt] = xs_addr + uint32_t((tok < a.tokens ? tok : a.tokens - 1) * x_pitch + t * 16);
+  }
+  // ldmatrix row addresses: lanes 0-7 rows 0-7 of a chunk, 8-15 rows 8-15, 16-31 the same of the next chunk.
+  const int lr = (lane & 7) + ((lane >> 3) & 1) * 8, lc = lane >> 4;
+  const uint32_t get = uint32_t(lr * 64), get_x = uint32_t((lr >> 1) & 3);
+  int get_stage = 0;
+
+  float acc[MT][NT][4];
+  bool loaded = false;
+  for (int base = blockIdx.x * per_cta; base < a.units; base += stride) {
+    const int unit = base + wu;
+    int step = unit < a.units ? wk : ksteps;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][nt][i] = 0.f;
+
+    for (int c0 = 0; c0 < ksteps; c0 += a.chunk) {
+      const int c1 = c0 + a.chunk < ksteps ? c0 + a.chunk : ksteps;
+      if (!loaded || a.chunk < ksteps) {  // (block-uniform)
+        if (loaded) __syncthreads();
+        const int per_row = (c1 - c0) * (kQ4Step / 8);
+        for (int i = threadIdx.x; i < per_row * a.tokens; i += kQ4Threads) {
+          const int tok = i / per_row, j = i - tok * per_row;
+          const uint4 v = *reinterpret_cast<const uint4*>(a.x + size_t(tok) * a.k + size_t(c0) * kQ4Step + j * 8);
+          uint4 w;
+          w.x = __byte_perm(v.x, v.z, 0x5410);
+          w.y = __byte_perm(v.x, v.z, 0x7632);
+          w.z = __byte_perm(v.y, v.w, 0x5410);
+          w.w = __byte_perm(v.y, v.w, 0x7632);
+          *reinterpret_cast<uint4*>(xs + tok * x_pitch + j * 16) = w;
+        }
+        loaded = true;
+        __syncthreads();
+      }
+      for (; step < c1; step += split) {
+        uint32_t s_now[2 * MT][kScaleWords], z_now[2 * MT];
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) {
+#pragma unroll
+          for (int j = 0; j < kScaleWords; ++j) s_now[i][j] = s_raw[i][j];
+          z_now[i] = z_raw[i];
+        }
+        load_scales();
+        cp_async_wait<kStages - 2>();
+        __syncwarp();
+        copy_step();  // into the stage that the step before has read
+        const uint32_t stage = ring_addr + get_stage * (MT * 1024) + get;
+        get_stage = get_stage + 1 == kStages ? 0 : get_stage + 1;
+        const uint32_t x_step = uint32_t((step - c0) * (kQ4Step * 2));
+        float part[MT][NT][4];
+#pragma unroll
+        for (int b2 = 0; b2 < 2; ++b2) {
+          uint32_t w[MT][4];
+#pragma unroll
+          for (int m = 0; m < MT; ++m) ldmatrix_x4(w[m], stage + m * 1024 + (((2 * b2 + lc) ^ get_x) << 4));
+#pragma unroll
+          for (int ci = 0; ci < 2; ++ci) {
+            constexpr int kBlocks = GROUP / 32;  // blocks of 32 values per group
+            const int b = 2 * b2 + ci, group = b / kBlocks;
+            if (b % kBlocks == 0) {
+#pragma unroll
+              for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) part[m][nt][i] = 0.f;
+            }
+            uint4 xv[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(xv[nt].x), "=r"(xv[nt].y), "=r"(xv[nt].z), "=r"(xv[nt].w)
+                           : "r"(x_row[nt] + x_step + b * 64)
+                           : "memory");
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              const uint32_t za = 0x43004300u + ((z_now[2 * m] >> (8 * group)) & 0xffu) * 0x00010001u;
+              const uint32_t zb = 0x43004300u + ((z_now[2 * m + 1] >> (8 * group)) & 0xffu) * 0x00010001u;
+              const uint32_t wa = w[m][2 * ci], wb = w[m][2 * ci + 1];
+              const uint32_t a0 = codes_to_bf16(wa, za), a1 = codes_to_bf16(wb, zb);
+              const uint32_t a2 = codes_to_bf16(wa >> 4, za), a3 = codes_to_bf16(wb >> 4, zb);
+              const uint32_t a4 = codes_to_bf16(wa >> 8, za), a5 = codes_to_bf16(wb >> 8, zb);
+              const uint32_t a6 = codes_to_bf16(wa >> 12, za), a7 = codes_to_bf16(wb >> 12, zb);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_bf16(part[m][nt], a0, a1, a2, a3, xv[nt].x, xv[nt].y);
+                mma_bf16(part[m][nt], a4, a5, a6, a7, xv[nt].z, xv[nt].w);
+              }
+            }
+            if (b % kBlocks == kBlocks - 1) {
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                float sc[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  if (SF32) {
+                    sc[i] = __uint_as_float(s_now[2 * m + i][group]);
+                  } else {
+                    const uint32_t h = (s_now[2 * m + i][group / 2] >> (16 * (group % 2))) & 0xffffu;
+                    sc[i] = a.scale_f16 ? __half2float(__ushort_as_half(uint16_t(h))) : __uint_as_float(h << 16);
+                  }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) acc[m][nt][i] = fmaf(sc[i >> 1], part[m][nt][i], acc[m][nt][i]);
+              }
+            }
+          }
+        }
+      }
+    }
+
+    // The warps of a row tile meet in shared memory; their threads share the outputs.
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          tile[(nt * 8 + 2 * t + (i & 1)) * kPitch + m * 16 + g + (i >> 1) * 8] = acc[m][nt][i];
+    if (split == 1) __syncwarp();
+    else named_bar_sync(1 + wu, 32 * split);
+    if (unit < a.units) {
+      const float* tiles = tile - wk * (8 * NT * kPitch);
+      const int rows = swiglu ? 16 : 16 * MT, shift = rows == 16 ? 4 : 5;
+      const int row0 = unit * rows, row_end = swiglu ? half : a.n;
+      for (int i = wk * 32 + lane; i < rows * a.tokens; i += 32 * split) {
+        const int r = i & (rows - 1), tok = i >> shift;
+        const float* p = tiles + tok * kPitch + r;
+        float v = 0.f, u = 0.f;
+        for (int w = 0; w < split; ++w) v += p[w * (8 * NT * kPitch)];
+        if (swiglu) {
+          for (int w = 0; w < split; ++w) u += p[w * (8 * NT * kPitch) + 16];
+        }
+        const int row = row0 + r;
+        if (row >= row_end) continue;
+        if (a.kind == FB_EPI_STORE_BF16) {
+          static_cast<__nv_bfloat16*>(a.out)[size_t(tok) * a.n + row] = __float2bfloat16_rn(v);
+        } else if (a.kind == FB_EPI_STORE_F32) {
+          static_cast<float*>(a.out)[size_t(tok) * a.n + row] = v;
+        } else if (swiglu) {
+          static_cast<__nv_bfloat16*>(a.out)[size_t(tok) * half + row] = __float2bfloat16_rn(v / (1.f + expf(-v)) * u);
+        } else if (a.kind == FB_EPI_SHARED_SCALE) {
+          const float gate = a.gate_logit[size_t(tok) * a.gate_stride];
+          static_cast<float*>(a.out)[size_t(tok) * a.n + row] = v / (1.f + expf(-gate));
+        } else {  // GrWrite: four residual streams
+          float* X = static_cast<float*>(a.out) + size_t(tok) * 4 * a.n + row;
+#pragma unroll
+          for (int s = 0; s < 4; ++s) X[size_t(s) * a.n] += a.inj[tok * 4 + s] * v;
+        }
+      }
+    }
+    if (split == 1) __syncwarp();
+    else named_bar_sync(1 + wu, 32 * split);
+  }
+  cp_async_wait<0>();
+}
+
+template <int MT, int NT, int GROUP, bool SF32>
+cudaError_t launch_q4(const Q4Args& a, int grid, size_t smem, cudaStream_t stream) {
+  static PerDeviceOnce once;
+  const cudaError_t e = per_device_once(once, [] { return opt_in_smem(q4_kernel<MT, NT, GROUP, SF32>, kQ4SmemLimit); });
+  if (e != cudaSuccess) return e;
+  return launch_pdl(q4_kernel<MT, NT, GROUP, SF32>, dim3(unsigned(grid)), dim3(kQ4Threads), smem, stream, a);
+}
+template <int MT, int NT>
+cudaError_t launch_q4_group(const Q4Args& a, int group, bool f32, int grid, size_t smem, cudaStream_t s) {
+  if (group == 32) return f32 ? launch_q4<MT, NT, 32, true>(a, grid, smem, s) : launch_q4<MT, NT, 32, false>(a, grid, smem, s);
+  if (group == 64) return f32 ? launch_q4<MT, NT, 64, true>(a, grid, smem, s) : launch_q4<MT, NT, 64, false>(a, grid, smem, s);
+  return f32 ? launch_q4<MT, NT, 128, true>(a, grid, smem, s) : launch_q4<MT, NT, 128, false>(a, grid, smem, s);
+}
+
+}  // namespace
+}  // namespace fb
+
+using namespace fb;
+
+extern "C" {
+
+int32_t fb_linear_q4_decode(const void* x_bf16, int32_t tokens, const fb_q4_weight* weight,
+                            const fb_linear_epilogue* epilogue, void* stream) {
+  if (!x_bf16 || !weight || !weight->codes || !weight->scales || !epilogue || !epilogue->out)
+    return invalid("linear_q4_decode: null argument");
+  if (tokens <= 0 || tokens > kQ4MaxTok) return invalid("linear_q4_decode: tokens must be 1..16");
+  const int n = weight->n, k = weight->k, group = weight->group, kind = epilogue->kind;
+  if (n <= 0 || k <= 0 || k % kQ4Step) return invalid("linear_q4_decode: unsupported shape (k %% 128)");
+  if (group != 32 && group != 64 && group != 128) return invalid("linear_q4_decode: groups of 32, 64 or 128 values");
+  if (weight->scales_dtype != FB_DT_F32 && weight->scales_dtype != FB_DT_BF16 && weight->scales_dtype != FB_DT_F16)
+    return invalid("linear_q4_decode: scales are fp32, bf16 or fp16");
+  if (kind < FB_EPI_STORE_BF16 || kind > FB_EPI_SHARED_SCALE) return invalid("linear_q4_decode: unknown epilogue");
+  if (kind == FB_EPI_GR_WRITE && !epilogue->inj) return invalid("linear_q4_decode: GrWrite needs inj fp32 [tokens][4]");
+  if (kind == FB_EPI_SHARED_SCALE && !epilogue->gate_logit)
+    return invalid("linear_q4_decode: SharedScale needs gate_logit");
+  if (kind == FB_EPI_SWIGLU && n % 2) return invalid("linear_q4_decode: SwiGlu needs n %% 2 == 0");
+  if ((reinterpret_cast<uintptr_t>(weight->codes) | reinterpret_cast<uintptr_t>(x_bf16) |
+       reinterpret_cast<uintptr_t>(weight->scales) | reinterpret_cast<uintptr_t>(weight->zeros)) & 15)
+    return invalid("linear_q4_decode: x, weight codes, scales and zeros must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(epilogue->out) & (kind == FB_EPI_STORE_BF16 || kind == FB_EPI_SWIGLU ? 1 : 3))
+    return invalid("linear_q4_decode: out is not aligned to its elements");
+  const size_t out_values = size_t(tokens) * size_t(n);
+  const size_t out_bytes = kind == FB_EPI_GR_WRITE ? 16 * out_values : kind == FB_EPI_STORE_BF16 ? 2 * out_values
+                           : kind == FB_EPI_SWIGLU ? out_values : 4 * out_values;
+  const uintptr_t x0 = reinterpret_cast<uintptr_t>(x_bf16), out0 = reinterpret_cast<uintptr_t>(epilogue->out);
+  if (out0 < x0 + size_t(tokens) * size_t(k) * 2 && x0 < out0 + out_bytes)
+    return invalid("linear_q4_decode: out lies in the memory of x");
+
+  Q4Args a;
+  a.x = static_cast<const __nv_bfloat16*>(x_bf16);
+  a.codes = weight->codes;
+  a.scales = weight->scales;
+  a.zeros = weight->zeros;
+  a.out = epilogue->out;
+  a.inj = epilogue->inj;
+  a.gate_logit = epilogue->gate_logit;
+  a.n = n;
+  a.k = k;
+  a.tokens = tokens;
+  a.kind = kind;
+  a.gate_stride = epilogue->gate_stride;
+  a.scale_f16 = weight->scales_dtype == FB_DT_F16;
+
+  const int sms = sm_count(), ksteps = k / kQ4Step, nt = tokens > 8 ? 2 : 1;
+  // Two row tiles of 16 per warp halve the reads of activations per weight.
+  const int mt = kind == FB_EPI_SWIGLU || nt == 2 ? 2 : 1;
+  const long long units = kind == FB_EPI_SWIGLU ? (n / 2 + 15) / 16 : (n + 16 * mt - 1LL) / (16 * mt);
+  // The number of warps per row tile that ends first, by the steps that the busiest warp takes.
+  long long best = -1;
+  for (int s = 1; s <= kQ4Warps && (s == 1 || s / 2 < ksteps); s *= 2) {
+    const long long per_wave = (long long)sms * (kQ4Warps / s);
+    const long long cost = (units + per_wave - 1) / per_wave * ((ksteps + s - 1) / s);
+    if (s <= ksteps && (best < 0 || cost < best)) {
+      best = cost;
+      a.split = s;
+    }
+  }
+  a.units = int(units);
+  const long long ctas = (units + kQ4Warps / a.split - 1) / (kQ4Warps / a.split);
+  const int grid = int(ctas < sms ? ctas : sms);
+  const int fixed = mt == 1 ? (nt == 1 ? q4_fixed_smem<1, 1>() : q4_fixed_smem<1, 2>())
+                            : (nt == 1 ? q4_fixed_smem<2, 1>() : q4_fixed_smem<2, 2>());
+  const int room = (kQ4SmemLimit - fixed) / tokens;  // bytes of a token's activations
+  a.chunk = (room - 64) / (kQ4Step * 2);
+  if (a.chunk > ksteps) a.chunk = ksteps;
+  const size_t smem = size_t(fixed) + size_t(tokens) * (size_t(a.chunk) * kQ4Step * 2 + 64);
+  const bool f32 = weight->scales_dtype == FB_DT_F32;
+  cudaStream_t s = as_stream(stream);
+  const cudaError_t e = mt == 1 ? launch_q4_group<1, 1>(a, group, f32, grid, smem, s)
+                        : nt == 1 ? launch_q4_group<2, 1>(a, group, f32, grid, smem, s)
+                                  : launch_q4_group<2, 2>(a, group, f32, grid, smem, s);
+  const int32_t st = check_launch("linear_q4_decode");
+  return st ? st : int32_t(e);
+}
+
+}  // extern "C"

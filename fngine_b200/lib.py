@@ -12,7 +12,7 @@ LIB_PATH = os.environ.get("FNGINE_B200_LIB") or os.path.join(HERE, "libfngine_b2
 
 FMT_IQ4_NL, FMT_IQ3_S = 20, 21
 FMT_IQ3_XXS, FMT_IQ2_S, FMT_IQ4_XS, FMT_Q2_0 = 18, 22, 23, 42  # decode width only
-DT_F32, DT_BF16 = 0, 1
+DT_F32, DT_BF16, DT_F16 = 0, 1, 2
 ACT_Q8_K, ACT_Q8_0 = 0, 1
 HIDDEN, EXPERTS, TOPK, ROUTER_ROWS = 2560, 512, 10, 513
 DECODE_MAX_TOKENS, DECODE_MAX_PAIRS = 16, 160
@@ -66,6 +66,12 @@ class LinearEpilogue(C.Structure):
     """fb_linear_epilogue: the output side of a decode-width projection."""
     _fields_ = [("kind", C.c_int32), ("gate_stride", C.c_int32), ("out", C.c_void_p), ("inj", C.c_void_p),
                 ("gate_logit", C.c_void_p)]
+
+
+class Q4Weight(C.Structure):
+    """fb_q4_weight: 4-bit codes with a scale and a zero point per group."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("zeros", C.c_void_p), ("scales_dtype", C.c_int32),
+                ("group", C.c_int32), ("n", C.c_int32), ("k", C.c_int32)]
 
 
 class SharedExpert(C.Structure):
@@ -142,6 +148,7 @@ _SIGNATURES = {
     "fb_fp8_quantize_tokens": (_I32, [_P, _I32, _I32, _P, _P, _P]),
     "fb_linear_fp8_decode_workspace_bytes": (C.c_size_t, [_I32, _I32]),
     "fb_linear_fp8_decode": (_I32, [_P, _I32, _P, _P, _I32, _I32, _I32, C.POINTER(LinearEpilogue), _P, C.c_size_t, _P]),
+    "fb_linear_q4_decode": (_I32, [_P, _I32, C.POINTER(Q4Weight), C.POINTER(LinearEpilogue), _P]),
     "fb_dequant_rows": (_I32, [_I32, _P, _I64, _I32, _I32, _P, _P]),
     "fb_quantize_act": (_I32, [_I32, _P, _I32, _I32, _I32, _P, _P]),
     "fb_synth_fill_blocks": (_I32, [_I32, _P, _I64, _I64, C.c_uint64, _P, _P]),

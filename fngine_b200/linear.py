@@ -99,6 +99,38 @@ def linear_fp8_decode(x, weight, epilogue, workspace):
         L.check(st, "linear_fp8_decode")
 
 
+class Q4GroupWeight:
+    """fb_q4_weight: codes uint8 [n][k / 2] (value 2j of a row in the low four bits of byte j), scales fp32, bf16 or fp16
+    [n][k / group], zeros uint8 [n][k / group] or None (eight everywhere). The group size follows from the shapes."""
+
+    def __init__(self, codes, scales, zeros=None):
+        assert codes.is_cuda and codes.dtype == torch.uint8 and codes.dim() == 2 and codes.is_contiguous()
+        assert scales.is_cuda and scales.dtype in _DTYPES and scales.dim() == 2 and scales.shape[0] == codes.shape[0]
+        self.codes, self.scales = codes, scales.contiguous()
+        self.n, self.k = codes.shape[0], 2 * codes.shape[1]
+        assert scales.shape[1] and self.k % scales.shape[1] == 0
+        self.group = self.k // scales.shape[1]
+        if zeros is not None:
+            assert zeros.is_cuda and zeros.dtype == torch.uint8 and zeros.shape == scales.shape
+            zeros = zeros.contiguous()
+        self.zeros = zeros
+        self.c = L.Q4Weight(self.codes.data_ptr(), self.scales.data_ptr(), None if zeros is None else zeros.data_ptr(),
+                            _DTYPES[scales.dtype], self.group, self.n, self.k)
+        self.ref = ctypes.byref(self.c)
+
+
+_DTYPES = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
+
+
+def linear_q4_decode(x, weight, epilogue):
+    """fb_linear_q4_decode: x bf16 [T][k], T <= 16; the output is whatever `epilogue` (store_bf16, store_f32, gr_write,
+    swiglu, shared_scale) names. Products are exact and sums fp32."""
+    assert x.dtype == torch.bfloat16 and x.is_contiguous() and x.shape[1] == weight.k
+    st = L.load().fb_linear_q4_decode(x.data_ptr(), x.shape[0], weight.ref, ctypes.byref(epilogue), L.stream())
+    if st:
+        L.check(st, "linear_q4_decode")
+
+
 def fp8_quantize_tokens(x):
     """Per-token E4M3 codes and fp32 scales of bf16 x [T][k]."""
     T, k = x.shape

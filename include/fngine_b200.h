@@ -38,8 +38,8 @@ extern "C" {
  * streaming decode kernel, IQ3_XXS, IQ2_S and IQ4_XS as gate/up, Q2_0 as down, IQ3_S and IQ4_NL as both; the prefill
  * kernels take IQ3_S and IQ4_NL. */
 enum { FB_FMT_IQ3_XXS = 18, FB_FMT_IQ4_NL = 20, FB_FMT_IQ3_S = 21, FB_FMT_IQ2_S = 22, FB_FMT_IQ4_XS = 23, FB_FMT_Q2_0 = 42 };
-/* element types of activation inputs */
-enum { FB_DT_F32 = 0, FB_DT_BF16 = 1 };
+/* element types of activation inputs (FB_DT_F16: only where an entry point names it) */
+enum { FB_DT_F32 = 0, FB_DT_BF16 = 1, FB_DT_F16 = 2 };
 /* activation block formats (src/cpu/iq_cpu.h:44) */
 enum { FB_ACT_Q8_K = 0, FB_ACT_Q8_0 = 1 };
 
@@ -460,6 +460,28 @@ size_t fb_linear_fp8_decode_workspace_bytes(int32_t n, int32_t k);
 int32_t fb_linear_fp8_decode(const void* x_bf16, int32_t tokens, const uint8_t* w_codes, const void* w_scales,
                              int32_t w_scales_dtype, int32_t n, int32_t k, const fb_linear_epilogue* epilogue,
                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- 4-bit projection at decode width
+ * Beside fb_linear_fp8_decode, for weights of four bits with a scale (and a zero point) per group of consecutive values of
+ * a row (no reference counterpart: the reference's dense weights are FP8 rows):
+ *   out = epilogue(sum over groups of scale[n][g] * sum_{i in g} (code[n][i] - zero[n][g]) * x[t][i])
+ * codes [n][k / 2]: value 2j of a row in the low four bits of byte j, value 2j + 1 in the high ones. scales [n][k / group],
+ * fp32, bf16 or fp16. zeros [n][k / group]: one byte per group, of which the low four bits count, or NULL: eight everywhere.
+ * group 32, 64 or 128; k % 128 == 0; any n (even for SwiGlu). codes, scales, zeros and x are 16-byte aligned.
+ * x is bf16 [tokens][k], tokens 1..16; the epilogues are those of fb_linear_fp8. Products are exact, sums are fp32; every
+ * output is written once, in an order of additions that the shape fixes: repeated calls are bitwise identical. `out` may not
+ * lie in the memory of x. No workspace. */
+typedef struct fb_q4_weight {
+  const uint8_t* codes;
+  const void* scales;
+  const uint8_t* zeros;
+  int32_t scales_dtype; /* FB_DT_F32, FB_DT_BF16 or FB_DT_F16 */
+  int32_t group;
+  int32_t n;
+  int32_t k;
+} fb_q4_weight;
+int32_t fb_linear_q4_decode(const void* x_bf16, int32_t tokens, const fb_q4_weight* weight,
+                            const fb_linear_epilogue* epilogue, void* stream);
 
 /* ---------------------------------------------------------------- parity probes (no reference counterpart)
  * The same device routines the GEMV kernels use, exposed so that dequantized weights and int8
