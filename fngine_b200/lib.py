@@ -74,6 +74,30 @@ class Q4Weight(C.Structure):
                 ("group", C.c_int32), ("n", C.c_int32), ("k", C.c_int32)]
 
 
+class Qkv(C.Structure):
+    """fb_qkv: queries, keys and values of packed tokens."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
+                ("v_stride", C.c_int64), ("dtype", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32)]
+
+
+class QkNorm(C.Structure):
+    """fb_qk_norm: weights of the norms per head."""
+    _fields_ = [("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("weight_dtype", C.c_int32), ("eps", C.c_float)]
+
+
+class RopeArgs(C.Structure):
+    """fb_rope: frequencies, positions and their axes."""
+    _fields_ = [("inv_freq", C.c_void_p), ("positions", C.c_void_p), ("axis_stride", C.c_int64), ("rot_dim", C.c_int32),
+                ("axes", C.c_int32), ("sections", C.c_int32 * 4), ("adjacent", C.c_int32), ("reserved", C.c_int32)]
+
+
+class QkvOut(C.Structure):
+    """fb_qkv_out: where rotated queries and keys and the values go."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
+                ("v_stride", C.c_int64), ("slots", C.c_void_p), ("n_slots", C.c_int64)]
+
+
 class SharedExpert(C.Structure):
     """fb_shared_expert: weights and intermediate buffers of a layer's shared expert."""
     _fields_ = [("gate_up_codes", C.c_void_p), ("gate_up_scales", C.c_void_p), ("down_codes", C.c_void_p),
@@ -149,6 +173,7 @@ _SIGNATURES = {
     "fb_linear_fp8_decode_workspace_bytes": (C.c_size_t, [_I32, _I32]),
     "fb_linear_fp8_decode": (_I32, [_P, _I32, _P, _P, _I32, _I32, _I32, C.POINTER(LinearEpilogue), _P, C.c_size_t, _P]),
     "fb_linear_q4_decode": (_I32, [_P, _I32, C.POINTER(Q4Weight), C.POINTER(LinearEpilogue), _P]),
+    "fb_qk_norm_rope": (_I32, [C.POINTER(Qkv), _I32, C.POINTER(QkNorm), C.POINTER(RopeArgs), C.POINTER(QkvOut), _P]),
     "fb_dequant_rows": (_I32, [_I32, _P, _I64, _I32, _I32, _P, _P]),
     "fb_quantize_act": (_I32, [_I32, _P, _I32, _I32, _I32, _P, _P]),
     "fb_synth_fill_blocks": (_I32, [_I32, _P, _I64, _I64, C.c_uint64, _P, _P]),

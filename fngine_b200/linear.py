@@ -126,6 +126,7 @@ def linear_q4_decode(x, weight, epilogue):
     """fb_linear_q4_decode: x bf16 [T][k], T <= 16; the output is whatever `epilogue` (store_bf16, store_f32, gr_write,
     swiglu, shared_scale) names. Products are exact and sums fp32."""
     assert x.dtype == torch.bfloat16 and x.is_contiguous() and x.shape[1] == weight.k
+    assert x.get_device() == weight.codes.get_device() == torch._C._cuda_getDevice()
     st = L.load().fb_linear_q4_decode(x.data_ptr(), x.shape[0], weight.ref, ctypes.byref(epilogue), L.stream())
     if st:
         L.check(st, "linear_q4_decode")

@@ -483,6 +483,59 @@ typedef struct fb_q4_weight {
 int32_t fb_linear_q4_decode(const void* x_bf16, int32_t tokens, const fb_q4_weight* weight,
                             const fb_linear_epilogue* epilogue, void* stream);
 
+/* ---------------------------------------------------------------- attention branch of a layer
+ * What stands between a layer's projections: norms and rotation of queries and keys, and attention. No counterpart in the
+ * reference's interface of this path (its own attention is a sparse one over an 8-bit cache). Tensors are bf16 (FB_DT_BF16)
+ * or fp16 (FB_DT_F16), [tokens][heads][head_dim] with the heads of a token side by side; strides are elements between
+ * tokens, so that q, k and v may be parts of one projection's output. */
+typedef struct fb_qkv {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_stride;
+  int64_t k_stride;
+  int64_t v_stride;
+  int32_t dtype;
+  int32_t heads;    /* of q */
+  int32_t kv_heads; /* of k and v */
+  int32_t head_dim;
+} fb_qkv;
+typedef struct fb_qk_norm {
+  const void* q_weight; /* [head_dim], or NULL: no norm */
+  const void* k_weight;
+  int32_t weight_dtype; /* FB_DT_F32, FB_DT_BF16 or FB_DT_F16 */
+  float eps;
+} fb_qk_norm;
+typedef struct fb_rope {
+  const float* inv_freq;     /* [rot_dim / 2] */
+  const int32_t* positions;  /* [axes][tokens] */
+  int64_t axis_stride;       /* elements between the positions of two axes */
+  int32_t rot_dim;           /* leading values of a head that are turned: a multiple of 16 */
+  int32_t axes;              /* 1..4 */
+  int32_t sections[4];       /* frequencies of each axis, in their order; they add up to rot_dim / 2 (not read for one axis) */
+  int32_t adjacent;          /* 0: frequency j turns the pair (j, j + rot_dim / 2); otherwise (2j, 2j + 1) */
+  int32_t reserved;
+} fb_rope;
+typedef struct fb_qkv_out {
+  void* q;
+  void* k;
+  void* v;
+  int64_t q_stride;
+  int64_t k_stride; /* elements between rows of k: tokens, or slots */
+  int64_t v_stride;
+  const int64_t* slots; /* [tokens] rows that k and v go to, or NULL: the token's own */
+  int64_t n_slots;      /* rows of k and v; a slot outside of them is not stored */
+} fb_qkv_out;
+/* y = x * rsqrt(mean(x^2) + eps) * weight per head of q and k (norm NULL or a weight NULL: y = x), then the rotation
+ * (a, b) -> (a cos p - b sin p, b cos p + a sin p) of every pair, p = position * inv_freq of the pair's frequency, formed in 64
+ * bits (rope NULL: none); v is copied. One pass, fp32 arithmetic, one rounding. With `slots` k and v go to rows of a
+ * cache (page * page_size + offset of a paged one): slots that differ from token to token; a negative one or one behind n_slots
+ * stores nothing, q is stored all the same. Any of q, k, v may be NULL together with its output. An output may be its input
+ * exactly (same address and stride, no slots) or lie apart from all inputs. head_dim 64, 128 or 256; everything 16-byte
+ * aligned, strides multiples of 8 elements. */
+int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm, const fb_rope* rope, const fb_qkv_out* out,
+                        void* stream);
+
 /* ---------------------------------------------------------------- parity probes (no reference counterpart)
  * The same device routines the GEMV kernels use, exposed so that dequantized weights and int8
  * activations can be compared bit for bit with the CPU reference. */
