@@ -81,3 +81,59 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, eps, rope, positions, q_out, k_out
     st = L.load().fb_qk_norm_rope(given, tokens, norm, None if rope is None else rope.c(positions, tokens), out, L.stream())
     if st:
         L.check(st, "qk_norm_rope")
+
+
+class KvCache:
+    """fb_kv_cache: k and v [n_pages][page_size][kv_heads][head_dim], bf16 or fp16. k_rows and v_rows are its slots one after
+    another (page * page_size + offset), the rows that qk_norm_rope writes to."""
+
+    def __init__(self, k, v):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _DTYPES or not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("KvCache: k and v [n_pages][page_size][kv_heads][head_dim] of one type, contiguous")
+        _here("KvCache", k, v)
+        self.k, self.v = k, v
+        self.n_pages, self.page_size, self.kv_heads, self.head_dim = k.shape
+        self.dtype = k.dtype
+        self.k_rows, self.v_rows = (x.view(-1, self.kv_heads, self.head_dim) for x in (k, v))
+        self.c = L.KvCacheArgs(k.data_ptr(), v.data_ptr(), self.n_pages, self.page_size, _DTYPES[k.dtype], self.kv_heads, self.head_dim)
+        self.ref = ctypes.byref(self.c)
+
+
+def attn_tree_workspace(n_seqs, drafted, heads, kv_heads, head_dim, device="cuda"):
+    """Zero-filled workspace of attn_tree_decode for up to n_seqs sequences of these shapes; every call leaves it ready for the next."""
+    n = L.load().fb_attn_tree_workspace_bytes(n_seqs, drafted, heads, kv_heads, head_dim)
+    if not n:
+        raise ValueError("attn_tree_workspace: unsupported shape")
+    buf = torch.zeros(n + 256, dtype=torch.uint8, device=device)
+    off = (-buf.data_ptr()) % 256
+    return buf[off:off + n]
+
+
+def attn_tree_decode(q, cache, block_table, contexts, out, workspace, mask=None, scale=None):
+    """fb_attn_tree_decode: q and out [n_seqs][drafted][heads][head_dim], block_table int32 [n_seqs][columns], contexts int32 [n_seqs],
+    mask int64 or uint64 [n_seqs][drafted] (bit d of token i: it sees drafted token d; None: d <= i), scale 1 / sqrt(head_dim) unless given."""
+    n_seqs, drafted, heads, dim = q.shape
+    if q.dtype != cache.dtype or out.dtype != q.dtype or out.shape != q.shape or dim != cache.head_dim:
+        raise ValueError("attn_tree_decode: q and out [n_seqs][drafted][heads][head_dim] of the cache's type")
+    strides = []
+    for x in (q, out):
+        s = x.stride()
+        token = s[1] if drafted > 1 else s[0] if n_seqs > 1 else heads * dim
+        if s[3] != 1 or (heads > 1 and s[2] != dim) or (n_seqs > 1 and s[0] != drafted * token):
+            raise ValueError("attn_tree_decode: the tokens of q and out lie at one stride, the heads of a token side by side")
+        strides.append(token)
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n_seqs or block_table.stride(1) != 1:
+        raise ValueError("attn_tree_decode: block_table int32 [n_seqs][columns]")
+    if contexts.dtype != torch.int32 or contexts.shape != (n_seqs,) or not contexts.is_contiguous():
+        raise ValueError("attn_tree_decode: contexts int32 [n_seqs]")
+    if mask is not None and (mask.dtype not in (torch.int64, torch.uint64) or mask.shape != (n_seqs, drafted) or not mask.is_contiguous()):
+        raise ValueError("attn_tree_decode: mask int64 [n_seqs][drafted]")
+    columns = block_table.stride(0) if n_seqs > 1 else block_table.shape[1]
+    if columns < block_table.shape[1]:
+        raise ValueError("attn_tree_decode: rows of block_table overlap")
+    _here("attn_tree_decode", q, out, block_table, contexts, mask, workspace)
+    st = L.load().fb_attn_tree_decode(q.data_ptr(), strides[0], heads, n_seqs, drafted, cache.ref, block_table.data_ptr(), columns,
+                                      contexts.data_ptr(), None if mask is None else mask.data_ptr(), dim ** -0.5 if scale is None else scale,
+                                      out.data_ptr(), strides[1], workspace.data_ptr(), workspace.numel(), L.stream())
+    if st:
+        L.check(st, "attn_tree_decode")

@@ -98,6 +98,12 @@ class QkvOut(C.Structure):
                 ("v_stride", C.c_int64), ("slots", C.c_void_p), ("n_slots", C.c_int64)]
 
 
+class KvCacheArgs(C.Structure):
+    """fb_kv_cache: a paged cache of keys and values."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_pages", C.c_int64), ("page_size", C.c_int32), ("dtype", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
 class SharedExpert(C.Structure):
     """fb_shared_expert: weights and intermediate buffers of a layer's shared expert."""
     _fields_ = [("gate_up_codes", C.c_void_p), ("gate_up_scales", C.c_void_p), ("down_codes", C.c_void_p),
@@ -174,6 +180,9 @@ _SIGNATURES = {
     "fb_linear_fp8_decode": (_I32, [_P, _I32, _P, _P, _I32, _I32, _I32, C.POINTER(LinearEpilogue), _P, C.c_size_t, _P]),
     "fb_linear_q4_decode": (_I32, [_P, _I32, C.POINTER(Q4Weight), C.POINTER(LinearEpilogue), _P]),
     "fb_qk_norm_rope": (_I32, [C.POINTER(Qkv), _I32, C.POINTER(QkNorm), C.POINTER(RopeArgs), C.POINTER(QkvOut), _P]),
+    "fb_attn_tree_workspace_bytes": (C.c_size_t, [_I32, _I32, _I32, _I32, _I32]),
+    "fb_attn_tree_decode": (_I32, [_P, _I64, _I32, _I32, _I32, C.POINTER(KvCacheArgs), _P, _I64, _P, _P, C.c_float, _P, _I64,
+                                   _P, C.c_size_t, _P]),
     "fb_dequant_rows": (_I32, [_I32, _P, _I64, _I32, _I32, _P, _P]),
     "fb_quantize_act": (_I32, [_I32, _P, _I32, _I32, _I32, _P, _P]),
     "fb_synth_fill_blocks": (_I32, [_I32, _P, _I64, _I64, C.c_uint64, _P, _P]),

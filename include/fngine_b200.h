@@ -536,6 +536,36 @@ typedef struct fb_qkv_out {
 int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm, const fb_rope* rope, const fb_qkv_out* out,
                         void* stream);
 
+/* A paged cache of keys and values: k and v [n_pages][page_size][kv_heads][head_dim], bf16 or fp16, 16-byte aligned. */
+typedef struct fb_kv_cache {
+  const void* k;
+  const void* v;
+  int64_t n_pages;
+  int32_t page_size; /* any size from 1 */
+  int32_t dtype;
+  int32_t kv_heads;
+  int32_t head_dim;
+} fb_kv_cache;
+/* Attention of `drafted` tokens (1..64) per sequence over the cache. Position p of sequence s lies in page block_table[s *
+ * table_stride + p / page_size]; positions 0 .. contexts[s] - 1 are the context, which every token sees, and the keys and
+ * values of the drafted tokens follow at contexts[s] .. contexts[s] + drafted - 1 (fb_qk_norm_rope puts them there). Token
+ * i sees drafted token d if bit d of mask[s * drafted + i] is set; mask NULL: if d <= i. So one token per sequence is plain
+ * decoding, and a shorter tree is padded with tokens whose masks are zero. q and out are [n_seqs * drafted][heads][head_dim] with
+ * strides between tokens; query head h reads key head h / (heads / kv_heads).
+ *   out[i] = sum_j softmax_j(scale q_i . k_j) v_j, scale > 0;  zeros where a token sees nothing.
+ * contexts, table and mask are read on the device: a captured call follows what they hold at its replay. A context outside
+ * of 0 .. table_stride * page_size is taken as the nearer end, positions behind the table are not there, and a page outside
+ * of the cache reads as zeros. What lies in the cache at positions that no token of the sequence sees is not looked at; keys and values that some
+ * token sees are to be finite. Softmax statistics and sums are fp32, the weights are rounded to the type of v. Joins of split
+ * work are in a fixed order: repeated calls are bitwise identical.
+ * `workspace`: fb_attn_tree_workspace_bytes() bytes (0 for an unsupported shape), 256-byte aligned, zero-filled once; the
+ * call leaves its counters clear. Calls that share one must not overlap, captured ones included. head_dim 64 or 128. */
+size_t fb_attn_tree_workspace_bytes(int32_t n_seqs, int32_t drafted, int32_t heads, int32_t kv_heads, int32_t head_dim);
+int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int32_t n_seqs, int32_t drafted,
+                            const fb_kv_cache* cache, const int32_t* block_table, int64_t table_stride, const int32_t* contexts,
+                            const uint64_t* mask, float scale, void* out, int64_t out_stride, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- parity probes (no reference counterpart)
  * The same device routines the GEMV kernels use, exposed so that dequantized weights and int8
  * activations can be compared bit for bit with the CPU reference. */

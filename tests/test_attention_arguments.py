@@ -53,3 +53,62 @@ def test_python_mirror_refuses_what_does_not_fit():
         a.update(change)
         with pytest.raises((ValueError, AttributeError)):
             A.qk_norm_rope(**a)
+
+
+def test_attn_tree_refusals(fb_built):
+    lib = L.load()
+    size = lib.fb_attn_tree_workspace_bytes
+    need = size(2, 3, 8, 2, 128)
+    assert need == 256 + 512 * 16 * 130 * 4 and size(2, 64, 8, 1, 64) == 256 + 512 * 128 * 66 * 4
+    assert size(100, 64, 16, 2, 64) == 100 * 2 * 4 * 4 + 128 + 512 * 128 * 66 * 4  # four row tiles of 128
+    for bad in [(-1, 3, 8, 2, 128), (2, 0, 8, 2, 128), (2, 65, 8, 2, 128), (2, 3, 9, 2, 128), (2, 3, 8, 0, 128), (2, 3, 2, 8, 128), (2, 3, 8, 2, 96)]:
+        assert size(*bad) == 0
+
+    def call(q=P, q_stride=1024, heads=8, n_seqs=2, drafted=3, cache={}, no_cache=False, table=2 * P, table_stride=4, contexts=3 * P, mask=4 * P,
+             scale=0.1, out=5 * P, out_stride=1024, workspace=6 * P, bytes=need):
+        c = dict(k=7 * P, v=8 * P, n_pages=9, page_size=16, dtype=L.DT_F16, kv_heads=2, head_dim=128)
+        c.update(cache)
+        c = L.KvCacheArgs(**c)
+        st = lib.fb_attn_tree_decode(q, q_stride, heads, n_seqs, drafted, None if no_cache else C.byref(c), table, table_stride, contexts, mask, scale,
+                                     out, out_stride, workspace, bytes, None)
+        return st, lib.fb_last_error_string()
+
+    for bad, word in [(dict(no_cache=True), b"null"), (dict(q=None), b"null"), (dict(out=None), b"null"), (dict(table=None), b"null"),
+                      (dict(contexts=None), b"null"), (dict(cache=dict(k=None)), b"null"), (dict(cache=dict(v=None)), b"null"),
+                      (dict(cache=dict(dtype=L.DT_F32)), b"bf16 or fp16"), (dict(drafted=0), b"1..64"), (dict(drafted=65), b"1..64"),
+                      (dict(heads=7), b"shape"), (dict(n_seqs=-1), b"shape"), (dict(cache=dict(kv_heads=0)), b"shape"), (dict(cache=dict(head_dim=80)), b"shape"),
+                      (dict(cache=dict(page_size=0)), b"pages"), (dict(cache=dict(n_pages=0)), b"pages"), (dict(table_stride=0), b"columns"),
+                      (dict(table_stride=2 ** 27), b"2^30"), (dict(q_stride=1016), b"stride"), (dict(out_stride=512), b"stride"), (dict(q_stride=1028), b"16 bytes"),
+                      (dict(q=P + 8), b"16 bytes"), (dict(cache=dict(v=8 * P + 2)), b"16 bytes"), (dict(table=2 * P + 2), b"aligned"),
+                      (dict(mask=4 * P + 4), b"aligned"), (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"),
+                      (dict(scale=float("inf")), b"scale"), (dict(workspace=None), b"workspace"), (dict(workspace=6 * P + 128), b"workspace"), (dict(bytes=need - 1), b"workspace")]:
+        st, msg = call(**bad)
+        assert st == 1 and word in msg, (bad, st, msg)
+    assert call(n_seqs=0)[0] == 0
+
+
+def test_how_tree_tiles_are_cut():
+    """The kernel's arithmetic: block b takes tiles [b total / blocks, (b + 1) total / blocks) of all segments' tiles. The blocks that a
+    segment says it has pieces in are those that hold some of its tiles, and a block's partial pieces go to different slots."""
+    import random
+    rng = random.Random(3)
+    for _ in range(300):
+        tiles = [rng.choice([1, 1, 2, 3, 17, 200]) for _ in range(rng.randint(1, 60))]
+        total = sum(tiles)
+        blocks = min(total, rng.choice([1, 2, 7, 148]))
+        owner = {}
+        for b in range(blocks):
+            lo, hi = b * total // blocks, (b + 1) * total // blocks
+            assert hi > lo
+            for t in range(lo, hi):
+                owner[t] = b
+        assert sorted(owner) == list(range(total))
+        slots, begin = {}, 0
+        for s, n in enumerate(tiles):
+            first, last = ((begin + 1) * blocks - 1) // total, ((begin + n) * blocks - 1) // total
+            assert {owner[t] for t in range(begin, begin + n)} == set(range(first, last + 1))
+            if first != last:
+                for b in range(first, last + 1):
+                    slot = 2 * b + (1 if max(begin, b * total // blocks) == begin else 0)
+                    assert slots.setdefault(slot, s) == s and slot == (2 * first + 1 if b == first else 2 * b)
+            begin += n
