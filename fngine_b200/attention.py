@@ -83,6 +83,26 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, eps, rope, positions, q_out, k_out
         L.check(st, "qk_norm_rope")
 
 
+def attn_prefill(q, k, v, cu_seqlens, out, scale=None, status=None):
+    """fb_attn_prefill: q and out [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim], cu_seqlens int32 [n_seqs + 1]; scale
+    1 / sqrt(head_dim) unless given. status: a word (int32 [1]) that a wait which ran out sets."""
+    tokens, heads, dim = q.shape
+    kv_heads = k.shape[1]
+    if q.dtype not in _DTYPES or not (q.dtype == k.dtype == v.dtype == out.dtype):
+        raise ValueError("attn_prefill: bf16 or fp16, the same for all tensors")
+    if k.shape != (tokens, kv_heads, dim) or v.shape != k.shape or out.shape != q.shape:
+        raise ValueError("attn_prefill: shapes do not fit")
+    if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or not cu_seqlens.is_contiguous():
+        raise ValueError("attn_prefill: cu_seqlens int32 [n_seqs + 1]")
+    q_at, k_at, v_at, o_at = _heads(q, "q"), _heads(k, "k"), _heads(v, "v"), _heads(out, "out")
+    _here("attn_prefill", q, k, v, cu_seqlens, out, status)
+    given = L.Qkv(q_at[0], k_at[0], v_at[0], q_at[1], k_at[1], v_at[1], _DTYPES[q.dtype], heads, kv_heads, dim)
+    st = L.load().fb_attn_prefill(given, tokens, cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, dim ** -0.5 if scale is None else scale,
+                                  o_at[0], o_at[1], None if status is None else status.data_ptr(), L.stream())
+    if st:
+        L.check(st, "attn_prefill")
+
+
 class KvCache:
     """fb_kv_cache: k and v [n_pages][page_size][kv_heads][head_dim], bf16 or fp16. k_rows and v_rows are its slots one after
     another (page * page_size + offset), the rows that qk_norm_rope writes to."""

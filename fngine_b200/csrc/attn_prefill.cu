@@ -1,0 +1,514 @@
+// Causal attention over packed prompts with grouped heads, on tcgen05.
+//
+//   out_i = sum_{j <= i} softmax_j(scale q_i . k_j) v_j     within a sequence; query head h reads key head h / (heads / kv_heads)
+//
+// One pass over the keys per query tile with a running maximum and sum. A block takes 256 queries of one head as two tiles of
+// 128 (TMEM lanes) and goes through the keys 128 at a time:
+//   S = Q K^T   tcgen05 kind::f16, both operands in shared memory, fp32 S in tensor memory (128 columns per tile)
+//   P = 2^(c S - c m) in the type of v, written over S by the tile's four softmax warps, a thread per row: no shuffles
+//   O += P V    P from tensor memory, V as it lies in memory (keys x head_dim: the operand's N-major form), fp32 O in tensor memory
+// The two tiles are half a step apart: while one is in its softmax, the tensor core has the other's two products.
+// m is the maximum that the exponents refer to, not the latest one: it moves up (and O is multiplied) only when a row's scores
+// rise above it by more than 2^8, which leaves every weight at most 256 and the sum in fp32 range. Normally that is
+// the first block alone, so O stays in tensor memory untouched.
+// Blocks are handed out longest first (causal: the last queries of a prompt have the most keys).
+#include "attn_common.cuh"
+
+#include <cuda.h>
+
+namespace fb {
+namespace {
+
+constexpr int kPfRows = 128;             // queries per tile, keys per block
+constexpr int kPfQueries = 2 * kPfRows;  // queries per CTA
+constexpr int kPfThreads = 384;          // two softmax warpgroups, one with the copying and the issuing warp
+constexpr float kPfSlack = 8.f;          // how far (in powers of two) scores may rise above the maximum in use
+
+template <int D>
+struct PfShape {
+  static constexpr int kTileBytes = kPfRows * D * 2;
+  static constexpr int kHalf = kPfRows * 128;  // a tile is D / 64 parts of 128 rows x 128 bytes
+  static constexpr int kStages = D == 128 ? 5 : 8;
+  static constexpr int kSmem = (2 + kStages) * kTileBytes + 1024 + 256;
+};
+
+struct PfArgs {
+  void* out;
+  const int32_t* cu_seqlens;
+  uint32_t* status;
+  int64_t out_stride;
+  float scale_log2;
+  int n_seqs, tokens, group;
+};
+struct PfMaps {
+  CUtensorMap q, k, v;
+};
+
+struct PfBars {
+  uint64_t q_full[2], s_full[2], p_full[2], o_done[2], full[8], empty[8], drained;  // 200 bytes
+  uint32_t tmem;
+  int aborted;
+  int issued;  // copies of keys and values
+};
+
+__device__ __forceinline__ void pf_tma(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                   dst),
+               "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void pf_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void pf_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pf_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void pf_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void pf_ld32(uint32_t taddr, float (&f)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void pf_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pf_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pf_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// Shared-memory operand descriptors, 128-byte swizzle, 8-row groups 1024 bytes apart, descriptor version 1. `lead`: for a
+// tile whose rows run along K (Q, K) not used (1); for V, whose rows run along N, the distance of its two 64-value parts.
+__device__ __forceinline__ uint64_t pf_desc(uint32_t addr, uint32_t lead) {
+  return uint64_t((addr & 0x3FFFFu) >> 4) | (uint64_t(lead) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+
+// Bounded wait. A wait that ran out is recorded, and every later one ends at once.
+__device__ __forceinline__ bool pf_wait(PfBars* bars, uint32_t* status, uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  for (uint32_t i = 0; i < (1u << 21); ++i) {
+    if (mbar_try_wait_hint(bar, parity)) return true;
+    if ((i & 63u) == 63u && *static_cast<volatile int*>(&bars->aborted)) return false;
+  }
+  *static_cast<volatile int*>(&bars->aborted) = 1;
+  if (status) atomicMax(status, uint32_t(FB_STATUS_PIPELINE_TIMEOUT));
+  return false;
+}
+
+static_assert(sizeof(PfBars) <= 256, "room behind the ring");
+
+template <class T, int D>
+__global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArgs a, const __grid_constant__ PfMaps maps) {
+  using S = PfShape<D>;
+  constexpr int kStages = S::kStages, kParts = D / 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* q_tiles = smem;
+  uint8_t* ring = smem + 2 * S::kTileBytes;
+  PfBars* bars = reinterpret_cast<PfBars*>(ring + kStages * S::kTileBytes);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait_prior();
+
+  // Which sequence and which 256 queries: item blockIdx.y counts the items of the sequences in order, each from its end.
+  int start = 0, length = -1, item = -1;
+  {
+    int before = 0;
+    for (int base = 0; base < a.n_seqs; base += 32) {
+      const int s = base + lane;
+      int lo = 0, hi = 0;
+      if (s < a.n_seqs) {
+        lo = a.cu_seqlens[s];
+        hi = a.cu_seqlens[s + 1];
+        lo = lo < 0 ? 0 : lo > a.tokens ? a.tokens : lo;
+        hi = hi < lo ? lo : hi > a.tokens ? a.tokens : hi;
+      }
+      const int n = (hi - lo + kPfQueries - 1) / kPfQueries;
+      int upto = n;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += other;
+      }
+      const int at = int(blockIdx.y) - before;
+      const bool mine = n > 0 && at < upto && at >= upto - n;
+      const uint32_t who = __ballot_sync(0xffffffffu, mine);
+      if (who) {
+        const int src = __ffs(who) - 1;
+        start = __shfl_sync(0xffffffffu, lo, src);
+        length = __shfl_sync(0xffffffffu, hi - lo, src);
+        item = __shfl_sync(0xffffffffu, upto - 1 - at, src);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  if (item < 0) return;  // (block-uniform)
+  const int head = blockIdx.x, kv_head = head / a.group;
+  const int row0 = item * kPfQueries;
+  const int blocks0 = 2 * item + 1, blocks1 = row0 + kPfRows < length ? 2 * item + 2 : 0;
+  const int blocks = blocks1 ? blocks1 : blocks0;
+
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->q_full[i], 1);
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_full[i], kPfRows);
+      mbar_init(&bars->o_done[i], 1);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bars->full[i], 1);
+      mbar_init(&bars->empty[i], 1);
+    }
+    mbar_init(&bars->drained, 1);
+    bars->aborted = 0;
+    bars->issued = 0;
+    mbar_fence_init();
+  }
+  pf_fence_before();
+  __syncthreads();
+  pf_fence_after();
+  // (not before the allocation: a block of the next kernel that took tensor memory and then waited for this one would hold it up)
+  pdl_launch_dependents();
+  const uint32_t tmem = bars->tmem;
+  constexpr uint32_t kS = 0, kO = 256;  // tile i: S in columns 128 i, O in 256 + 128 i
+
+  if (warp == 9) {
+    // ------------------------------------------------------------------ copies
+    if (lane == 0) {
+      auto tile = [&](uint8_t* dst, const CUtensorMap* map, int h, int row, uint64_t* bar) {
+        mbar_expect_tx(bar, S::kTileBytes);
+        for (int p = 0; p < kParts; ++p) pf_tma(smem_u32(dst) + p * S::kHalf, map, p * 64, h, row, bar);
+      };
+      tile(q_tiles, &maps.q, head, start + row0, &bars->q_full[0]);
+      for (int i = 0; i < 2 * blocks; ++i) {  // K_0 V_0 K_1 V_1 ...
+        const int slot = i % kStages;
+        if (i >= kStages && !pf_wait(bars, a.status, &bars->empty[slot], uint32_t(i / kStages - 1) & 1)) break;
+        tile(ring + slot * S::kTileBytes, i & 1 ? &maps.v : &maps.k, kv_head, start + (i >> 1) * kPfRows, &bars->full[slot]);
+        bars->issued = i + 1;
+        if (i == 0 && blocks1)
+          tile(q_tiles + S::kTileBytes, &maps.q, head, start + row0 + kPfRows, &bars->q_full[1]);
+      }
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ products
+    constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kPfRows >> 4) << 24);
+    constexpr uint32_t kIdescQk = kIdesc | (uint32_t(kPfRows >> 3) << 17);
+    constexpr uint32_t kIdescPv = kIdesc | (uint32_t(D >> 3) << 17) | (1u << 16);  // V runs along N
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && __all_sync(0xffffffffu, pf_wait(bars, a.status, bar, parity));
+    };
+    auto scores = [&](int t, int j) {
+      const int slot = (2 * j) % kStages;
+      wait(&bars->full[slot], uint32_t(2 * j / kStages) & 1);
+      if (!ok) return;
+      pf_fence_after();
+      if (elect_one()) {
+        const uint64_t qd = pf_desc(smem_u32(q_tiles + t * S::kTileBytes), 1), kd = pf_desc(smem_u32(ring + slot * S::kTileBytes), 1);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t at = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
+          pf_mma_ss(tmem + kS + 128 * t, qd + at, kd + at, kIdescQk, k > 0);
+        }
+        pf_commit(&bars->s_full[t]);
+      }
+      __syncwarp();
+    };
+    bool cleared = false;
+    auto outputs = [&](int t, int j) {
+      const int slot = (2 * j + 1) % kStages;
+      wait(&bars->p_full[t], uint32_t(j) & 1);
+      wait(&bars->full[slot], uint32_t((2 * j + 1) / kStages) & 1);
+      if (!ok) return;
+      const int there = length - j * kPfRows;
+      if (there < kPfRows && !cleared) {
+        // Rows of the next sequence: their weights are zero, but they need not be finite.
+        for (int i = lane; i < (kPfRows - there) * (D / 8); i += 32) {
+          const int row = there + i / (D / 8), c = i % (D / 8);
+          *reinterpret_cast<uint4*>(ring + slot * S::kTileBytes + (c / 8) * S::kHalf + row * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        cleared = true;
+      }
+      pf_fence_after();
+      if (elect_one()) {
+        const uint64_t vd = pf_desc(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
+#pragma unroll
+        for (int k = 0; k < kPfRows / 16; ++k)
+          pf_mma_ts(tmem + kO + 128 * t, tmem + kS + 128 * t + 8 * k, vd + k * (2048 >> 4), kIdescPv, j > 0 || k > 0);
+        pf_commit(&bars->o_done[t]);
+      }
+      __syncwarp();
+    };
+    auto release = [&](int i) {
+      if (ok && elect_one()) pf_commit(&bars->empty[i % kStages]);
+      __syncwarp();
+    };
+    wait(&bars->q_full[0], 0);
+    scores(0, 0);
+    if (blocks1) {
+      wait(&bars->q_full[1], 0);
+      scores(1, 0);
+    }
+    release(0);
+    for (int j = 0; j < blocks && ok; ++j) {
+      if (j < blocks0) {
+        outputs(0, j);
+        if (j + 1 < blocks0) scores(0, j + 1);
+      }
+      if (j < blocks1) {
+        outputs(1, j);
+        if (j + 1 < blocks1) scores(1, j + 1);
+      }
+      release(2 * j + 1);
+      if (j + 1 < blocks) release(2 * j + 2);
+    }
+    // Nothing issued here is still running when the tensor memory is given back.
+    if (elect_one()) pf_commit(&bars->drained);
+    __syncwarp();
+    for (uint32_t n = 0; n < (1u << 16) && !__all_sync(0xffffffffu, mbar_try_wait_hint(&bars->drained, 0)); ++n) {}
+  } else if (warp < 8) {
+    // ------------------------------------------------------------------ softmax
+    const int t = warp >> 2, row = tid & 127;
+    const int n = t ? blocks1 : blocks0;
+    const uint32_t lanes = uint32_t(warp & 3) << 21;  // (32 (warp % 4)) << 16
+    const uint32_t s_at = tmem + lanes + kS + 128 * t, o_at = tmem + lanes + kO + 128 * t;
+    const bool real = row0 + t * kPfRows + row < length;
+    float top = -INFINITY, sum = 0.f;
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      ok = ok && __all_sync(0xffffffffu, pf_wait(bars, a.status, &bars->s_full[t], uint32_t(j) & 1));
+      if (!ok) break;
+      pf_fence_after();
+      float s[4][32];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf_ld32(s_at + 32 * i, s[i]);
+      pf_ld_wait();
+      if (j == n - 1) {  // the diagonal
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (32 * i + c > row) s[i][c] = -INFINITY;
+      }
+      float m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        m[i] = s[i][0];
+#pragma unroll
+        for (int c = 1; c < 32; ++c) m[i] = fmaxf(m[i], s[i][c]);
+      }
+      const float latest = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      // (always in the first block; rows behind the sequence are nobody's and decide nothing)
+      const bool rises = real && (latest - top) * a.scale_log2 > kPfSlack;
+      if (__any_sync(0xffffffffu, rises)) {
+        const float up = fmaxf(latest, top);
+        const float fade = exp2_approx((top - up) * a.scale_log2);
+        top = up;
+        sum *= fade;
+        if (j > 0) {
+          ok = __all_sync(0xffffffffu, pf_wait(bars, a.status, &bars->o_done[t], uint32_t(j - 1) & 1));
+          if (!ok) break;
+          pf_fence_after();
+#pragma unroll 1
+          for (int i = 0; i < D / 32; ++i) {
+            float o[32];
+            pf_ld32(o_at + 32 * i, o);
+            pf_ld_wait();
+            uint32_t r[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(o[c] * fade);
+            pf_st16(o_at + 32 * i, r);
+            pf_st16(o_at + 32 * i + 16, r + 16);
+          }
+          pf_st_wait();
+        }
+      }
+      const float base = top * a.scale_log2;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t p[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const float x = exp2_approx(fmaf(s[i][2 * c], a.scale_log2, -base));
+          const float y = exp2_approx(fmaf(s[i][2 * c + 1], a.scale_log2, -base));
+          part[c & 3] += x + y;
+          p[c] = pack2<T>(x, y);  // rounded to the type of v: half a step of each weight, averaged over the keys
+        }
+        pf_st16(s_at + 16 * i, p);
+      }
+      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      pf_st_wait();
+      pf_fence_before();
+      mbar_arrive(&bars->p_full[t]);
+    }
+    if (n > 0 && ok) ok = __all_sync(0xffffffffu, pf_wait(bars, a.status, &bars->o_done[t], uint32_t(n - 1) & 1));
+    if (n > 0 && ok) {
+      pf_fence_after();
+      // Through the query tile's memory, which nothing reads any more, to whole rows of 16-byte stores.
+      const float inv = 1.f / sum;
+      uint8_t* stage = q_tiles + t * S::kTileBytes + (warp & 3) * (32 * D * 2);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        float o[32];
+        pf_ld32(o_at + 32 * i, o);
+        pf_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint4 v;
+          v.x = pack2<T>(o[8 * c] * inv, o[8 * c + 1] * inv);
+          v.y = pack2<T>(o[8 * c + 2] * inv, o[8 * c + 3] * inv);
+          v.z = pack2<T>(o[8 * c + 4] * inv, o[8 * c + 5] * inv);
+          v.w = pack2<T>(o[8 * c + 6] * inv, o[8 * c + 7] * inv);
+          *reinterpret_cast<uint4*>(stage + lane * (D * 2) + (((4 * i + c) ^ (lane & 7)) << 4)) = v;
+        }
+      }
+      __syncwarp();
+      constexpr int kChunks = D / 8, kRows = 32 / kChunks;
+      const int chunk = lane % kChunks;
+#pragma unroll 4
+      for (int i = 0; i < 32 / kRows; ++i) {
+        const int r = i * kRows + lane / kChunks, q = row0 + t * kPfRows + (warp & 3) * 32 + r;
+        if (q < length) {
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + r * (D * 2) + ((chunk ^ (r & 7)) << 4));
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + int64_t(start + q) * a.out_stride + head * D + chunk * 8) = v;
+        }
+      }
+      pf_fence_before();
+    }
+  }
+  __syncthreads();
+  pf_fence_after();
+  if (bars->aborted && tid == 0) {  // copies that nobody waited for
+    const int issued = bars->issued;
+    for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+      for (uint32_t n = 0; n < (1u << 16) && !mbar_try_wait_hint(&bars->full[i % kStages], uint32_t(i / kStages) & 1); ++n) {}
+    for (int i = 0; i < (blocks1 ? 2 : 1); ++i)
+      for (uint32_t n = 0; n < (1u << 16) && !mbar_try_wait_hint(&bars->q_full[i], 0); ++n) {}
+  }
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+using PfEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+PfEncodeFn pf_encode_fn() {
+  static PfEncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PfEncodeFn>(p);
+  }();
+  return fn;
+}
+// [tokens][heads][dim] in boxes of 128 tokens x 64 values of one head; tokens behind the last one read as zeros.
+bool pf_map(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, int tokens, int64_t stride) {
+  const cuuint64_t dims[3] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(tokens)};
+  const cuuint64_t strides[2] = {cuuint64_t(dim) * 2, cuuint64_t(stride) * 2};
+  const cuuint32_t box[3] = {64, 1, kPfRows}, elem[3] = {1, 1, 1};
+  return pf_encode_fn()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                        const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T, int D>
+cudaError_t launch_pf(const PfArgs& a, const PfMaps& maps, dim3 grid, cudaStream_t s) {
+  static PerDeviceOnce once;
+  const cudaError_t e = per_device_once(once, [] { return opt_in_smem(attn_prefill_kernel<T, D>, PfShape<D>::kSmem); });
+  if (e != cudaSuccess) return e;
+  return launch_pdl(attn_prefill_kernel<T, D>, grid, dim3(kPfThreads), size_t(PfShape<D>::kSmem), s, a, maps);
+}
+
+}  // namespace
+}  // namespace fb
+
+using namespace fb;
+
+extern "C" {
+
+int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seqlens, int32_t n_seqs, float scale, void* out,
+                        int64_t out_stride, uint32_t* status, void* stream) {
+  if (!in) return invalid("attn_prefill: null argument");
+  const int dim = in->head_dim;
+  if (in->dtype != FB_DT_BF16 && in->dtype != FB_DT_F16) return invalid("attn_prefill: bf16 or fp16");
+  if (dim != 64 && dim != 128) return invalid("attn_prefill: head_dim 64 or 128");
+  if (in->kv_heads < 1 || in->heads < in->kv_heads || in->heads % in->kv_heads || in->heads > 1024)
+    return invalid("attn_prefill: heads is a multiple of kv_heads, up to 1024");
+  if (tokens < 0 || n_seqs < 0) return invalid("attn_prefill: tokens or n_seqs is negative");
+  if (!tokens || !n_seqs) return 0;
+  if (!in->q || !in->k || !in->v || !out || !cu_seqlens) return invalid("attn_prefill: null argument");
+  if (in->q_stride < int64_t(in->heads) * dim || in->k_stride < int64_t(in->kv_heads) * dim ||
+      in->v_stride < int64_t(in->kv_heads) * dim || out_stride < int64_t(in->heads) * dim)
+    return invalid("attn_prefill: a stride is smaller than a token's heads");
+  if ((in->q_stride | in->k_stride | in->v_stride) >= int64_t(1) << 38) return invalid("attn_prefill: a stride is too large");
+  if ((reinterpret_cast<uintptr_t>(in->q) | reinterpret_cast<uintptr_t>(in->k) | reinterpret_cast<uintptr_t>(in->v) |
+       reinterpret_cast<uintptr_t>(out)) & 15 || (in->q_stride | in->k_stride | in->v_stride | out_stride) % 8)
+    return invalid("attn_prefill: tensors start on 16 bytes and tokens lie a multiple of 8 elements apart");
+  if ((reinterpret_cast<uintptr_t>(cu_seqlens) | reinterpret_cast<uintptr_t>(status)) & 3)
+    return invalid("attn_prefill: cu_seqlens or status is not aligned");
+  if (!(scale > 0.f && scale <= 1.0e30f)) return invalid("attn_prefill: scale is not positive and finite");
+  const int64_t items = tokens / kPfQueries + int64_t(n_seqs < tokens ? n_seqs : tokens);
+  if (items > 65535) return invalid("attn_prefill: more than 65535 blocks of 256 queries");
+  if (!pf_encode_fn()) {
+    set_error("attn_prefill: cuTensorMapEncodeTiled is not available");
+    return int32_t(cudaErrorNotSupported);
+  }
+  const bool bf = in->dtype == FB_DT_BF16;
+  PfMaps maps;
+  if (!pf_map(&maps.q, in->q, bf, dim, in->heads, tokens, in->q_stride) ||
+      !pf_map(&maps.k, in->k, bf, dim, in->kv_heads, tokens, in->k_stride) ||
+      !pf_map(&maps.v, in->v, bf, dim, in->kv_heads, tokens, in->v_stride))
+    return invalid("attn_prefill: cuTensorMapEncodeTiled failed");
+  PfArgs a;
+  a.out = out;
+  a.cu_seqlens = cu_seqlens;
+  a.status = status;
+  a.out_stride = out_stride;
+  a.scale_log2 = scale * 1.4426950408889634f;  // scores are kept in powers of two
+  a.n_seqs = n_seqs;
+  a.tokens = tokens;
+  a.group = in->heads / in->kv_heads;
+  const dim3 grid(unsigned(in->heads), unsigned(items));
+  cudaStream_t s = as_stream(stream);
+  const cudaError_t e = dim == 64 ? (bf ? launch_pf<__nv_bfloat16, 64>(a, maps, grid, s) : launch_pf<__half, 64>(a, maps, grid, s))
+                                  : (bf ? launch_pf<__nv_bfloat16, 128>(a, maps, grid, s) : launch_pf<__half, 128>(a, maps, grid, s));
+  const int32_t st = check_launch("attn_prefill");
+  return st ? st : int32_t(e);
+}
+
+}  // extern "C"

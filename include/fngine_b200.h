@@ -536,6 +536,17 @@ typedef struct fb_qkv_out {
 int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm, const fb_rope* rope, const fb_qkv_out* out,
                         void* stream);
 
+/* Causal attention over packed prompts: sequence s is the tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1 of q, k and v (device,
+ * [n_seqs + 1], not falling, within 0 .. tokens; empty sequences are allowed),
+ *   out_i = sum_{j <= i} softmax_j(scale q_i . k_j) v_j     over the tokens j of i's sequence, scale > 0;
+ * query head h reads key head h / (heads / kv_heads). out is [tokens][heads][head_dim] with its own stride; tokens outside
+ * of all sequences are left as they were. A sequence's result does not depend on what lies beside it; its own keys and values are to
+ * be finite. Softmax statistics and sums are fp32, the weights are rounded to the type of v; repeated calls are bitwise
+ * identical. cu_seqlens is read on the device. `status` (one device word, may be NULL) is set to FB_STATUS_PIPELINE_TIMEOUT when a bounded
+ * wait ran out. No workspace. head_dim 64 or 128; everything 16-byte aligned, strides multiples of 8 elements. */
+int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seqlens, int32_t n_seqs, float scale, void* out,
+                        int64_t out_stride, uint32_t* status, void* stream);
+
 /* A paged cache of keys and values: k and v [n_pages][page_size][kv_heads][head_dim], bf16 or fp16, 16-byte aligned. */
 typedef struct fb_kv_cache {
   const void* k;

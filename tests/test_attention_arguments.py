@@ -112,3 +112,25 @@ def test_how_tree_tiles_are_cut():
                     slot = 2 * b + (1 if max(begin, b * total // blocks) == begin else 0)
                     assert slots.setdefault(slot, s) == s and slot == (2 * first + 1 if b == first else 2 * b)
             begin += n
+
+
+def test_attn_prefill_refusals(fb_built):
+    lib = L.load()
+
+    def call(given={}, none=False, tokens=70, cu=4 * P, n_seqs=2, scale=0.1, out=5 * P, out_stride=1024, status=None):
+        q = dict(q=P, k=2 * P, v=3 * P, q_stride=1024, k_stride=256, v_stride=256, dtype=L.DT_BF16, heads=8, kv_heads=2, head_dim=128)
+        q.update(given)
+        return lib.fb_attn_prefill(None if none else C.byref(L.Qkv(**q)), tokens, cu, n_seqs, scale, out, out_stride, status, None), lib.fb_last_error_string()
+
+    for bad, word in [(dict(none=True), b"null"), (dict(given=dict(q=None)), b"null"), (dict(given=dict(k=None)), b"null"), (dict(given=dict(v=None)), b"null"),
+                      (dict(out=None), b"null"), (dict(cu=None), b"null"), (dict(given=dict(dtype=L.DT_F32)), b"bf16 or fp16"),
+                      (dict(given=dict(head_dim=256)), b"head_dim"), (dict(given=dict(heads=7)), b"multiple"), (dict(given=dict(kv_heads=0)), b"multiple"),
+                      (dict(given=dict(heads=0)), b"multiple"), (dict(given=dict(heads=1026)), b"multiple"), (dict(tokens=-1), b"negative"), (dict(n_seqs=-1), b"negative"),
+                      (dict(given=dict(q_stride=512)), b"stride"), (dict(given=dict(v_stride=248)), b"stride"), (dict(out_stride=1000), b"stride"),
+                      (dict(given=dict(k_stride=260)), b"16 bytes"), (dict(given=dict(q=P + 8)), b"16 bytes"), (dict(out=5 * P + 4), b"16 bytes"),
+                      (dict(given=dict(k_stride=2 ** 39)), b"too large"), (dict(cu=4 * P + 2), b"aligned"), (dict(status=P + 1), b"aligned"),
+                      (dict(scale=0.0), b"scale"), (dict(scale=-0.1), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(scale=float("inf")), b"scale"),
+                      (dict(tokens=2 ** 31 - 1), b"65535"), (dict(tokens=70000, n_seqs=70000), b"65535")]:
+        st, msg = call(**bad)
+        assert st == 1 and word in msg, (bad, st, msg)
+    assert call(tokens=0)[0] == 0 and call(n_seqs=0)[0] == 0
