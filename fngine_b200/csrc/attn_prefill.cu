@@ -14,8 +14,6 @@
 // Blocks are handed out longest first (causal: the last queries of a prompt have the most keys).
 #include "attn_common.cuh"
 
-#include <cuda.h>
-
 namespace fb {
 namespace {
 
@@ -45,81 +43,11 @@ struct PfMaps {
 };
 
 struct PfBars {
-  uint64_t q_full[2], s_full[2], p_full[2], o_done[2], full[8], empty[8], drained;  // 200 bytes
+  uint64_t q_full[2], s_full[2], p_full[2], o_done[2], full[8], empty[8], drained;
   uint32_t tmem;
   int aborted;
   int issued;  // copies of keys and values
 };
-
-__device__ __forceinline__ void pf_tma(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-                   dst),
-               "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-               : "memory");
-}
-__device__ __forceinline__ void pf_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void pf_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void pf_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void pf_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void pf_ld32(uint32_t taddr, float (&f)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
-        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void pf_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void pf_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void pf_st16(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-// Shared-memory operand descriptors, 128-byte swizzle, 8-row groups 1024 bytes apart, descriptor version 1. `lead`: for a
-// tile whose rows run along K (Q, K) not used (1); for V, whose rows run along N, the distance of its two 64-value parts.
-__device__ __forceinline__ uint64_t pf_desc(uint32_t addr, uint32_t lead) {
-  return uint64_t((addr & 0x3FFFFu) >> 4) | (uint64_t(lead) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
-         (uint64_t(2) << 61);
-}
-
-// Bounded wait. A wait that ran out is recorded, and every later one ends at once.
-__device__ __forceinline__ bool pf_wait(PfBars* bars, uint32_t* status, uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
-  for (uint32_t i = 0; i < (1u << 21); ++i) {
-    if (mbar_try_wait_hint(bar, parity)) return true;
-    if ((i & 63u) == 63u && *static_cast<volatile int*>(&bars->aborted)) return false;
-  }
-  *static_cast<volatile int*>(&bars->aborted) = 1;
-  if (status) atomicMax(status, uint32_t(FB_STATUS_PIPELINE_TIMEOUT));
-  return false;
-}
-
 static_assert(sizeof(PfBars) <= 256, "room behind the ring");
 
 template <class T, int D>
@@ -194,9 +122,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
     bars->issued = 0;
     mbar_fence_init();
   }
-  pf_fence_before();
+  tc_fence_before();
   __syncthreads();
-  pf_fence_after();
+  tc_fence_after();
   // (not before the allocation: a block of the next kernel that took tensor memory and then waited for this one would hold it up)
   pdl_launch_dependents();
   const uint32_t tmem = bars->tmem;
@@ -207,12 +135,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
     if (lane == 0) {
       auto tile = [&](uint8_t* dst, const CUtensorMap* map, int h, int row, uint64_t* bar) {
         mbar_expect_tx(bar, S::kTileBytes);
-        for (int p = 0; p < kParts; ++p) pf_tma(smem_u32(dst) + p * S::kHalf, map, p * 64, h, row, bar);
+        for (int p = 0; p < kParts; ++p) tma_load_3d(smem_u32(dst) + p * S::kHalf, map, p * 64, h, row, bar);
       };
       tile(q_tiles, &maps.q, head, start + row0, &bars->q_full[0]);
       for (int i = 0; i < 2 * blocks; ++i) {  // K_0 V_0 K_1 V_1 ...
         const int slot = i % kStages;
-        if (i >= kStages && !pf_wait(bars, a.status, &bars->empty[slot], uint32_t(i / kStages - 1) & 1)) break;
+        if (i >= kStages && !bounded_wait(&bars->aborted, a.status, &bars->empty[slot], uint32_t(i / kStages - 1) & 1)) break;
         tile(ring + slot * S::kTileBytes, i & 1 ? &maps.v : &maps.k, kv_head, start + (i >> 1) * kPfRows, &bars->full[slot]);
         bars->issued = i + 1;
         if (i == 0 && blocks1)
@@ -227,21 +155,21 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
     constexpr uint32_t kIdescPv = kIdesc | (uint32_t(D >> 3) << 17) | (1u << 16);  // V runs along N
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = ok && __all_sync(0xffffffffu, pf_wait(bars, a.status, bar, parity));
+      ok = ok && bounded_wait_warp(&bars->aborted, a.status, bar, parity);
     };
     auto scores = [&](int t, int j) {
       const int slot = (2 * j) % kStages;
       wait(&bars->full[slot], uint32_t(2 * j / kStages) & 1);
       if (!ok) return;
-      pf_fence_after();
+      tc_fence_after();
       if (elect_one()) {
-        const uint64_t qd = pf_desc(smem_u32(q_tiles + t * S::kTileBytes), 1), kd = pf_desc(smem_u32(ring + slot * S::kTileBytes), 1);
+        const uint64_t qd = umma_desc(smem_u32(q_tiles + t * S::kTileBytes), 1), kd = umma_desc(smem_u32(ring + slot * S::kTileBytes), 1);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t at = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
-          pf_mma_ss(tmem + kS + 128 * t, qd + at, kd + at, kIdescQk, k > 0);
+          umma_ss(tmem + kS + 128 * t, qd + at, kd + at, kIdescQk, k > 0);
         }
-        pf_commit(&bars->s_full[t]);
+        umma_commit(&bars->s_full[t]);
       }
       __syncwarp();
     };
@@ -262,18 +190,18 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
         __syncwarp();
         cleared = true;
       }
-      pf_fence_after();
+      tc_fence_after();
       if (elect_one()) {
-        const uint64_t vd = pf_desc(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
+        const uint64_t vd = umma_desc(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
 #pragma unroll
         for (int k = 0; k < kPfRows / 16; ++k)
-          pf_mma_ts(tmem + kO + 128 * t, tmem + kS + 128 * t + 8 * k, vd + k * (2048 >> 4), kIdescPv, j > 0 || k > 0);
-        pf_commit(&bars->o_done[t]);
+          umma_ts(tmem + kO + 128 * t, tmem + kS + 128 * t + 8 * k, vd + k * (2048 >> 4), kIdescPv, j > 0 || k > 0);
+        umma_commit(&bars->o_done[t]);
       }
       __syncwarp();
     };
     auto release = [&](int i) {
-      if (ok && elect_one()) pf_commit(&bars->empty[i % kStages]);
+      if (ok && elect_one()) umma_commit(&bars->empty[i % kStages]);
       __syncwarp();
     };
     wait(&bars->q_full[0], 0);
@@ -296,7 +224,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
       if (j + 1 < blocks) release(2 * j + 2);
     }
     // Nothing issued here is still running when the tensor memory is given back.
-    if (elect_one()) pf_commit(&bars->drained);
+    if (elect_one()) umma_commit(&bars->drained);
     __syncwarp();
     for (uint32_t n = 0; n < (1u << 16) && !__all_sync(0xffffffffu, mbar_try_wait_hint(&bars->drained, 0)); ++n) {}
   } else if (warp < 8) {
@@ -309,13 +237,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
     float top = -INFINITY, sum = 0.f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      ok = ok && __all_sync(0xffffffffu, pf_wait(bars, a.status, &bars->s_full[t], uint32_t(j) & 1));
+      ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->s_full[t], uint32_t(j) & 1);
       if (!ok) break;
-      pf_fence_after();
+      tc_fence_after();
       float s[4][32];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) pf_ld32(s_at + 32 * i, s[i]);
-      pf_ld_wait();
+      for (int i = 0; i < 4; ++i) tmem_ld32(s_at + 32 * i, s[i]);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_landed(s[i]);
       if (j == n - 1) {  // the diagonal
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -339,21 +269,22 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
         top = up;
         sum *= fade;
         if (j > 0) {
-          ok = __all_sync(0xffffffffu, pf_wait(bars, a.status, &bars->o_done[t], uint32_t(j - 1) & 1));
+          ok = bounded_wait_warp(&bars->aborted, a.status, &bars->o_done[t], uint32_t(j - 1) & 1);
           if (!ok) break;
-          pf_fence_after();
+          tc_fence_after();
 #pragma unroll 1
           for (int i = 0; i < D / 32; ++i) {
             float o[32];
-            pf_ld32(o_at + 32 * i, o);
-            pf_ld_wait();
+            tmem_ld32(o_at + 32 * i, o);
+            tmem_ld_wait();
+            tmem_landed(o);
             uint32_t r[32];
 #pragma unroll
             for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(o[c] * fade);
-            pf_st16(o_at + 32 * i, r);
-            pf_st16(o_at + 32 * i + 16, r + 16);
+            tmem_st16(o_at + 32 * i, r);
+            tmem_st16(o_at + 32 * i + 16, r + 16);
           }
-          pf_st_wait();
+          tmem_st_wait();
         }
       }
       const float base = top * a.scale_log2;
@@ -368,24 +299,25 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
           part[c & 3] += x + y;
           p[c] = pack2<T>(x, y);  // rounded to the type of v: half a step of each weight, averaged over the keys
         }
-        pf_st16(s_at + 16 * i, p);
+        tmem_st16(s_at + 16 * i, p);
       }
       sum += (part[0] + part[1]) + (part[2] + part[3]);
-      pf_st_wait();
-      pf_fence_before();
+      tmem_st_wait();
+      tc_fence_before();
       mbar_arrive(&bars->p_full[t]);
     }
-    if (n > 0 && ok) ok = __all_sync(0xffffffffu, pf_wait(bars, a.status, &bars->o_done[t], uint32_t(n - 1) & 1));
+    if (n > 0 && ok) ok = bounded_wait_warp(&bars->aborted, a.status, &bars->o_done[t], uint32_t(n - 1) & 1);
     if (n > 0 && ok) {
-      pf_fence_after();
+      tc_fence_after();
       // Through the query tile's memory, which nothing reads any more, to whole rows of 16-byte stores.
       const float inv = 1.f / sum;
       uint8_t* stage = q_tiles + t * S::kTileBytes + (warp & 3) * (32 * D * 2);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) {
         float o[32];
-        pf_ld32(o_at + 32 * i, o);
-        pf_ld_wait();
+        tmem_ld32(o_at + 32 * i, o);
+        tmem_ld_wait();
+        tmem_landed(o);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint4 v;
@@ -407,11 +339,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
           *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + int64_t(start + q) * a.out_stride + head * D + chunk * 8) = v;
         }
       }
-      pf_fence_before();
+      tc_fence_before();
     }
   }
   __syncthreads();
-  pf_fence_after();
+  tc_fence_after();
   if (bars->aborted && tid == 0) {  // copies that nobody waited for
     const int issued = bars->issued;
     for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
@@ -422,25 +354,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-using PfEncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-PfEncodeFn pf_encode_fn() {
-  static PfEncodeFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<PfEncodeFn>(p);
-  }();
-  return fn;
-}
 // [tokens][heads][dim] in boxes of 128 tokens x 64 values of one head; tokens behind the last one read as zeros.
 bool pf_map(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, int tokens, int64_t stride) {
   const cuuint64_t dims[3] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(tokens)};
   const cuuint64_t strides[2] = {cuuint64_t(dim) * 2, cuuint64_t(stride) * 2};
   const cuuint32_t box[3] = {64, 1, kPfRows}, elem[3] = {1, 1, 1};
-  return pf_encode_fn()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+  return encode_tiled_fn()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                         const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -484,7 +403,7 @@ int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seql
   if (!(scale > 0.f && scale <= 1.0e30f)) return invalid("attn_prefill: scale is not positive and finite");
   const int64_t items = tokens / kPfQueries + int64_t(n_seqs < tokens ? n_seqs : tokens);
   if (items > 65535) return invalid("attn_prefill: more than 65535 blocks of 256 queries");
-  if (!pf_encode_fn()) {
+  if (!encode_tiled_fn()) {
     set_error("attn_prefill: cuTensorMapEncodeTiled is not available");
     return int32_t(cudaErrorNotSupported);
   }

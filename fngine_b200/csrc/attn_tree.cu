@@ -1,113 +1,92 @@
-// Attention of a few drafted tokens per sequence over a paged cache (one token per sequence: plain decoding).
+// Attention of a few drafted tokens per sequence over a paged cache (one token per sequence: plain decoding), on tcgen05.
 //
 //   out[i] = sum_j softmax_j(scale q_i . k_j) v_j over the keys j that token i sees: all ctx keys of the context, and of the
 //   drafted tokens, whose keys follow the context's in the cache, those in its mask.
 //
-// Bound by the cache's bytes: each key and value is read once for all rows (tokens x query heads of a group) of a key head. Up to
-// 128 rows are a block's row tile; the tiles of keys of all (sequence, key head, row tile) segments are one sequence that is cut
+// Bound by the cache's bytes: each key and value is read once for all rows (tokens x query heads of a group) of a key head. The
+// rows, up to 128, are the lanes of the products' results in tensor memory, whether they are 4 or 128: a block of 128 keys costs the
+// tensor core 1024 cycles at head_dim 128 and a multiprocessor's share of the memory bandwidth 2800. (Products by mma.sync with
+// fragments in registers, 16 to 128 rows, were bound by the latencies of eight warps: 446 us for 32 sequences of up to 16384 keys
+// and four tokens, 87 for eight of 4096 and sixteen.)
+//   S = Q K^T   both operands in shared memory, two buffers of fp32 S: the next block's product runs under this one's softmax
+//   P = 2^(c S - c m) over S in the type of v, by a thread per row; only warps that hold rows read S
+//   O += P V    fp32 in tensor memory; multiplied only when a maximum rises by more than 2^8 above the one in use
+// Keys and values come by cp.async, 16 bytes a thread, from slots that a table look-up a block ahead has found: pages of any size, and
+// what is not to be read is written as zeros. (TMA gathers of four cache rows took 41 ns each per multiprocessor, 512 bytes: 919 us
+// for the 32 sequences.) The blocks of keys of all (sequence, key head, row tile) segments are one sequence that is cut
 // evenly over the multiprocessors, so that sequences of different lengths leave none of them idle, whatever lengths the
 // device finds (the host does not know them). A segment that several blocks share is joined by the last of them to arrive, in
-// block order: results do not depend on timing. Inside a block RW warps share the rows and 8 / RW the keys of a tile; with few rows
-// every warp has 16 keys of its own and the warps' running maxima, sums and outputs meet once per segment. Keys arrive by
-// cp.async some tiles ahead; the products are mma.sync m16n8k16: at 16 to 128 rows per key they need 2 to 13 % of what tcgen05
-// gives, and fragments in registers spare the trip of scores and weights through tensor memory.
+// block order: results do not depend on timing.
 #include "attn_common.cuh"
 
 namespace fb {
 namespace {
 
-constexpr int kTreeWarps = 8;
-constexpr int kTreeThreads = 32 * kTreeWarps;
+constexpr int kTreeThreads = 288;        // four softmax warps, four that copy, one that issues products
+constexpr int kTreeWarps = kTreeThreads / 32;
+constexpr int kTreeLag = 3;              // copies of tiles that a copying thread has in flight behind the one it announces
+constexpr int kTreeRows = 128;           // rows of a tile
+constexpr int kTreeKeys = 128;           // keys of a block
 constexpr int kTreeMaxDrafted = 64;
-constexpr int kTreeMaxSms = 256;  // partial results are sized for this many blocks
+constexpr int kTreeMaxSms = 256;         // partial results are sized for this many blocks
+constexpr float kTreeSlack = 8.f;        // how far (in powers of two) scores may rise above the maximum in use
 
 struct TreeArgs {
-  const void* q;
   void* out;
   const void* k;
   const void* v;
   const int32_t* table;
   const int32_t* contexts;
   const uint64_t* mask;
-  int64_t q_stride, out_stride;  // elements between tokens
-  int64_t n_pages;
+  int64_t out_stride;  // elements between tokens
   int64_t table_stride;
-  int32_t* counters;  // [segments]
-  float* partial;     // [2 * blocks][16 RW][D + 2]
+  uint32_t* status;
+  int32_t* counters;   // [segments]
+  float* partial;      // [2 * blocks]: outputs [128][D], maxima [128], sums [128]
   float scale_log2;
-  int n_seqs, drafted, kv_heads, group, page_size, page_shift, row_tiles;
+  int n_pages, n_seqs, drafted, kv_heads, group, page_size, page_shift;
+  int row_tiles, tile_tokens;  // row tiles per key head, drafted tokens per row tile
 };
-
-__device__ __forceinline__ void tree_cp16(uint32_t dst, const void* src, bool there) {
-  // (a source size of zero writes zeros and reads nothing)
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void tree_cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void tree_ldm(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-__device__ __forceinline__ void tree_ldm_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-template <class T>
-__device__ __forceinline__ void tree_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-template <int D, int RW>
+template <int D>
 struct TreeShape {
-  static constexpr int kKeys = RW <= 2 ? 128 : 64;  // keys per tile
-  static constexpr int kStages = RW <= 2 ? 3 : 4;
-  static constexpr int kKeyWarps = kTreeWarps / RW;
-  static constexpr int kWarpKeys = kKeys / kKeyWarps;
-  static constexpr int kTileBytes = kKeys * D * 2;
-  static constexpr int kMergeWords = (D / 2 + 4) * 32;  // a warp's outputs, maxima and sums
-  static constexpr int kMergeBytes = (kKeyWarps > 1 ? kTreeWarps / 2 : 1) * kMergeWords * 4;
-  static constexpr int kSmem = kStages * 2 * kTileBytes + kMergeBytes;
+  static constexpr int kTileBytes = kTreeKeys * D * 2;
+  static constexpr int kHalf = kTreeKeys * 128;  // a tile is D / 64 parts of 128 rows x 128 bytes
+  static constexpr int kStages = D == 128 ? 5 : 10;
+  static constexpr int kSmem = (2 + kStages) * kTileBytes + 1024 + 1536;
+  static constexpr int kSlot = (D + 2) * kTreeRows;  // floats of a partial result
 };
 
-// Walks through the tiles of the segments in their order.
+struct TreeBars {
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_done, full[10], empty[10], drained;
+  int64_t sums[kTreeWarps];
+  int64_t found[2];
+  int slots[2][kTreeKeys];  // cache slots of a key block, -1: zeros
+  uint32_t tmem;
+  int aborted;
+  int q_issued;
+  int last_block;
+};
+static_assert(sizeof(TreeBars) <= 1536, "room behind the ring");
+
+// Walks through the key blocks of the segments in their order.
 struct TreeCursor {
-  int seq, part, tile;       // part: key head * row tiles + row tile
-  int tiles, ctx, length;    // of the sequence
-  uint64_t seen;             // drafted tokens that some token of the sequence sees
+  int seq, part, tile;     // part: key head * row tiles + row tile
+  int tiles, ctx, length;  // of the sequence
 };
 
-template <class T, int D, int RW>
-__global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a) {
-  using S = TreeShape<D, RW>;
-  constexpr int kKeys = S::kKeys, kStages = S::kStages, kKeyWarps = S::kKeyWarps, kWarpKeys = S::kWarpKeys;
-  constexpr int kChunks = D / 8;                         // 16-byte chunks of a key
-  constexpr int kRowsPerPass = kTreeThreads / kChunks;   // keys per pass of the copying threads
-  constexpr int kPasses = kKeys / kRowsPerPass;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  float* merge = reinterpret_cast<float*>(smem + kStages * 2 * S::kTileBytes);
-  __shared__ int last_block;
-  __shared__ int64_t found[2];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int rw = warp / kKeyWarps, kw = warp % kKeyWarps;
-  const int parts = a.kv_heads * a.row_tiles, rows_all = a.drafted * a.group;
+template <class T, int D>
+__global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a, const __grid_constant__ CUtensorMap q_map) {
+  using S = TreeShape<D>;
+  constexpr int kStages = S::kStages, kParts = D / 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t* q_tiles = smem;
+  uint8_t* ring = smem + 2 * S::kTileBytes;
+  TreeBars* bars = reinterpret_cast<TreeBars*>(ring + kStages * S::kTileBytes);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int parts = a.kv_heads * a.row_tiles;
   const int64_t room = a.table_stride * a.page_size;  // keys that the table can hold
   pdl_wait_prior();
-  pdl_launch_dependents();
 
   auto length_of = [&](int seq, int* ctx) {
     int c = a.contexts[seq];
@@ -117,34 +96,45 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a)
     const int64_t n = int64_t(c) + a.drafted;
     return int(n < room ? n : room);
   };
+  auto blocks_of = [](int length) { return length > kTreeKeys ? (length + kTreeKeys - 1) / kTreeKeys : 1; };
   auto tiles_of = [&](int seq) {
     int c;
-    const int n = (length_of(seq, &c) + kKeys - 1) / kKeys;
-    return n > 0 ? n : 1;
+    return blocks_of(length_of(seq, &c));
   };
 
-  // All tiles, and the sequence that this block's first one lies in.
-  int64_t total = 0;
-  {
-    int64_t* sums = reinterpret_cast<int64_t*>(merge);
+  // All key blocks, and the sequence that this block's first one lies in.
+  int64_t total = 0, begin = 0, end = 0, seq_begin = 0;
+  int blocks = 0, first_seq = 0;
+  if (a.n_seqs <= 32) {  // every warp for itself
+    const int64_t n = lane < a.n_seqs ? int64_t(tiles_of(lane)) * parts : 0;
+    int64_t upto = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += other;
+    }
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    blocks = int(total < int64_t(gridDim.x) ? total : int64_t(gridDim.x));
+    if (int(blockIdx.x) >= blocks) return;
+    begin = int64_t(blockIdx.x) * total / blocks;
+    const uint32_t who = __ballot_sync(0xffffffffu, n && upto > begin && upto - n <= begin);
+    first_seq = __ffs(who) - 1;
+    seq_begin = __shfl_sync(0xffffffffu, upto - n, first_seq);
+  } else {
     int64_t mine = 0;
     for (int s = tid; s < a.n_seqs; s += kTreeThreads) mine += tiles_of(s);
 #pragma unroll
     for (int m = 16; m; m >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, m);
-    if (lane == 0) sums[warp] = mine;
+    if (lane == 0) bars->sums[warp] = mine;
     __syncthreads();
-    for (int w = 0; w < kTreeWarps; ++w) total += sums[w];
+    for (int w = 0; w < kTreeWarps; ++w) total += bars->sums[w];
     __syncthreads();
-  }
-  total *= parts;
-  const int blocks = int(total < int64_t(gridDim.x) ? total : int64_t(gridDim.x));
-  if (int(blockIdx.x) >= blocks) return;
-  const int64_t begin = int64_t(blockIdx.x) * total / blocks, end = int64_t(blockIdx.x + 1) * total / blocks;
-  int64_t seq_begin = 0;  // first tile of the sequence of the products' cursor
-  {
-    int64_t* sums = reinterpret_cast<int64_t*>(merge);
+    total *= parts;
+    blocks = int(total < int64_t(gridDim.x) ? total : int64_t(gridDim.x));
+    if (int(blockIdx.x) >= blocks) return;
+    begin = int64_t(blockIdx.x) * total / blocks;
     int64_t before = 0;
-    for (int base = 0; base < a.n_seqs; base += kTreeThreads) {
+    for (int base = 0; base < a.n_seqs && before <= begin; base += kTreeThreads) {
       const int s = base + tid;
       const int64_t n = s < a.n_seqs ? int64_t(tiles_of(s)) * parts : 0;
       int64_t upto = n;
@@ -153,358 +143,463 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a)
         const int64_t other = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += other;
       }
-      if (lane == 31) sums[warp] = upto;
+      if (lane == 31) bars->sums[warp] = upto;
       __syncthreads();
       int64_t all = 0;
       for (int w = 0; w < kTreeWarps; ++w) {
-        if (w < warp) upto += sums[w];
-        all += sums[w];
+        if (w < warp) upto += bars->sums[w];
+        all += bars->sums[w];
       }
       if (n && before + upto > begin && before + upto - n <= begin) {
-        found[0] = s;
-        found[1] = before + upto - n;
+        bars->found[0] = s;
+        bars->found[1] = before + upto - n;
       }
       before += all;
       __syncthreads();
-      if (before > begin) break;
     }
+    first_seq = int(bars->found[0]);
+    seq_begin = bars->found[1];
   }
-  auto enter = [&](TreeCursor& c) {
-    c.length = length_of(c.seq, &c.ctx);
-    const int n = (c.length + kKeys - 1) / kKeys;
-    c.tiles = n > 0 ? n : 1;
-    c.seen = 0;
-    if (a.mask) {
-      uint64_t m = 0;
-      for (int i = lane; i < a.drafted; i += 32) m |= a.mask[int64_t(c.seq) * a.drafted + i];
-      const uint32_t lo = __reduce_or_sync(0xffffffffu, uint32_t(m)), hi = __reduce_or_sync(0xffffffffu, uint32_t(m >> 32));
-      c.seen = (uint64_t(hi) << 32) | lo;
-    } else {
-      c.seen = ~0ull;
-    }
-  };
+  end = int64_t(blockIdx.x + 1) * total / blocks;
+  const int n_tiles = int(end - begin);
+
+  TreeCursor now;
+  now.seq = first_seq;
+  now.length = length_of(now.seq, &now.ctx);
+  now.tiles = blocks_of(now.length);
+  now.part = int((begin - seq_begin) / now.tiles);
+  now.tile = int((begin - seq_begin) % now.tiles);
   auto advance = [&](TreeCursor& c) {  // true: a new segment
     if (++c.tile < c.tiles) return false;
     c.tile = 0;
     if (++c.part == parts) {
       c.part = 0;
-      ++c.seq;
-      if (c.seq < a.n_seqs) enter(c);
+      if (++c.seq < a.n_seqs) {
+        c.length = length_of(c.seq, &c.ctx);
+        c.tiles = blocks_of(c.length);
+      }
     }
     return true;
   };
 
-  TreeCursor now;
-  now.seq = int(found[0]);
-  seq_begin = found[1];
-  enter(now);
-  now.part = int((begin - seq_begin) / now.tiles);
-  now.tile = int((begin - seq_begin) % now.tiles);
-  TreeCursor ahead = now;
-  const int n_tiles = int(end - begin);
-
-  // Page numbers of the tile to be copied next: asked for a tile before they are used.
-  const int my_chunk = tid % kChunks, my_row = tid / kChunks;
-  int pages[kPasses];
-  auto ask = [&] {
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-      const int key = ahead.tile * kKeys + i * kRowsPerPass + my_row;
-      const int d = key - ahead.ctx;
-      const bool seen = key < ahead.length && (d < 0 || ((ahead.seen >> (d & 63)) & 1));
-      const int index = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
-      pages[i] = seen ? a.table[ahead.seq * a.table_stride + index] : -1;
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->q_full[i], 1);
+      mbar_init(&bars->q_empty[i], 1);
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_full[i], kTreeRows);
     }
-  };
-  const uint32_t ring = smem_u32(smem);
-  const size_t key_elems = size_t(a.kv_heads) * D;
-  int asked = 0, put_stage = 0;
-  auto copy = [&] {
-    if (asked < n_tiles) {
-      const uint32_t stage = ring + put_stage * (2 * S::kTileBytes);
-      const size_t head = size_t(ahead.part / a.row_tiles) * D + my_chunk * 8;
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int row = i * kRowsPerPass + my_row, key = ahead.tile * kKeys + row;
-        const int index = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
-        // A page outside of the cache reads as zeros, as does a drafted token that nobody sees.
-        const bool there = pages[i] >= 0 && pages[i] < a.n_pages;
-        const size_t at = there ? (size_t(pages[i]) * a.page_size + size_t(key - index * a.page_size)) * key_elems + head : 0;
-        const uint32_t dst = stage + row * (D * 2) + ((my_chunk ^ (row & 7)) << 4);
-        tree_cp16(dst, static_cast<const T*>(a.k) + at, there);
-        tree_cp16(dst + S::kTileBytes, static_cast<const T*>(a.v) + at, there);
+    mbar_init(&bars->o_done, 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bars->full[i], kTreeKeys);
+      mbar_init(&bars->empty[i], 1);
+    }
+    mbar_init(&bars->drained, 1);
+    bars->aborted = 0;
+    bars->q_issued = 0;
+    mbar_fence_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // (not before the allocation: a block of the next kernel that took tensor memory and then waited for this one would hold it up)
+  pdl_launch_dependents();
+  const uint32_t tmem = bars->tmem;
+  constexpr uint32_t kS = 0, kO = 256;  // S of an even and an odd key block, outputs
+
+  if (warp >= 4 && warp < 8) {
+    // ------------------------------------------------------------------ copies
+    const int me = tid - 128;  // looks up key `me` of a block
+    uint64_t seen = 0;         // drafted tokens that some token of the sequence sees
+    auto look = [&](int seq) {
+      seen = ~0ull;
+      if (!a.mask) return;
+      uint64_t m = 0;
+      for (int i = lane; i < a.drafted; i += 32) m |= a.mask[int64_t(seq) * a.drafted + i];
+      const uint32_t lo = __reduce_or_sync(0xffffffffu, uint32_t(m)), hi = __reduce_or_sync(0xffffffffu, uint32_t(m >> 32));
+      seen = (uint64_t(hi) << 32) | lo;
+    };
+    int page = -1;  // of the block to be copied next
+    auto ask = [&] {
+      const int key = now.tile * kTreeKeys + me, d = key - now.ctx;
+      const bool read = key < now.length && (d < 0 || ((seen >> (d & 63)) & 1));
+      const int index = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+      page = read ? a.table[now.seq * a.table_stride + index] : -1;
+    };
+    constexpr int kChunks = D / 8, kPerPass = kTreeKeys / kChunks, kPasses = kTreeKeys / kPerPass;
+    const int chunk = me % kChunks, row = me / kChunks;
+    const uint32_t put = uint32_t((chunk / 8) * S::kHalf + ((((chunk & 7) ^ (row & 7)) << 4) + row * 128));
+    const size_t slot_values = size_t(a.kv_heads) * D;
+    static_assert(kPerPass % 8 == 0, "a thread's rows have one place in their 128-byte swizzle");
+    look(now.seq);
+    ask();
+    bool ok = true, fresh = true;
+    int segment = 0;
+    // (after a wait that ran out the loop goes on without copies: all four warps meet at the same barriers)
+    for (int it = 0; it < n_tiles; ++it) {
+      const int head = now.part / a.row_tiles;
+      if (fresh) {
+        const int b = segment & 1;
+        if (segment >= 2) ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->q_empty[b], uint32_t(segment / 2 - 1) & 1);
+        if (ok && me == 0) {
+          const int token = now.seq * a.drafted + (now.part % a.row_tiles) * a.tile_tokens;
+          mbar_expect_tx(&bars->q_full[b], uint32_t(a.tile_tokens * a.group) * D * 2);
+          for (int p = 0; p < kParts; ++p)
+            tma_load_3d(smem_u32(q_tiles + b * S::kTileBytes) + p * S::kHalf, &q_map, p * 64, head * a.group, token, &bars->q_full[b]);
+          bars->q_issued = segment + 1;
+        }
+        ++segment;
       }
-      ++asked;
-      if (asked < n_tiles) {
-        advance(ahead);
+      {
+        const int key = now.tile * kTreeKeys + me, index = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+        // A page outside of the cache reads as zeros, as does a drafted token that nobody sees.
+        bars->slots[it & 1][me] = page >= 0 && page < a.n_pages ? page * a.page_size + (key - index * a.page_size) : -1;
+      }
+      if (it + 1 < n_tiles) {
+        const int seq = now.seq;
+        fresh = advance(now);
+        if (now.seq != seq) look(now.seq);
         ask();
       }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    put_stage = put_stage + 1 == kStages ? 0 : put_stage + 1;
-  };
-  ask();
-  for (int i = 0; i < kStages - 1; ++i) copy();
-
-  uint32_t qf[D / 16][4];
-  float o[D / 8][4], m_run[2], l_run[2];
-  uint64_t row_mask[2];
-  auto begin_segment = [&] {
-    const int head0 = (now.part / a.row_tiles) * a.group, row0 = (now.part % a.row_tiles) * (16 * RW) + rw * 16;
+      warps_sync(2, kTreeKeys);
+      const int* slots = &bars->slots[it & 1][row];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = row0 + g + 8 * i, token = row / a.group, head = head0 + row - token * a.group;
-      const bool real = row < rows_all;
-      const T* p = static_cast<const T*>(a.q) + (int64_t(now.seq) * a.drafted + token) * a.q_stride + head * D;
+      for (int kv = 0; kv < 2; ++kv) {
+        const int i = 2 * it + kv, at = i % kStages;
+        if (i >= kStages) ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->empty[at], uint32_t(i / kStages - 1) & 1);
+        if (ok) {
+          const T* from = static_cast<const T*>(kv ? a.v : a.k) + head * D + chunk * 8;
+          const uint32_t dst = smem_u32(ring + at * S::kTileBytes) + put;
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        qf[kk][i] = real ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 2 * t) : 0u;
-        qf[kk][i + 2] = real ? *reinterpret_cast<const uint32_t*>(p + kk * 16 + 8 + 2 * t) : 0u;
-      }
-      row_mask[i] = !real ? 0 : a.mask ? a.mask[int64_t(now.seq) * a.drafted + token]
-                                       : token == 63 ? ~0ull : (2ull << token) - 1;
-      m_run[i] = -INFINITY;
-      l_run[i] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-  };
-  begin_segment();
-
-  int stage_at = 0;
-  int64_t piece_begin = begin;
-  const int lr = (lane & 7) + ((lane >> 4) & 1) * 8, lc = (lane >> 3) & 1;    // K: keys 0-7 | 8-15 by chunk c | c + 1
-  const int vr = (lane & 7) + ((lane >> 3) & 1) * 8, vc = (lane >> 4) & 1;    // V: chunk c | c + 1 by keys 0-7 | 8-15
-  for (int it = 0; it < n_tiles; ++it) {
-    tree_cp_wait<kStages - 2>();
-    __syncthreads();
-    copy();
-    const uint32_t ks = ring + stage_at * (2 * S::kTileBytes) + kw * kWarpKeys * (D * 2), vs = ks + S::kTileBytes;
-    stage_at = stage_at + 1 == kStages ? 0 : stage_at + 1;
-
-    float s[kWarpKeys / 8][4];
-#pragma unroll
-    for (int i = 0; i < kWarpKeys / 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-#pragma unroll
-      for (int n2 = 0; n2 < kWarpKeys / 16; ++n2) {
-        uint32_t b[4];
-        const int row = n2 * 16 + lr;
-        tree_ldm(b, ks + row * (D * 2) + (((2 * kk + lc) ^ (row & 7)) << 4));
-        tree_mma<T>(s[2 * n2], qf[kk], b[0], b[1]);
-        tree_mma<T>(s[2 * n2 + 1], qf[kk], b[2], b[3]);
-      }
-    }
-    const int key0 = now.tile * kKeys + kw * kWarpKeys;
-    if (key0 + kWarpKeys > now.ctx) {
-#pragma unroll
-      for (int n = 0; n < kWarpKeys / 8; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int key = key0 + n * 8 + 2 * t + (j & 1), d = key - now.ctx;
-          const bool sees = key < now.length && (d < 0 || ((row_mask[j >> 1] >> (d & 63)) & 1));
-          if (!sees) s[n][j] = -INFINITY;
-        }
-    }
-    float base[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float m = m_run[i];
-#pragma unroll
-      for (int n = 0; n < kWarpKeys / 8; ++n) m = fmaxf(m, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      base[i] = m == -INFINITY ? 0.f : m * a.scale_log2;  // a row that has seen nothing yet
-      const float fade = exp2_approx(m_run[i] * a.scale_log2 - base[i]);
-      m_run[i] = m;
-      l_run[i] *= fade;
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        o[n][2 * i] *= fade;
-        o[n][2 * i + 1] *= fade;
-      }
-    }
-#pragma unroll
-    for (int n2 = 0; n2 < kWarpKeys / 16; ++n2) {
-      float p[2][4];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          p[h][j] = exp2_approx(fmaf(s[2 * n2 + h][j], a.scale_log2, -base[j >> 1]));
-          l_run[j >> 1] += p[h][j];
-        }
-      // Weights are rounded to the type of v: half a step of them each, averaged over the keys.
-      const uint32_t pf[4] = {pack2<T>(p[0][0], p[0][1]), pack2<T>(p[0][2], p[0][3]), pack2<T>(p[1][0], p[1][1]),
-                              pack2<T>(p[1][2], p[1][3])};
-#pragma unroll
-      for (int n = 0; n < D / 16; ++n) {
-        uint32_t b[4];
-        const int row = n2 * 16 + vr;
-        tree_ldm_trans(b, vs + row * (D * 2) + (((2 * n + vc) ^ (row & 7)) << 4));
-        tree_mma<T>(o[2 * n], pf, b[0], b[1]);
-        tree_mma<T>(o[2 * n + 1], pf, b[2], b[3]);
-      }
-    }
-
-    const int64_t at = begin + it;  // this tile
-    const bool segment_ends = now.tile + 1 == now.tiles;
-    if (segment_ends || it + 1 == n_tiles) {
-      const int64_t segment_begin = seq_begin + int64_t(now.part) * now.tiles;
-      // Sums of the four lanes that share a row.
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
-        l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
-      }
-      // The warps that share rows meet pairwise.
-#pragma unroll
-      for (int half = kKeyWarps / 2; half > 0; half >>= 1) {
-        float* slot = merge + (rw * (kKeyWarps / 2) + (kw % half)) * S::kMergeWords + lane;
-        if (kw >= half && kw < 2 * half) {
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) slot[(4 * i + j) * 32] = o[i][j];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            slot[(D / 2 + i) * 32] = m_run[i];
-            slot[(D / 2 + 2 + i) * 32] = l_run[i];
+          for (int p = 0; p < kPasses; ++p) {
+            const int slot = slots[p * kPerPass];
+            const T* src = from + size_t(slot < 0 ? 0 : slot) * slot_values;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + p * (kPerPass * 128)), "l"(src), "r"(slot < 0 ? 0 : 16)
+                         : "memory");
           }
         }
-        __syncthreads();
-        if (kw < half) {
-          float mine[2], theirs[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float m2 = slot[(D / 2 + i) * 32], l2 = slot[(D / 2 + 2 + i) * 32], m = fmaxf(m_run[i], m2);
-            const float b = m == -INFINITY ? 0.f : m;
-            mine[i] = exp2_approx((m_run[i] - b) * a.scale_log2);
-            theirs[i] = exp2_approx((m2 - b) * a.scale_log2);
-            m_run[i] = m;
-            l_run[i] = l_run[i] * mine[i] + l2 * theirs[i];
-          }
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              o[i][j] = o[i][j] * mine[j >> 1] + slot[(4 * i + j) * 32] * theirs[j >> 1];
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (i >= kTreeLag) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kTreeLag) : "memory");
+          fence_proxy_async();  // (the products read shared memory through the other proxy)
+          mbar_arrive(&bars->full[(i - kTreeLag) % kStages]);
         }
-        __syncthreads();
       }
-      const bool whole = piece_begin == segment_begin && segment_ends;
-      const int head0 = (now.part / a.row_tiles) * a.group, row0 = (now.part % a.row_tiles) * (16 * RW);
-      if (whole) {
-        if (kw == 0) {
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    fence_proxy_async();
+    for (int i = 2 * n_tiles > kTreeLag ? 2 * n_tiles - kTreeLag : 0; i < 2 * n_tiles; ++i) mbar_arrive(&bars->full[i % kStages]);
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ products
+    constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kTreeRows >> 4) << 24);
+    constexpr uint32_t kIdescQk = kIdesc | (uint32_t(kTreeKeys >> 3) << 17);
+    constexpr uint32_t kIdescPv = kIdesc | (uint32_t(D >> 3) << 17) | (1u << 16);  // V runs along N
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      ok = ok && bounded_wait_warp(&bars->aborted, a.status, bar, parity);
+    };
+    TreeCursor next = now;  // of the scores, a block ahead of the outputs
+    int segment = 0;
+    auto scores = [&](int it, bool first) {
+      const int slot = (2 * it) % kStages, b = segment & 1;
+      if (first) wait(&bars->q_full[b], uint32_t(segment / 2) & 1);
+      wait(&bars->full[slot], uint32_t(2 * it / kStages) & 1);
+      const bool last = next.tile + 1 == next.tiles;
+      if (ok) {
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t qd = umma_desc(smem_u32(q_tiles + b * S::kTileBytes), 1), kd = umma_desc(smem_u32(ring + slot * S::kTileBytes), 1);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int row = row0 + rw * 16 + g + 8 * i;
-            if (row >= rows_all) continue;
-            const int token = row / a.group, head = head0 + row - token * a.group;
-            const float inv = l_run[i] > 0.f || l_run[i] != l_run[i] ? 1.f / l_run[i] : 0.f;  // a row that sees nothing: zeros
-            T* p = static_cast<T*>(a.out) + (int64_t(now.seq) * a.drafted + token) * a.out_stride + head * D;
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
+            umma_ss(tmem + kS + 128 * (it & 1), qd + at, kd + at, kIdescQk, k > 0);
+          }
+          umma_commit(&bars->s_full[it & 1]);
+          umma_commit(&bars->empty[slot]);
+          if (last) umma_commit(&bars->q_empty[b]);
+        }
+        __syncwarp();
+      }
+      if (last) ++segment;
+    };
+    scores(0, true);
+    bool first = true;  // block of its segment, in this block's share
+    for (int it = 0; it < n_tiles && ok; ++it) {
+      bool next_first = false;
+      if (it + 1 < n_tiles) {
+        next_first = advance(next);
+        scores(it + 1, next_first);
+      }
+      const int slot = (2 * it + 1) % kStages;
+      wait(&bars->p_full[it & 1], uint32_t(it >> 1) & 1);
+      wait(&bars->full[slot], uint32_t((2 * it + 1) / kStages) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t vd = umma_desc(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-              *reinterpret_cast<uint32_t*>(p + n * 8 + 2 * t) = pack2<T>(o[n][2 * i] * inv, o[n][2 * i + 1] * inv);
+        for (int k = 0; k < kTreeKeys / 16; ++k)
+          umma_ts(tmem + kO, tmem + kS + 128 * (it & 1) + 8 * k, vd + k * (2048 >> 4), kIdescPv, !first || k > 0);
+        umma_commit(&bars->o_done);
+        umma_commit(&bars->empty[slot]);
+      }
+      __syncwarp();
+      first = next_first;
+    }
+    // Nothing issued here is still running when the tensor memory is given back.
+    if (elect_one()) umma_commit(&bars->drained);
+    __syncwarp();
+    for (uint32_t n = 0; n < (1u << 16) && !__all_sync(0xffffffffu, mbar_try_wait_hint(&bars->drained, 0)); ++n) {}
+  } else {
+    // ------------------------------------------------------------------ softmax: thread = row
+    const uint32_t lanes = uint32_t(warp) << 21;  // (32 warp) << 16
+    const uint32_t o_at = tmem + lanes + kO;
+    bool ok = true, fresh = true;
+    float top = -INFINITY, sum = 0.f;
+    int head0 = 0, token = 0, rows = 0, head = 0;
+    uint64_t sees = 0;
+    int64_t piece_begin = begin;
+    for (int it = 0; it < n_tiles; ++it) {
+      if (fresh) {
+        top = -INFINITY;
+        sum = 0.f;
+        const int token0 = (now.part % a.row_tiles) * a.tile_tokens;
+        const int tokens = a.drafted - token0 < a.tile_tokens ? a.drafted - token0 : a.tile_tokens;
+        rows = tokens * a.group;
+        head0 = (now.part / a.row_tiles) * a.group;
+        token = token0 + tid / a.group;
+        head = head0 + tid % a.group;
+        sees = 0;
+        if (tid < rows) sees = a.mask ? a.mask[int64_t(now.seq) * a.drafted + token] : token == 63 ? ~0ull : (2ull << token) - 1;
+        const int there = now.length - now.ctx;  // drafted tokens that the table has room for
+        if (there < 64) sees &= (1ull << there) - 1;
+      }
+      const bool segment_ends = now.tile + 1 == now.tiles;
+      // (after a wait that ran out the loop goes on without work: all four warps meet at the same barriers)
+      ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->s_full[it & 1], uint32_t(it >> 1) & 1);
+      if (ok && 32 * warp < rows) {
+        tc_fence_after();
+        const uint32_t s_at = tmem + lanes + kS + 128 * (it & 1);
+        float s[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld32(s_at + 32 * i, s[i]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_landed(s[i]);
+        const int off = now.ctx - now.tile * kTreeKeys;  // first column behind the context
+        if (off < kTreeKeys) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int sh = off - 32 * i;  // bit of this word that drafted token 0 has
+            uint32_t bits;
+            if (sh >= 32) bits = 0xffffffffu;
+            else if (sh >= 0) bits = uint32_t(sees << sh) | ((1u << sh) - 1u);
+            else bits = -sh < 64 ? uint32_t(sees >> -sh) : 0u;
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (!((bits >> c) & 1)) s[i][c] = -INFINITY;
           }
         }
-      } else {
-        constexpr size_t kSlot = size_t(16 * RW) * (D + 2);
+        float m[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          m[i] = s[i][0];
+#pragma unroll
+          for (int c = 1; c < 32; ++c) m[i] = fmaxf(m[i], s[i][c]);
+        }
+        const float latest = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+        // (no for a row that has seen nothing yet; rows behind the last one are nobody's and decide nothing)
+        const bool rises = tid < rows && (latest - top) * a.scale_log2 > kTreeSlack;
+        if (__any_sync(0xffffffffu, rises)) {
+          const float up = fmaxf(latest, top);
+          const float fade = up == -INFINITY ? 1.f : exp2_approx((top - up) * a.scale_log2);
+          top = up;
+          sum *= fade;
+          if (!fresh) {
+            ok = bounded_wait_warp(&bars->aborted, a.status, &bars->o_done, uint32_t(it - 1) & 1);
+            tc_fence_after();
+#pragma unroll 1
+            for (int i = 0; i < D / 32; ++i) {
+              float o[32];
+              tmem_ld32(o_at + 32 * i, o);
+              tmem_ld_wait();
+              tmem_landed(o);
+              uint32_t r[32];
+#pragma unroll
+              for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(o[c] * fade);
+              tmem_st16(o_at + 32 * i, r);
+              tmem_st16(o_at + 32 * i + 16, r + 16);
+            }
+            tmem_st_wait();
+          }
+        }
+        const float base = top == -INFINITY ? 0.f : top * a.scale_log2;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t p[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float x = exp2_approx(fmaf(s[i][2 * c], a.scale_log2, -base));
+            const float y = exp2_approx(fmaf(s[i][2 * c + 1], a.scale_log2, -base));
+            part[c & 3] += x + y;
+            p[c] = pack2<T>(x, y);  // rounded to the type of v: half a step of each weight, averaged over the keys
+          }
+          tmem_st16(s_at + 16 * i, p);
+        }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        tmem_st_wait();
+        tc_fence_before();
+      }
+      // Where the outputs are read next, the block before has to be known done, and while the barrier cannot be two phases on: the
+      // scores of this block only say that the block before that one is.
+      const bool piece_ends = segment_ends || it + 1 == n_tiles;
+      if (piece_ends && it) ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->o_done, uint32_t(it - 1) & 1);
+      mbar_arrive(&bars->p_full[it & 1]);
+      fresh = false;
+
+      if (piece_ends) {
+        const int64_t segment_begin = seq_begin + int64_t(now.part) * now.tiles;
+        const bool whole = piece_begin == segment_begin && segment_ends;
+        ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->o_done, uint32_t(it) & 1);
+        tc_fence_after();
         // A block has at most two pieces that are not whole: one that begins with its segment, one that does not.
-        float* mine = a.partial + (2 * size_t(blockIdx.x) + (piece_begin == segment_begin ? 1 : 0)) * kSlot;
-        if (kw == 0) {
+        float* mine = a.partial + (2 * size_t(blockIdx.x) + (piece_begin == segment_begin ? 1 : 0)) * S::kSlot;
+        if (ok && 32 * warp < rows) {
+          const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;  // a row that sees nothing: zeros
+          T* to = static_cast<T*>(a.out) + (int64_t(now.seq) * a.drafted + token) * a.out_stride + int64_t(head) * D;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int row = rw * 16 + g + 8 * i;
-            if (t == 0) {
-              mine[row] = m_run[i];
-              mine[16 * RW + row] = l_run[i];
+          for (int i = 0; i < D / 32; ++i) {
+            float o[32];
+            tmem_ld32(o_at + 32 * i, o);
+            tmem_ld_wait();
+            tmem_landed(o);
+            if (whole) {
+              if (tid < rows) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  uint4 v;
+                  v.x = pack2<T>(o[8 * c] * inv, o[8 * c + 1] * inv);
+                  v.y = pack2<T>(o[8 * c + 2] * inv, o[8 * c + 3] * inv);
+                  v.z = pack2<T>(o[8 * c + 4] * inv, o[8 * c + 5] * inv);
+                  v.w = pack2<T>(o[8 * c + 6] * inv, o[8 * c + 7] * inv);
+                  *reinterpret_cast<uint4*>(to + 32 * i + 8 * c) = v;
+                }
+              }
+            } else if (tid < rows) {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<float4*>(mine + tid * D + 32 * i + 4 * c) = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
             }
-            float* p = mine + 32 * RW + row * D + 2 * t;
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(p + n * 8) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+            __syncwarp();  // (the next read of tensor memory takes the whole warp)
           }
+          if (!whole) {
+            mine[D * kTreeRows + tid] = top;
+            mine[(D + 1) * kTreeRows + tid] = sum;
+          }
+          tc_fence_before();
         }
-        __threadfence();
-        __syncthreads();
-        const int64_t segment_end = segment_begin + now.tiles;
-        const int first = int(((segment_begin + 1) * blocks - 1) / total), last = int((segment_end * blocks - 1) / total);
-        int32_t* counter = a.counters + int64_t(now.seq) * parts + now.part;
-        if (tid == 0) {
-          last_block = atomicAdd(counter, 1) == last - first;
-          if (last_block) *counter = 0;  // for the next call
-        }
-        __syncthreads();
-        if (last_block) {
+        if (!whole) {
           __threadfence();
-          const float* head_piece = a.partial + (2 * size_t(first) + 1) * kSlot;
-          for (int i = tid; i < 16 * RW * (D / 4); i += kTreeThreads) {
-            const int r = i / (D / 4), c = 4 * (i % (D / 4)), row = row0 + r;
-            if (row >= rows_all) break;
-            float m = -INFINITY, l = 0.f;
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int b = first; b <= last; ++b) {
-              const float* piece = b == first ? head_piece : a.partial + 2 * size_t(b) * kSlot;
-              const float m2 = __ldcg(piece + r), l2 = __ldcg(piece + 16 * RW + r);
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(piece + 32 * RW + r * D + c));
-              const float top = fmaxf(m, m2), zero = top == -INFINITY ? 0.f : top;
-              const float f1 = exp2_approx((m - zero) * a.scale_log2), f2 = exp2_approx((m2 - zero) * a.scale_log2);
-              m = top;
-              l = l * f1 + l2 * f2;
-              sum.x = sum.x * f1 + x.x * f2;
-              sum.y = sum.y * f1 + x.y * f2;
-              sum.z = sum.z * f1 + x.z * f2;
-              sum.w = sum.w * f1 + x.w * f2;
+          warps_sync(1, kTreeRows);
+          const int64_t segment_end = segment_begin + now.tiles;
+          const int first = int(((segment_begin + 1) * blocks - 1) / total), last = int((segment_end * blocks - 1) / total);
+          if (tid == 0) {
+            int32_t* counter = a.counters + int64_t(now.seq) * parts + now.part;
+            bars->last_block = atomicAdd(counter, 1) == last - first;
+            if (bars->last_block) *counter = 0;  // for the next call
+          }
+          warps_sync(1, kTreeRows);
+          if (bars->last_block) {
+            __threadfence();
+            const int64_t token0 = int64_t(now.seq) * a.drafted + (now.part % a.row_tiles) * a.tile_tokens;
+            for (int i = tid; i < rows * (D / 4); i += kTreeRows) {
+              const int r = i / (D / 4), c = 4 * (i % (D / 4));
+              // Piece b of the segment is block b's: the first begins with the segment, the others do not.
+              const float* piece = a.partial + (2 * size_t(first) + 1) * S::kSlot;
+              float up = __ldcg(piece + D * kTreeRows + r);
+#pragma unroll 4
+              for (int b = first + 1; b <= last; ++b) up = fmaxf(up, __ldcg(a.partial + 2 * size_t(b) * S::kSlot + D * kTreeRows + r));
+              if (up == -INFINITY) up = 0.f;  // a row that sees nothing
+              float l = 0.f;
+              float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+              for (int b = first; b <= last; ++b) {
+                piece = a.partial + (2 * size_t(b) + (b == first ? 1 : 0)) * S::kSlot;
+                const float4 o = __ldcg(reinterpret_cast<const float4*>(piece + r * D + c));
+                const float f = exp2_approx((__ldcg(piece + D * kTreeRows + r) - up) * a.scale_log2);
+                l = fmaf(__ldcg(piece + (D + 1) * kTreeRows + r), f, l);
+                x.x = fmaf(o.x, f, x.x);
+                x.y = fmaf(o.y, f, x.y);
+                x.z = fmaf(o.z, f, x.z);
+                x.w = fmaf(o.w, f, x.w);
+              }
+              const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+              T* to = static_cast<T*>(a.out) + (token0 + r / a.group) * a.out_stride + int64_t(head0 + r % a.group) * D + c;
+              *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
             }
-            const int token = row / a.group, head = head0 + row - token * a.group;
-            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-            T* p = static_cast<T*>(a.out) + (int64_t(now.seq) * a.drafted + token) * a.out_stride + head * D + c;
-            *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(sum.x * inv, sum.y * inv), pack2<T>(sum.z * inv, sum.w * inv));
           }
         }
-        __syncthreads();
+        piece_begin = begin + it + 1;
       }
-      piece_begin = at + 1;
-    }
-    if (it + 1 < n_tiles) {
-      const int seq = now.seq, tiles = now.tiles;
-      if (advance(now)) {
+      if (it + 1 < n_tiles) {
+        const int seq = now.seq, tiles = now.tiles;
+        fresh = advance(now);
         if (now.seq != seq) seq_begin += int64_t(tiles) * parts;
-        begin_segment();
       }
     }
+    tc_fence_before();
   }
-  tree_cp_wait<0>();
+  __syncthreads();
+  tc_fence_after();
+  if (bars->aborted && tid == 0) {  // copies that nobody waited for
+    const int q_issued = bars->q_issued;
+    for (int i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i)
+      for (uint32_t n = 0; n < (1u << 16) && !mbar_try_wait_hint(&bars->q_full[i & 1], uint32_t(i / 2) & 1); ++n) {}
+  }
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Row warps: enough for the rows of a key head, up to eight.
-int tree_row_warps(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
-
-template <class T, int D, int RW>
-cudaError_t launch_tree(const TreeArgs& a, cudaStream_t s) {
-  constexpr int smem = TreeShape<D, RW>::kSmem;
-  static PerDeviceOnce once;
-  const cudaError_t e = per_device_once(once, [] { return opt_in_smem(tree_kernel<T, D, RW>, smem); });
-  if (e != cudaSuccess) return e;
-  return launch_pdl(tree_kernel<T, D, RW>, dim3(unsigned(sm_count())), dim3(kTreeThreads), size_t(smem), s, a);
-}
 template <class T, int D>
-cudaError_t launch_tree_rows(const TreeArgs& a, int rw, cudaStream_t s) {
-  return rw == 1 ? launch_tree<T, D, 1>(a, s) : rw == 2 ? launch_tree<T, D, 2>(a, s) : rw == 4 ? launch_tree<T, D, 4>(a, s)
-                                                                                             : launch_tree<T, D, 8>(a, s);
+cudaError_t launch_tree(const TreeArgs& a, const CUtensorMap& q_map, cudaStream_t s) {
+  static PerDeviceOnce once;
+  const cudaError_t e = per_device_once(once, [] { return opt_in_smem(tree_kernel<T, D>, TreeShape<D>::kSmem); });
+  if (e != cudaSuccess) return e;
+  return launch_pdl(tree_kernel<T, D>, dim3(unsigned(sm_count())), dim3(kTreeThreads), size_t(TreeShape<D>::kSmem), s, a, q_map);
+}
+
+// Drafted tokens of a row tile: whole tokens, as many as 128 rows hold.
+int tree_tile_tokens(int drafted, int group) {
+  const int fit = kTreeRows / group;
+  return drafted < fit ? drafted : fit;
+}
+int tree_row_tiles(int drafted, int group) {
+  const int t = tree_tile_tokens(drafted, group);
+  return (drafted + t - 1) / t;
 }
 size_t tree_counter_bytes(int64_t n_seqs, int drafted, int heads, int kv_heads) {
-  const int rows = drafted * (heads / kv_heads), tile = 16 * tree_row_warps(rows);
-  return (size_t(n_seqs) * kv_heads * ((rows + tile - 1) / tile) * 4 + 255) & ~size_t(255);
+  return (size_t(n_seqs) * kv_heads * tree_row_tiles(drafted, heads / kv_heads) * 4 + 255) & ~size_t(255);
 }
 bool tree_shape_ok(int n_seqs, int drafted, int heads, int kv_heads, int dim) {
   return n_seqs >= 0 && drafted >= 1 && drafted <= kTreeMaxDrafted && kv_heads >= 1 && heads >= kv_heads && heads <= 1024 &&
-         heads % kv_heads == 0 && (dim == 64 || dim == 128);
+         heads % kv_heads == 0 && heads / kv_heads <= kTreeRows && (dim == 64 || dim == 128);
+}
+
+// [tokens][heads][dim] in boxes of a row tile: its tokens x the heads of a group x 64 values.
+bool tree_map_q(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, int64_t tokens, int64_t stride, int group, int tile) {
+  const cuuint64_t dims[3] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(tokens)};
+  const cuuint64_t strides[2] = {cuuint64_t(dim) * 2, cuuint64_t(stride) * 2};
+  const cuuint32_t box[3] = {64, cuuint32_t(group), cuuint32_t(tile)}, elem[3] = {1, 1, 1};
+  return encode_tiled_fn()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                           const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace
@@ -516,8 +611,7 @@ extern "C" {
 
 size_t fb_attn_tree_workspace_bytes(int32_t n_seqs, int32_t drafted, int32_t heads, int32_t kv_heads, int32_t head_dim) {
   if (!tree_shape_ok(n_seqs, drafted, heads, kv_heads, head_dim)) return 0;
-  const int tile = 16 * tree_row_warps(drafted * (heads / kv_heads));
-  return tree_counter_bytes(n_seqs, drafted, heads, kv_heads) + size_t(2 * kTreeMaxSms) * tile * (head_dim + 2) * 4;
+  return 256 + tree_counter_bytes(n_seqs, drafted, heads, kv_heads) + size_t(2 * kTreeMaxSms) * kTreeRows * (head_dim + 2) * 4;
 }
 
 int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int32_t n_seqs, int32_t drafted,
@@ -529,12 +623,15 @@ int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int3
   if (cache->dtype != FB_DT_BF16 && cache->dtype != FB_DT_F16) return invalid("attn_tree_decode: bf16 or fp16");
   if (drafted < 1 || drafted > kTreeMaxDrafted) return invalid("attn_tree_decode: 1..64 drafted tokens per sequence");
   if (!tree_shape_ok(n_seqs, drafted, heads, kv, dim))
-    return invalid("attn_tree_decode: unsupported shape (head_dim 64 or 128, heads a multiple of kv_heads up to 1024)");
+    return invalid("attn_tree_decode: unsupported shape (head_dim 64 or 128, heads a multiple of kv_heads, up to 1024 and 128 per key head)");
   if (!n_seqs) return 0;
   if (!q || !out || !block_table || !contexts || !cache->k || !cache->v) return invalid("attn_tree_decode: null argument");
   if (cache->page_size < 1 || cache->n_pages < 1) return invalid("attn_tree_decode: a cache without pages");
   if (table_stride < 1) return invalid("attn_tree_decode: a table without columns");
   if (table_stride > INT32_MAX / 2 / cache->page_size) return invalid("attn_tree_decode: more than 2^30 keys per sequence");
+  if (cache->n_pages > INT32_MAX / cache->page_size) return invalid("attn_tree_decode: a cache of more than 2^31 slots");
+  if (int64_t(n_seqs) * drafted > INT32_MAX || q_stride >= int64_t(1) << 38)
+    return invalid("attn_tree_decode: q is too large");
   if (q_stride < int64_t(heads) * dim || out_stride < int64_t(heads) * dim)
     return invalid("attn_tree_decode: a stride is smaller than a token's heads");
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(cache->k) |
@@ -547,21 +644,25 @@ int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int3
       workspace_bytes < fb_attn_tree_workspace_bytes(n_seqs, drafted, heads, kv, dim))
     return invalid("attn_tree_decode: workspace missing, misaligned (256 B) or smaller than fb_attn_tree_workspace_bytes");
   if (sm_count() > kTreeMaxSms) return invalid("attn_tree_decode: more than 256 multiprocessors");
+  if (!encode_tiled_fn()) {
+    set_error("attn_tree_decode: cuTensorMapEncodeTiled is not available");
+    return int32_t(cudaErrorNotSupported);
+  }
   TreeArgs a;
-  a.q = q;
   a.out = out;
   a.k = cache->k;
   a.v = cache->v;
   a.table = block_table;
   a.contexts = contexts;
   a.mask = mask;
-  a.q_stride = q_stride;
   a.out_stride = out_stride;
-  a.n_pages = cache->n_pages;
   a.table_stride = table_stride;
-  a.counters = static_cast<int32_t*>(workspace);
-  a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + tree_counter_bytes(n_seqs, drafted, heads, kv));
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  a.status = reinterpret_cast<uint32_t*>(base);
+  a.counters = reinterpret_cast<int32_t*>(base + 256);
+  a.partial = reinterpret_cast<float*>(base + 256 + tree_counter_bytes(n_seqs, drafted, heads, kv));
   a.scale_log2 = scale * 1.4426950408889634f;  // scores are kept in powers of two
+  a.n_pages = int(cache->n_pages);
   a.n_seqs = n_seqs;
   a.drafted = drafted;
   a.kv_heads = kv;
@@ -570,12 +671,15 @@ int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int3
   a.page_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (cache->page_size == 1 << i) a.page_shift = i;
-  const int rows = drafted * a.group, rw = tree_row_warps(rows);
-  a.row_tiles = (rows + 16 * rw - 1) / (16 * rw);
-  cudaStream_t s = as_stream(stream);
+  a.tile_tokens = tree_tile_tokens(drafted, a.group);
+  a.row_tiles = tree_row_tiles(drafted, a.group);
   const bool bf = cache->dtype == FB_DT_BF16;
-  const cudaError_t e = dim == 64 ? (bf ? launch_tree_rows<__nv_bfloat16, 64>(a, rw, s) : launch_tree_rows<__half, 64>(a, rw, s))
-                                  : (bf ? launch_tree_rows<__nv_bfloat16, 128>(a, rw, s) : launch_tree_rows<__half, 128>(a, rw, s));
+  CUtensorMap q_map;
+  if (!tree_map_q(&q_map, q, bf, dim, heads, int64_t(n_seqs) * drafted, q_stride, a.group, a.tile_tokens))
+    return invalid("attn_tree_decode: cuTensorMapEncodeTiled failed");
+  cudaStream_t s = as_stream(stream);
+  const cudaError_t e = dim == 64 ? (bf ? launch_tree<__nv_bfloat16, 64>(a, q_map, s) : launch_tree<__half, 64>(a, q_map, s))
+                                  : (bf ? launch_tree<__nv_bfloat16, 128>(a, q_map, s) : launch_tree<__half, 128>(a, q_map, s));
   const int32_t st = check_launch("attn_tree_decode");
   return st ? st : int32_t(e);
 }

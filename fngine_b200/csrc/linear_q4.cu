@@ -311,8 +311,8 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           tile[(nt * 8 + 2 * t + (i & 1)) * kPitch + m * 16 + g + (i >> 1) * 8] = acc[m][nt][i];
-    if (split == 1) __syncwarp();
-    else named_bar_sync(1 + wu, 32 * split);
+    __syncwarp();
+    if (split > 1) named_bar_sync(1 + wu, 32 * split);
     if (unit < a.units) {
       const float* tiles = tile - wk * (8 * NT * kPitch);
       const int rows = swiglu ? 16 : 16 * MT, shift = rows == 16 ? 4 : 5;
@@ -343,8 +343,8 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
         }
       }
     }
-    if (split == 1) __syncwarp();
-    else named_bar_sync(1 + wu, 32 * split);
+    __syncwarp();
+    if (split > 1) named_bar_sync(1 + wu, 32 * split);
   }
   cp_async_wait<0>();
 }

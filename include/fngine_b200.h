@@ -570,7 +570,9 @@ typedef struct fb_kv_cache {
  * token sees are to be finite. Softmax statistics and sums are fp32, the weights are rounded to the type of v. Joins of split
  * work are in a fixed order: repeated calls are bitwise identical.
  * `workspace`: fb_attn_tree_workspace_bytes() bytes (0 for an unsupported shape), 256-byte aligned, zero-filled once; the
- * call leaves its counters clear. Calls that share one must not overlap, captured ones included. head_dim 64 or 128. */
+ * call leaves its counters clear. Its first word is a status (FB_STATUS_*): FB_STATUS_PIPELINE_TIMEOUT once a bounded wait has run out,
+ * after which it is to be zero-filled again. Calls that share one must not overlap, captured ones included, and have the
+ * same shapes or are separated by a zero-fill. head_dim 64 or 128, up to 128 query heads per key head, up to 2^31 - 1 slots. */
 size_t fb_attn_tree_workspace_bytes(int32_t n_seqs, int32_t drafted, int32_t heads, int32_t kv_heads, int32_t head_dim);
 int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int32_t n_seqs, int32_t drafted,
                             const fb_kv_cache* cache, const int32_t* block_table, int64_t table_stride, const int32_t* contexts,

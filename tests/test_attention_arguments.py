@@ -59,9 +59,9 @@ def test_attn_tree_refusals(fb_built):
     lib = L.load()
     size = lib.fb_attn_tree_workspace_bytes
     need = size(2, 3, 8, 2, 128)
-    assert need == 256 + 512 * 16 * 130 * 4 and size(2, 64, 8, 1, 64) == 256 + 512 * 128 * 66 * 4
-    assert size(100, 64, 16, 2, 64) == 100 * 2 * 4 * 4 + 128 + 512 * 128 * 66 * 4  # four row tiles of 128
-    for bad in [(-1, 3, 8, 2, 128), (2, 0, 8, 2, 128), (2, 65, 8, 2, 128), (2, 3, 9, 2, 128), (2, 3, 8, 0, 128), (2, 3, 2, 8, 128), (2, 3, 8, 2, 96)]:
+    assert need == 512 + 512 * 128 * 130 * 4 and size(2, 64, 8, 1, 64) == 512 + 512 * 128 * 66 * 4
+    assert size(100, 64, 16, 2, 64) == 256 + 100 * 2 * 4 * 4 + 128 + 512 * 128 * 66 * 4  # four row tiles of sixteen tokens
+    for bad in [(-1, 3, 8, 2, 128), (2, 0, 8, 2, 128), (2, 65, 8, 2, 128), (2, 3, 9, 2, 128), (2, 3, 8, 0, 128), (2, 3, 2, 8, 128), (2, 3, 8, 2, 96), (2, 1, 129, 1, 64)]:
         assert size(*bad) == 0
 
     def call(q=P, q_stride=1024, heads=8, n_seqs=2, drafted=3, cache={}, no_cache=False, table=2 * P, table_stride=4, contexts=3 * P, mask=4 * P,
@@ -78,7 +78,7 @@ def test_attn_tree_refusals(fb_built):
                       (dict(cache=dict(dtype=L.DT_F32)), b"bf16 or fp16"), (dict(drafted=0), b"1..64"), (dict(drafted=65), b"1..64"),
                       (dict(heads=7), b"shape"), (dict(n_seqs=-1), b"shape"), (dict(cache=dict(kv_heads=0)), b"shape"), (dict(cache=dict(head_dim=80)), b"shape"),
                       (dict(cache=dict(page_size=0)), b"pages"), (dict(cache=dict(n_pages=0)), b"pages"), (dict(table_stride=0), b"columns"),
-                      (dict(table_stride=2 ** 27), b"2^30"), (dict(q_stride=1016), b"stride"), (dict(out_stride=512), b"stride"), (dict(q_stride=1028), b"16 bytes"),
+                      (dict(table_stride=2 ** 27), b"2^30"), (dict(cache=dict(n_pages=2 ** 27)), b"2^31"), (dict(q_stride=2 ** 39), b"too large"), (dict(q_stride=1016), b"stride"), (dict(out_stride=512), b"stride"), (dict(q_stride=1028), b"16 bytes"),
                       (dict(q=P + 8), b"16 bytes"), (dict(cache=dict(v=8 * P + 2)), b"16 bytes"), (dict(table=2 * P + 2), b"aligned"),
                       (dict(mask=4 * P + 4), b"aligned"), (dict(scale=0.0), b"scale"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"),
                       (dict(scale=float("inf")), b"scale"), (dict(workspace=None), b"workspace"), (dict(workspace=6 * P + 128), b"workspace"), (dict(bytes=need - 1), b"workspace")]:

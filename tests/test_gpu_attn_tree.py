@@ -101,6 +101,10 @@ CASES = [
     (300, 2, 4, 2, 64, 16, [(37 * j) % 211 for j in range(300)], "bfloat16", True),  # more sequences than threads
     (9, 4, 32, 8, 128, 128, [0, 1, 2, 3, 1000, 1, 0, 5000, 9], "float16", True),
     (1, 64, 3, 1, 128, 16, [0], "float16", False),
+    (3, 16, 48, 8, 128, 64, [4096, 2500, 3001], "bfloat16", True),    # many key blocks per multiprocessor
+    (2, 2, 8, 8, 64, 16, [12000, 9000], "float16", True),
+    (2, 9, 100, 1, 64, 16, [300, 41], "bfloat16", True),              # a hundred heads of one key head: a token per row tile
+    (3, 11, 45, 5, 128, 32, [260, 0, 513], "float16", True),          # 99 rows
     (7, 8, 8, 8, 128, 16, [15, 16, 17, 143, 144, 145, 120], "bfloat16", False),
 ]
 
@@ -119,6 +123,7 @@ def test_against_the_formula(seqs, drafted, heads, kv, dim, page, contexts, dtyp
     again = torch.full_like(q, float("nan"))
     A.attn_tree_decode(q, cache, table, ctx, again, ws, mask=mask)
     assert torch.equal(again, out)  # and the counters were left clear
+    assert not bool(ws[:256].any())  # no wait ran out
 
 
 def test_what_nobody_sees_is_not_looked_at():
