@@ -24,7 +24,6 @@ namespace {
 
 constexpr int kTreeThreads = 288;        // four softmax warps, four that copy, one that issues products
 constexpr int kTreeWarps = kTreeThreads / 32;
-constexpr int kTreeLag = 3;              // copies of tiles that a copying thread has in flight behind the one it announces
 constexpr int kTreeRows = 128;           // rows of a tile
 constexpr int kTreeKeys = 128;           // keys of a block
 constexpr int kTreeMaxDrafted = 64;
@@ -283,17 +282,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
                          : "memory");
           }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (i >= kTreeLag) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(kTreeLag) : "memory");
-          fence_proxy_async();  // (the products read shared memory through the other proxy)
-          mbar_arrive(&bars->full[(i - kTreeLag) % kStages]);
-        }
+        // One of the slot's 128 arrivals, made when this thread's copies have landed.
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars->full[at])) : "memory");
       }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    fence_proxy_async();
-    for (int i = 2 * n_tiles > kTreeLag ? 2 * n_tiles - kTreeLag : 0; i < 2 * n_tiles; ++i) mbar_arrive(&bars->full[i % kStages]);
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == 8) {
     // ------------------------------------------------------------------ products
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -312,6 +305,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
       wait(&bars->full[slot], uint32_t(2 * it / kStages) & 1);
       const bool last = next.tile + 1 == next.tiles;
       if (ok) {
+        fence_proxy_async();  // (the copies were made by the generic proxy, the product reads through the other)
         tc_fence_after();
         if (elect_one()) {
           const uint64_t qd = umma_desc(smem_u32(q_tiles + b * S::kTileBytes), 1), kd = umma_desc(smem_u32(ring + slot * S::kTileBytes), 1);
@@ -340,6 +334,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
       wait(&bars->p_full[it & 1], uint32_t(it >> 1) & 1);
       wait(&bars->full[slot], uint32_t((2 * it + 1) / kStages) & 1);
       if (!ok) break;
+      fence_proxy_async();
       tc_fence_after();
       if (elect_one()) {
         const uint64_t vd = umma_desc(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
