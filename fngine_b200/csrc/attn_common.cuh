@@ -27,11 +27,69 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return r;
 }
 
+// ------------------------------------------------------------------------------ a row's scores, 32 at a time
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// The larger of m and 32 scores.
+__device__ __forceinline__ float scores_max(const float (&s)[32], float m) {
+  float a = max3(m, s[0], s[1]), b = max3(s[2], s[3], s[4]), c = max3(s[5], s[6], s[7]);
+#pragma unroll
+  for (int i = 8; i < 32; i += 6) {
+    a = max3(a, s[i], s[i + 1]);
+    b = max3(b, s[i + 2], s[i + 3]);
+    c = max3(c, s[i + 4], s[i + 5]);
+  }
+  return max3(a, b, c);
+}
+// 32 weights 2^(scale s - base) as pairs of T (rounded to the type of v: half a step of each weight, averaged over the keys) and, before
+// that rounding, added to `sum` (a pair of partial sums).
+template <class T>
+__device__ __forceinline__ void scores_exp(const float (&s)[32], uint64_t scale, uint64_t minus_base, uint32_t (&p)[16], uint64_t (&sum)[2]) {
+#pragma unroll
+  for (int c = 0; c < 16; ++c) {
+    float x, y;
+    unpair(fma2(pair_of(s[2 * c], s[2 * c + 1]), scale, minus_base), x, y);
+    x = exp2_approx(x);
+    y = exp2_approx(y);
+    sum[c & 1] = add2(sum[c & 1], pair_of(x, y));
+    p[c] = pack2<T>(x, y);
+  }
+}
+__device__ __forceinline__ float pairs_sum(const uint64_t (&sum)[2]) {
+  float a, b;
+  unpair(add2(sum[0], sum[1]), a, b);
+  return a + b;
+}
+
 // ------------------------------------------------------------------------------ copies and products
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
                    dst),
                "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+               "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
                : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {

@@ -8,12 +8,15 @@
 // tensor core 1024 cycles at head_dim 128 and a multiprocessor's share of the memory bandwidth 2800. (Products by mma.sync with
 // fragments in registers, 16 to 128 rows, were bound by the latencies of eight warps: 446 us for 32 sequences of up to 16384 keys
 // and four tokens, 87 for eight of 4096 and sixteen.)
-//   S = Q K^T   both operands in shared memory, two buffers of fp32 S: the next block's product runs under this one's softmax
+//   S = Q K^T   both operands in shared memory, fp32 S in tensor memory
 //   P = 2^(c S - c m) over S in the type of v, by a thread per row; only warps that hold rows read S
 //   O += P V    fp32 in tensor memory; multiplied only when a maximum rises by more than 2^8 above the one in use
-// Keys and values come by cp.async, 16 bytes a thread, from slots that a table look-up a block ahead has found: pages of any size, and
-// what is not to be read is written as zeros. (TMA gathers of four cache rows took 41 ns each per multiprocessor, 512 bytes: 919 us
-// for the 32 sequences.) The blocks of keys of all (sequence, key head, row tile) segments are one sequence that is cut
+// A block of keys keeps its softmax warps for some 3300 cycles, longer than its bytes take. So even and odd blocks are two streams with
+// warps, S, O, maxima and sums of their own, which meet where a segment ends: each O is read there by both, half of the columns each.
+// Blocks of context keys come by TMA, a box per run of slots that a page holds (up to 128, the power of two in the page size). The
+// block where the context ends, and all blocks where that power is below kTreeMinBox, come by cp.async, 16 bytes a thread: any slots, and
+// what is not to be read is written as zeros. (cp.async alone moves 4.4 TB/s; TMA gathers of four cache rows took 41 ns each per
+// multiprocessor, 512 bytes.) The blocks of keys of all (sequence, key head, row tile) segments are one sequence that is cut
 // evenly over the multiprocessors, so that sequences of different lengths leave none of them idle, whatever lengths the
 // device finds (the host does not know them). A segment that several blocks share is joined by the last of them to arrive, in
 // block order: results do not depend on timing.
@@ -22,12 +25,13 @@
 namespace fb {
 namespace {
 
-constexpr int kTreeThreads = 288;        // four softmax warps, four that copy, one that issues products
+constexpr int kTreeThreads = 416;        // two streams of four softmax warps, four warps that copy, one that issues products
 constexpr int kTreeWarps = kTreeThreads / 32;
 constexpr int kTreeRows = 128;           // rows of a tile
 constexpr int kTreeKeys = 128;           // keys of a block
 constexpr int kTreeMaxDrafted = 64;
 constexpr int kTreeMaxSms = 256;         // partial results are sized for this many blocks
+constexpr int kTreeMinBox = 8;           // slots of the smallest box
 constexpr float kTreeSlack = 8.f;        // how far (in powers of two) scores may rise above the maximum in use
 
 struct TreeArgs {
@@ -41,31 +45,43 @@ struct TreeArgs {
   int64_t table_stride;
   uint32_t* status;
   int32_t* counters;   // [segments]
-  float* partial;      // [2 * blocks]: outputs [128][D], maxima [128], sums [128]
+  float* partial;      // [2 * blocks]: outputs [D / 4][128][4], maxima [128], sums [128]
   float scale_log2;
   int n_pages, n_seqs, drafted, kv_heads, group, page_size, page_shift;
+  int box;                     // slots of a copied box, 0: no boxes
   int row_tiles, tile_tokens;  // row tiles per key head, drafted tokens per row tile
 };
+struct TreeMaps {
+  CUtensorMap q, k, v;
+};
+
 template <int D>
 struct TreeShape {
   static constexpr int kTileBytes = kTreeKeys * D * 2;
   static constexpr int kHalf = kTreeKeys * 128;  // a tile is D / 64 parts of 128 rows x 128 bytes
   static constexpr int kStages = D == 128 ? 5 : 10;
-  static constexpr int kSmem = (2 + kStages) * kTileBytes + 1024 + 1536;
+  static constexpr int kSmem = (2 + kStages) * kTileBytes + 3072;
   static constexpr int kSlot = (D + 2) * kTreeRows;  // floats of a partial result
 };
 
 struct TreeBars {
-  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_done, full[10], empty[10], drained;
-  int64_t sums[kTreeWarps];
-  int64_t found[2];
-  int slots[2][kTreeKeys];  // cache slots of a key block, -1: zeros
+  uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2], full[10], empty[10], drained;
+  float tops[2][kTreeRows], sum_of[2][kTreeRows];  // of the two streams, where they meet
+  union {
+    int slots[kTreeKeys];  // cache slots of a key block, -1: zeros
+    struct {               // before the first of them
+      int64_t sums[kTreeWarps];
+      int64_t found[2];
+    };
+  };
   uint32_t tmem;
   int aborted;
   int q_issued;
+  int in_flight;  // copies up to the last one made by TMA
   int last_block;
 };
-static_assert(sizeof(TreeBars) <= 1536, "room behind the ring");
+static_assert(sizeof(TreeBars) <= 3072, "room behind the ring");
+static_assert(TreeShape<128>::kSmem <= 227 * 1024, "all of a multiprocessor's shared memory");
 
 // Walks through the key blocks of the segments in their order.
 struct TreeCursor {
@@ -74,11 +90,10 @@ struct TreeCursor {
 };
 
 template <class T, int D>
-__global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a, const __grid_constant__ CUtensorMap q_map) {
+__global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a, const __grid_constant__ TreeMaps maps) {
   using S = TreeShape<D>;
   constexpr int kStages = S::kStages, kParts = D / 64;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* q_tiles = smem;
   uint8_t* ring = smem + 2 * S::kTileBytes;
   TreeBars* bars = reinterpret_cast<TreeBars*>(ring + kStages * S::kTileBytes);
@@ -86,6 +101,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
   const int parts = a.kv_heads * a.row_tiles;
   const int64_t room = a.table_stride * a.page_size;  // keys that the table can hold
   pdl_wait_prior();
+  if (smem_u32(smem) & 1023u) {  // (tiles and their swizzle start on 1024 bytes)
+    if (tid == 0) atomicMax(a.status, uint32_t(FB_STATUS_BAD_WORK));
+    return;
+  }
 
   auto length_of = [&](int seq, int* ctx) {
     int c = a.contexts[seq];
@@ -181,7 +200,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
     return true;
   };
 
-  if (warp == 8) {
+  if (warp == 12) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem)), "r"(512)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -192,8 +211,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
       mbar_init(&bars->q_empty[i], 1);
       mbar_init(&bars->s_full[i], 1);
       mbar_init(&bars->p_full[i], kTreeRows);
+      mbar_init(&bars->o_done[i], 1);
     }
-    mbar_init(&bars->o_done, 1);
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&bars->full[i], kTreeKeys);
       mbar_init(&bars->empty[i], 1);
@@ -201,6 +220,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
     mbar_init(&bars->drained, 1);
     bars->aborted = 0;
     bars->q_issued = 0;
+    bars->in_flight = 0;
     mbar_fence_init();
   }
   tc_fence_before();
@@ -209,11 +229,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
   // (not before the allocation: a block of the next kernel that took tensor memory and then waited for this one would hold it up)
   pdl_launch_dependents();
   const uint32_t tmem = bars->tmem;
-  constexpr uint32_t kS = 0, kO = 256;  // S of an even and an odd key block, outputs
+  constexpr uint32_t kS = 0, kO = 256;  // stream t: S in columns 128 t, O in 256 + 128 t
 
-  if (warp >= 4 && warp < 8) {
+  if (warp >= 8 && warp < 12) {
     // ------------------------------------------------------------------ copies
-    const int me = tid - 128;  // looks up key `me` of a block
+    const int me = tid - 256;  // looks up key `me` of a block
     uint64_t seen = 0;         // drafted tokens that some token of the sequence sees
     auto look = [&](int seq) {
       seen = ~0ull;
@@ -249,45 +269,63 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
           const int token = now.seq * a.drafted + (now.part % a.row_tiles) * a.tile_tokens;
           mbar_expect_tx(&bars->q_full[b], uint32_t(a.tile_tokens * a.group) * D * 2);
           for (int p = 0; p < kParts; ++p)
-            tma_load_3d(smem_u32(q_tiles + b * S::kTileBytes) + p * S::kHalf, &q_map, p * 64, head * a.group, token, &bars->q_full[b]);
+            tma_load_3d(smem_u32(q_tiles + b * S::kTileBytes) + p * S::kHalf, &maps.q, p * 64, head * a.group, token, &bars->q_full[b]);
           bars->q_issued = segment + 1;
         }
         ++segment;
       }
-      {
-        const int key = now.tile * kTreeKeys + me, index = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
-        // A page outside of the cache reads as zeros, as does a drafted token that nobody sees.
-        bars->slots[it & 1][me] = page >= 0 && page < a.n_pages ? page * a.page_size + (key - index * a.page_size) : -1;
-      }
+      // A page outside of the cache reads as zeros, as does a drafted token that nobody sees.
+      const int key = now.tile * kTreeKeys + me, index = a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size;
+      const int mine = page >= 0 && page < a.n_pages ? page * a.page_size + (key - index * a.page_size) : -1;
+      const bool boxes = a.box && (now.tile + 1) * kTreeKeys <= now.ctx;  // (the same for all)
+      if (!boxes) bars->slots[me] = mine;
       if (it + 1 < n_tiles) {
         const int seq = now.seq;
         fresh = advance(now);
         if (now.seq != seq) look(now.seq);
         ask();
       }
-      warps_sync(2, kTreeKeys);
-      const int* slots = &bars->slots[it & 1][row];
+      if (!boxes) warps_sync(2, kTreeKeys);
+      const int* slots = &bars->slots[row];
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         const int i = 2 * it + kv, at = i % kStages;
         if (i >= kStages) ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->empty[at], uint32_t(i / kStages - 1) & 1);
-        if (ok) {
-          const T* from = static_cast<const T*>(kv ? a.v : a.k) + head * D + chunk * 8;
-          const uint32_t dst = smem_u32(ring + at * S::kTileBytes) + put;
-#pragma unroll
-          for (int p = 0; p < kPasses; ++p) {
-            const int slot = slots[p * kPerPass];
-            const T* src = from + size_t(slot < 0 ? 0 : slot) * slot_values;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + p * (kPerPass * 128)), "l"(src), "r"(slot < 0 ? 0 : 16)
-                         : "memory");
+        // Each thread makes one of the slot's 128 arrivals.
+        if (boxes) {
+          if (ok && me == 0) {
+            mbar_expect_tx(&bars->full[at], S::kTileBytes);
+            bars->in_flight = i + 1;
+          } else {
+            mbar_arrive(&bars->full[at]);
           }
+          if (ok && me % a.box == 0) {
+            const uint32_t dst = smem_u32(ring + at * S::kTileBytes) + me * 128;
+#pragma unroll
+            for (int p = 0; p < kParts; ++p)
+              tma_load_2d(dst + p * S::kHalf, kv ? &maps.v : &maps.k, head * D + p * 64, mine >= 0 ? mine : a.n_pages * a.page_size, &bars->full[at]);
+          }
+          __syncwarp();
+        } else {
+          if (ok) {
+            const T* from = static_cast<const T*>(kv ? a.v : a.k) + head * D + chunk * 8;
+            const uint32_t dst = smem_u32(ring + at * S::kTileBytes) + put;
+#pragma unroll
+            for (int p = 0; p < kPasses; ++p) {
+              const int slot = slots[p * kPerPass];
+              const T* src = from + size_t(slot < 0 ? 0 : slot) * slot_values;
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + p * (kPerPass * 128)), "l"(src), "r"(slot < 0 ? 0 : 16)
+                           : "memory");
+            }
+          }
+          // (made when this thread's copies have landed)
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars->full[at])) : "memory");
         }
-        // One of the slot's 128 arrivals, made when this thread's copies have landed.
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bars->full[at])) : "memory");
       }
+      if (!boxes) warps_sync(2, kTreeKeys);  // the slots have been read
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == 8) {
+  } else if (warp == 12) {
     // ------------------------------------------------------------------ products
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kTreeRows >> 4) << 24);
@@ -323,7 +361,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
       if (last) ++segment;
     };
     scores(0, true);
-    bool first = true;  // block of its segment, in this block's share
+    int piece = 0;  // first block of the segment in this block's share
     for (int it = 0; it < n_tiles && ok; ++it) {
       bool next_first = false;
       if (it + 1 < n_tiles) {
@@ -340,57 +378,56 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
         const uint64_t vd = umma_desc(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
 #pragma unroll
         for (int k = 0; k < kTreeKeys / 16; ++k)
-          umma_ts(tmem + kO, tmem + kS + 128 * (it & 1) + 8 * k, vd + k * (2048 >> 4), kIdescPv, !first || k > 0);
-        umma_commit(&bars->o_done);
+          umma_ts(tmem + kO + 128 * (it & 1), tmem + kS + 128 * (it & 1) + 8 * k, vd + k * (2048 >> 4), kIdescPv, it - piece >= 2 || k > 0);
+        umma_commit(&bars->o_done[it & 1]);
         umma_commit(&bars->empty[slot]);
       }
       __syncwarp();
-      first = next_first;
+      if (next_first) piece = it + 1;
     }
     // Nothing issued here is still running when the tensor memory is given back.
     if (elect_one()) umma_commit(&bars->drained);
     __syncwarp();
     for (uint32_t n = 0; n < (1u << 16) && !__all_sync(0xffffffffu, mbar_try_wait_hint(&bars->drained, 0)); ++n) {}
   } else {
-    // ------------------------------------------------------------------ softmax: thread = row
-    const uint32_t lanes = uint32_t(warp) << 21;  // (32 warp) << 16
-    const uint32_t o_at = tmem + lanes + kO;
+    // ------------------------------------------------------------------ softmax: thread = row, warps 4 t .. 4 t + 3 take stream t
+    const int t = warp >> 2, row = tid & (kTreeRows - 1), lane_row = 32 * (warp & 3);
+    const uint32_t lanes = uint32_t(lane_row) << 16;
+    const uint32_t s_at = tmem + lanes + kS + 128 * t, o_at = tmem + lanes + kO + 128 * t;
+    const uint64_t scale = pair_of(a.scale_log2, a.scale_log2);
     bool ok = true, fresh = true;
     float top = -INFINITY, sum = 0.f;
-    int head0 = 0, token = 0, rows = 0, head = 0;
+    int rows = 0, head0 = 0;
+    int64_t token0 = 0;
     uint64_t sees = 0;
-    int64_t piece_begin = begin;
+    int piece = 0;  // first block of the segment in this block's share
+    // (after a wait that ran out the loop goes on without work: all eight warps meet at the same barriers)
     for (int it = 0; it < n_tiles; ++it) {
       if (fresh) {
+        fresh = false;
+        piece = it;
         top = -INFINITY;
         sum = 0.f;
-        const int token0 = (now.part % a.row_tiles) * a.tile_tokens;
-        const int tokens = a.drafted - token0 < a.tile_tokens ? a.drafted - token0 : a.tile_tokens;
+        const int first = (now.part % a.row_tiles) * a.tile_tokens;
+        const int tokens = a.drafted - first < a.tile_tokens ? a.drafted - first : a.tile_tokens;
         rows = tokens * a.group;
         head0 = (now.part / a.row_tiles) * a.group;
-        token = token0 + tid / a.group;
-        head = head0 + tid % a.group;
+        token0 = int64_t(now.seq) * a.drafted + first;
         sees = 0;
-        if (tid < rows) sees = a.mask ? a.mask[int64_t(now.seq) * a.drafted + token] : token == 63 ? ~0ull : (2ull << token) - 1;
+        const int token = row / a.group;
+        if (row < rows) sees = a.mask ? a.mask[token0 + token] : first + token == 63 ? ~0ull : (2ull << (first + token)) - 1;
         const int there = now.length - now.ctx;  // drafted tokens that the table has room for
         if (there < 64) sees &= (1ull << there) - 1;
       }
-      const bool segment_ends = now.tile + 1 == now.tiles;
-      // (after a wait that ran out the loop goes on without work: all four warps meet at the same barriers)
-      ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->s_full[it & 1], uint32_t(it >> 1) & 1);
-      if (ok && 32 * warp < rows) {
-        tc_fence_after();
-        const uint32_t s_at = tmem + lanes + kS + 128 * (it & 1);
-        float s[4][32];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32(s_at + 32 * i, s[i]);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_landed(s[i]);
-        const int off = now.ctx - now.tile * kTreeKeys;  // first column behind the context
-        if (off < kTreeKeys) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
+      const bool segment_ends = now.tile + 1 == now.tiles, piece_ends = segment_ends || it + 1 == n_tiles;
+      if ((it & 1) == t) {
+        ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->s_full[t], uint32_t(it >> 1) & 1);
+        if (ok && lane_row < rows) {
+          tc_fence_after();
+          // (The scores are read twice, once for the maximum and once for the weights: 130 cycles of 3300, for 64 registers.)
+          const int off = now.ctx - now.tile * kTreeKeys;  // first column behind the context
+          auto unseen = [&](int i, float (&s)[32]) {
+            if (off >= kTreeKeys) return;
             const int sh = off - 32 * i;  // bit of this word that drafted token 0 has
             uint32_t bits;
             if (sh >= 32) bits = 0xffffffffu;
@@ -398,111 +435,125 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
             else bits = -sh < 64 ? uint32_t(sees >> -sh) : 0u;
 #pragma unroll
             for (int c = 0; c < 32; ++c)
-              if (!((bits >> c) & 1)) s[i][c] = -INFINITY;
+              if (!((bits >> c) & 1)) s[c] = -INFINITY;
+          };
+          float s[2][32], latest = -INFINITY;
+          tmem_ld32(s_at, s[0]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            tmem_ld_wait();
+            tmem_landed(s[i & 1]);
+            if (i < 3) tmem_ld32(s_at + 32 * (i + 1), s[(i + 1) & 1]);
+            unseen(i, s[i & 1]);
+            latest = scores_max(s[i & 1], latest);
           }
-        }
-        float m[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          m[i] = s[i][0];
-#pragma unroll
-          for (int c = 1; c < 32; ++c) m[i] = fmaxf(m[i], s[i][c]);
-        }
-        const float latest = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-        // (no for a row that has seen nothing yet; rows behind the last one are nobody's and decide nothing)
-        const bool rises = tid < rows && (latest - top) * a.scale_log2 > kTreeSlack;
-        if (__any_sync(0xffffffffu, rises)) {
-          const float up = fmaxf(latest, top);
-          const float fade = up == -INFINITY ? 1.f : exp2_approx((top - up) * a.scale_log2);
-          top = up;
-          sum *= fade;
-          if (!fresh) {
-            ok = bounded_wait_warp(&bars->aborted, a.status, &bars->o_done, uint32_t(it - 1) & 1);
-            tc_fence_after();
+          // (no for a row that has seen nothing yet; rows behind the last one are nobody's and decide nothing)
+          const bool rises = row < rows && (latest - top) * a.scale_log2 > kTreeSlack;
+          if (__any_sync(0xffffffffu, rises)) {
+            const float up = fmaxf(latest, top);
+            const float fade = up == -INFINITY ? 1.f : exp2_approx((top - up) * a.scale_log2);
+            top = up;
+            sum *= fade;
+            if (it - piece >= 2) {  // (the stream's last outputs are done: these scores were issued behind them)
 #pragma unroll 1
-            for (int i = 0; i < D / 32; ++i) {
-              float o[32];
-              tmem_ld32(o_at + 32 * i, o);
-              tmem_ld_wait();
-              tmem_landed(o);
-              uint32_t r[32];
+              for (int i = 0; i < D / 32; ++i) {
+                float o[32];
+                tmem_ld32(o_at + 32 * i, o);
+                tmem_ld_wait();
+                tmem_landed(o);
+                uint32_t r[32];
 #pragma unroll
-              for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(o[c] * fade);
-              tmem_st16(o_at + 32 * i, r);
-              tmem_st16(o_at + 32 * i + 16, r + 16);
+                for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(o[c] * fade);
+                tmem_st16(o_at + 32 * i, r);
+                tmem_st16(o_at + 32 * i + 16, r + 16);
+              }
             }
-            tmem_st_wait();
           }
-        }
-        const float base = top == -INFINITY ? 0.f : top * a.scale_log2;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+          const float base = top == -INFINITY ? 0.f : top * a.scale_log2;
+          const uint64_t minus = pair_of(-base, -base);
+          uint64_t part[2] = {0, 0};
+          tmem_ld32(s_at, s[0]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t p[16];
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const float x = exp2_approx(fmaf(s[i][2 * c], a.scale_log2, -base));
-            const float y = exp2_approx(fmaf(s[i][2 * c + 1], a.scale_log2, -base));
-            part[c & 3] += x + y;
-            p[c] = pack2<T>(x, y);  // rounded to the type of v: half a step of each weight, averaged over the keys
+          for (int i = 0; i < 4; ++i) {
+            tmem_ld_wait();
+            tmem_landed(s[i & 1]);
+            if (i < 3) tmem_ld32(s_at + 32 * (i + 1), s[(i + 1) & 1]);
+            unseen(i, s[i & 1]);
+            uint32_t p[16];
+            scores_exp<T>(s[i & 1], scale, minus, p, part);
+            tmem_st16(s_at + 16 * i, p);  // (over scores that have been read)
           }
-          tmem_st16(s_at + 16 * i, p);
+          sum += pairs_sum(part);
+          tmem_st_wait();
+          tc_fence_before();
         }
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
-        tmem_st_wait();
-        tc_fence_before();
+        mbar_arrive(&bars->p_full[t]);
       }
-      // Where the outputs are read next, the block before has to be known done, and while the barrier cannot be two phases on: the
-      // scores of this block only say that the block before that one is.
-      const bool piece_ends = segment_ends || it + 1 == n_tiles;
-      if (piece_ends && it) ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->o_done, uint32_t(it - 1) & 1);
-      mbar_arrive(&bars->p_full[it & 1]);
-      fresh = false;
 
       if (piece_ends) {
-        const int64_t segment_begin = seq_begin + int64_t(now.part) * now.tiles;
-        const bool whole = piece_begin == segment_begin && segment_ends;
-        ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->o_done, uint32_t(it) & 1);
+        // The stream's last block of this segment, if it has one. Its scores were issued behind the outputs of the block before it, so
+        // the barrier is not two phases behind, and not ahead: the next outputs need this warp's weights.
+        const int last_own = (it & 1) == t ? it : it - 1;
+        if (last_own >= piece) ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->o_done[t], uint32_t(last_own >> 1) & 1);
         tc_fence_after();
+        bars->tops[t][row] = top;
+        bars->sum_of[t][row] = sum;
+        warps_sync(1, 2 * kTreeRows);
+        const int64_t segment_begin = seq_begin + int64_t(now.part) * now.tiles, piece_begin = begin + piece;
+        const bool whole = piece_begin == segment_begin && segment_ends;
         // A block has at most two pieces that are not whole: one that begins with its segment, one that does not.
         float* mine = a.partial + (2 * size_t(blockIdx.x) + (piece_begin == segment_begin ? 1 : 0)) * S::kSlot;
-        if (ok && 32 * warp < rows) {
-          const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;  // a row that sees nothing: zeros
-          T* to = static_cast<T*>(a.out) + (int64_t(now.seq) * a.drafted + token) * a.out_stride + int64_t(head) * D;
+        if (ok && lane_row < rows) {
+          const float m0 = bars->tops[0][row], m1 = bars->tops[1][row], up = fmaxf(m0, m1), zero = up == -INFINITY ? 0.f : up;
+          float f[2] = {exp2_approx((m0 - zero) * a.scale_log2), exp2_approx((m1 - zero) * a.scale_log2)};
+          const float l = bars->sum_of[0][row] * f[0] + bars->sum_of[1][row] * f[1];
+          if (whole) {
+            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row that sees nothing: zeros
+            f[0] *= inv;
+            f[1] *= inv;
+          } else if (t == 0) {
+            mine[D * kTreeRows + row] = up;
+            mine[(D + 1) * kTreeRows + row] = l;
+          }
+          T* to = static_cast<T*>(a.out) + (token0 + row / a.group) * a.out_stride + int64_t(head0 + row % a.group) * D;
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            float o[32];
-            tmem_ld32(o_at + 32 * i, o);
-            tmem_ld_wait();
-            tmem_landed(o);
-            if (whole) {
-              if (tid < rows) {
+          for (int i = t * (D / 64); i < (t + 1) * (D / 64); ++i) {
+            float o[32], x[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[c] = 0.f;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              if (it == piece && w != (it & 1)) continue;  // one block: one stream
+              tmem_ld32(tmem + lanes + kO + 128 * w + 32 * i, o);
+              tmem_ld_wait();
+              tmem_landed(o);
+#pragma unroll
+              for (int c = 0; c < 32; ++c) x[c] = fmaf(o[c], f[w], x[c]);
+            }
+            if (row < rows) {
+              if (whole) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                   uint4 v;
-                  v.x = pack2<T>(o[8 * c] * inv, o[8 * c + 1] * inv);
-                  v.y = pack2<T>(o[8 * c + 2] * inv, o[8 * c + 3] * inv);
-                  v.z = pack2<T>(o[8 * c + 4] * inv, o[8 * c + 5] * inv);
-                  v.w = pack2<T>(o[8 * c + 6] * inv, o[8 * c + 7] * inv);
+                  v.x = pack2<T>(x[8 * c], x[8 * c + 1]);
+                  v.y = pack2<T>(x[8 * c + 2], x[8 * c + 3]);
+                  v.z = pack2<T>(x[8 * c + 4], x[8 * c + 5]);
+                  v.w = pack2<T>(x[8 * c + 6], x[8 * c + 7]);
                   *reinterpret_cast<uint4*>(to + 32 * i + 8 * c) = v;
                 }
-              }
-            } else if (tid < rows) {
+              } else {
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<float4*>(mine + tid * D + 32 * i + 4 * c) = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+                for (int c = 0; c < 8; ++c)
+                  *reinterpret_cast<float4*>(mine + ((8 * i + c) * kTreeRows + row) * 4) = make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+              }
             }
             __syncwarp();  // (the next read of tensor memory takes the whole warp)
-          }
-          if (!whole) {
-            mine[D * kTreeRows + tid] = top;
-            mine[(D + 1) * kTreeRows + tid] = sum;
           }
           tc_fence_before();
         }
         if (!whole) {
           __threadfence();
-          warps_sync(1, kTreeRows);
+          warps_sync(1, 2 * kTreeRows);
           const int64_t segment_end = segment_begin + now.tiles;
           const int first = int(((segment_begin + 1) * blocks - 1) / total), last = int((segment_end * blocks - 1) / total);
           if (tid == 0) {
@@ -510,38 +561,36 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
             bars->last_block = atomicAdd(counter, 1) == last - first;
             if (bars->last_block) *counter = 0;  // for the next call
           }
-          warps_sync(1, kTreeRows);
+          warps_sync(1, 2 * kTreeRows);
           if (bars->last_block) {
             __threadfence();
-            const int64_t token0 = int64_t(now.seq) * a.drafted + (now.part % a.row_tiles) * a.tile_tokens;
-            for (int i = tid; i < rows * (D / 4); i += kTreeRows) {
-              const int r = i / (D / 4), c = 4 * (i % (D / 4));
+            for (int i = tid; i < rows * (D / 4); i += 2 * kTreeRows) {
+              const int r = i % rows, c = i / rows;
               // Piece b of the segment is block b's: the first begins with the segment, the others do not.
-              const float* piece = a.partial + (2 * size_t(first) + 1) * S::kSlot;
-              float up = __ldcg(piece + D * kTreeRows + r);
-#pragma unroll 4
+              float up = __ldcg(a.partial + (2 * size_t(first) + 1) * S::kSlot + D * kTreeRows + r);
+#pragma unroll 8
               for (int b = first + 1; b <= last; ++b) up = fmaxf(up, __ldcg(a.partial + 2 * size_t(b) * S::kSlot + D * kTreeRows + r));
               if (up == -INFINITY) up = 0.f;  // a row that sees nothing
               float l = 0.f;
               float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
               for (int b = first; b <= last; ++b) {
-                piece = a.partial + (2 * size_t(b) + (b == first ? 1 : 0)) * S::kSlot;
-                const float4 o = __ldcg(reinterpret_cast<const float4*>(piece + r * D + c));
-                const float f = exp2_approx((__ldcg(piece + D * kTreeRows + r) - up) * a.scale_log2);
-                l = fmaf(__ldcg(piece + (D + 1) * kTreeRows + r), f, l);
+                const float* from = a.partial + (2 * size_t(b) + (b == first ? 1 : 0)) * S::kSlot;
+                const float4 o = __ldcg(reinterpret_cast<const float4*>(from + (c * kTreeRows + r) * 4));
+                const float f = exp2_approx((__ldcg(from + D * kTreeRows + r) - up) * a.scale_log2);
+                l = fmaf(__ldcg(from + (D + 1) * kTreeRows + r), f, l);
                 x.x = fmaf(o.x, f, x.x);
                 x.y = fmaf(o.y, f, x.y);
                 x.z = fmaf(o.z, f, x.z);
                 x.w = fmaf(o.w, f, x.w);
               }
               const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-              T* to = static_cast<T*>(a.out) + (token0 + r / a.group) * a.out_stride + int64_t(head0 + r % a.group) * D + c;
+              T* to = static_cast<T*>(a.out) + (token0 + r / a.group) * a.out_stride + int64_t(head0 + r % a.group) * D + 4 * c;
               *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
             }
           }
         }
-        piece_begin = begin + it + 1;
+        warps_sync(1, 2 * kTreeRows);  // both streams' outputs have been read
       }
       if (it + 1 < n_tiles) {
         const int seq = now.seq, tiles = now.tiles;
@@ -554,19 +603,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
   __syncthreads();
   tc_fence_after();
   if (bars->aborted && tid == 0) {  // copies that nobody waited for
-    const int q_issued = bars->q_issued;
+    const int issued = bars->in_flight, q_issued = bars->q_issued;
+    for (int i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
+      for (uint32_t n = 0; n < (1u << 16) && !mbar_try_wait_hint(&bars->full[i % kStages], uint32_t(i / kStages) & 1); ++n) {}
     for (int i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i)
       for (uint32_t n = 0; n < (1u << 16) && !mbar_try_wait_hint(&bars->q_full[i & 1], uint32_t(i / 2) & 1); ++n) {}
   }
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 template <class T, int D>
-cudaError_t launch_tree(const TreeArgs& a, const CUtensorMap& q_map, cudaStream_t s) {
+cudaError_t launch_tree(const TreeArgs& a, const TreeMaps& maps, cudaStream_t s) {
   static PerDeviceOnce once;
   const cudaError_t e = per_device_once(once, [] { return opt_in_smem(tree_kernel<T, D>, TreeShape<D>::kSmem); });
   if (e != cudaSuccess) return e;
-  return launch_pdl(tree_kernel<T, D>, dim3(unsigned(sm_count())), dim3(kTreeThreads), size_t(TreeShape<D>::kSmem), s, a, q_map);
+  return launch_pdl(tree_kernel<T, D>, dim3(unsigned(sm_count())), dim3(kTreeThreads), size_t(TreeShape<D>::kSmem), s, a, maps);
 }
 
 // Drafted tokens of a row tile: whole tokens, as many as 128 rows hold.
@@ -586,6 +637,15 @@ bool tree_shape_ok(int n_seqs, int drafted, int heads, int kv_heads, int dim) {
          heads % kv_heads == 0 && heads / kv_heads <= kTreeRows && (dim == 64 || dim == 128);
 }
 
+// The cache's slots as rows of kv_heads * dim values, in boxes of `box` slots x 64 values; slots behind the last one read as zeros.
+bool tree_map_cache(CUtensorMap* map, const void* base, bool bf16, int64_t slots, int row, int box_slots) {
+  const cuuint64_t dims[2] = {cuuint64_t(row), cuuint64_t(slots)}, strides[1] = {cuuint64_t(row) * 2};
+  const cuuint32_t box[2] = {64, cuuint32_t(box_slots)}, elem[2] = {1, 1};
+  return encode_tiled_fn()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                           const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 // [tokens][heads][dim] in boxes of a row tile: its tokens x the heads of a group x 64 values.
 bool tree_map_q(CUtensorMap* map, const void* base, bool bf16, int dim, int heads, int64_t tokens, int64_t stride, int group, int tile) {
   const cuuint64_t dims[3] = {cuuint64_t(dim), cuuint64_t(heads), cuuint64_t(tokens)};
@@ -669,12 +729,18 @@ int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int3
   a.tile_tokens = tree_tile_tokens(drafted, a.group);
   a.row_tiles = tree_row_tiles(drafted, a.group);
   const bool bf = cache->dtype == FB_DT_BF16;
-  CUtensorMap q_map;
-  if (!tree_map_q(&q_map, q, bf, dim, heads, int64_t(n_seqs) * drafted, q_stride, a.group, a.tile_tokens))
+  a.box = cache->page_size & -cache->page_size;  // slots that start on a multiple of it lie in one page
+  if (a.box > kTreeKeys) a.box = kTreeKeys;
+  if (a.box < kTreeMinBox) a.box = 0;
+  const int64_t slots = cache->n_pages * cache->page_size;
+  TreeMaps maps;
+  if (!tree_map_q(&maps.q, q, bf, dim, heads, int64_t(n_seqs) * drafted, q_stride, a.group, a.tile_tokens) ||
+      !tree_map_cache(&maps.k, cache->k, bf, slots, kv * dim, a.box ? a.box : kTreeMinBox) ||
+      !tree_map_cache(&maps.v, cache->v, bf, slots, kv * dim, a.box ? a.box : kTreeMinBox))
     return invalid("attn_tree_decode: cuTensorMapEncodeTiled failed");
   cudaStream_t s = as_stream(stream);
-  const cudaError_t e = dim == 64 ? (bf ? launch_tree<__nv_bfloat16, 64>(a, q_map, s) : launch_tree<__half, 64>(a, q_map, s))
-                                  : (bf ? launch_tree<__nv_bfloat16, 128>(a, q_map, s) : launch_tree<__half, 128>(a, q_map, s));
+  const cudaError_t e = dim == 64 ? (bf ? launch_tree<__nv_bfloat16, 64>(a, maps, s) : launch_tree<__half, 64>(a, maps, s))
+                                  : (bf ? launch_tree<__nv_bfloat16, 128>(a, maps, s) : launch_tree<__half, 128>(a, maps, s));
   const int32_t st = check_launch("attn_tree_decode");
   return st ? st : int32_t(e);
 }
