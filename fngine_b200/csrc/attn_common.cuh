@@ -60,16 +60,45 @@ __device__ __forceinline__ float scores_max(const float (&s)[32], float m) {
   }
   return max3(a, b, c);
 }
+// 2^x of a pair on the multiply-add pipe: x = n + f with n whole and |f| <= 1/2 (adding 1.5 * 2^23 rounds to whole numbers and leaves
+// n in the low bits), a polynomial of degree four for 2^f (minimax by Remez exchange, relative error 2.7e-6), n into the exponent.
+// Below -126 it stays at 2^-126, so not for scores that are masked; NaN does not turn into a number that passes for a weight.
+__device__ __forceinline__ void exp2_poly(uint64_t x2, float& x, float& y) {
+  float a, b;
+  unpair(x2, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  x2 = pair_of(a, b);
+  constexpr float kRound = 12582912.f;
+  const uint64_t t = add2(x2, pair_of(kRound, kRound));
+  const uint64_t f = fma2(add2(t, pair_of(-kRound, -kRound)), pair_of(-1.f, -1.f), x2);
+  uint64_t p = fma2(f, pair_of(0.009570102207362652f, 0.009570102207362652f), pair_of(0.05591785907745361f, 0.05591785907745361f));
+  p = fma2(p, f, pair_of(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
+  float n0, n1;
+  unpair(t, n0, n1);
+  unpair(p, a, b);
+  x = __uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23));
+  y = __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23));
+}
 // 32 weights 2^(scale s - base) as pairs of T (rounded to the type of v: half a step of each weight, averaged over the keys) and, before
-// that rounding, added to `sum` (a pair of partial sums).
-template <class T>
+// that rounding, added to `sum` (a pair of partial sums). MIXED: six of sixteen pairs by exp2_poly. The exponential unit takes eight
+// cycles per warp and instruction, 2048 for the two softmax warps of a scheduler per block of 128 keys; with six of sixteen
+// elsewhere it and the issue slots are both done in about 1300.
+template <class T, bool MIXED>
 __device__ __forceinline__ void scores_exp(const float (&s)[32], uint64_t scale, uint64_t minus_base, uint32_t (&p)[16], uint64_t (&sum)[2]) {
 #pragma unroll
   for (int c = 0; c < 16; ++c) {
     float x, y;
-    unpair(fma2(pair_of(s[2 * c], s[2 * c + 1]), scale, minus_base), x, y);
-    x = exp2_approx(x);
-    y = exp2_approx(y);
+    const uint64_t x2 = fma2(pair_of(s[2 * c], s[2 * c + 1]), scale, minus_base);
+    if (MIXED && (c % 8 == 1 || c % 8 == 4 || c % 8 == 6)) {
+      exp2_poly(x2, x, y);
+    } else {
+      unpair(x2, x, y);
+      x = exp2_approx(x);
+      y = exp2_approx(y);
+    }
     sum[c & 1] = add2(sum[c & 1], pair_of(x, y));
     p[c] = pack2<T>(x, y);
   }
@@ -78,6 +107,16 @@ __device__ __forceinline__ float pairs_sum(const uint64_t (&sum)[2]) {
   float a, b;
   unpair(add2(sum[0], sum[1]), a, b);
   return a + b;
+}
+
+// Moves a warpgroup's registers per thread up or down; the shares have to add up to what the block was launched with.
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // ------------------------------------------------------------------------------ copies and products
@@ -97,18 +136,30 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Shared-memory operand descriptors (128-byte swizzle, 8-row groups 1024 bytes apart, descriptor version 1) are given by their low
+// words: address / 16, and in the high half `lead`: for a tile whose rows run along K (Q, K) not used (1); for V, whose rows run along
+// N, the distance of its two 64-value parts / 16. The lane that issues steps through a tile with 32-bit adds, everything else is a
+// constant: an instruction whose operands have to be put together first took 125 cycles beside two busy softmax warps, 1000 for the
+// eight of a tile, against the 528 that the tensor core works on them.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t umma_desc_lo(uint32_t addr, uint32_t lead) { return ((addr & 0x3FFFFu) >> 4) | (lead << 16); }
+// D[tmem] (+)= A[smem] B[smem] and A[tmem] B[smem], 16 of K.
+template <uint32_t IDESC>
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "n"(IDESC), "r"(uint32_t(accumulate)), "n"(kDescHi)
       : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+template <uint32_t IDESC>
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "n"(IDESC), "r"(uint32_t(accumulate)), "n"(kDescHi)
       : "memory");
 }
 // 32 columns of the warp's 32 lanes; the values are there after tmem_ld_wait and tmem_landed.
@@ -138,12 +189,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-// Shared-memory operand descriptors, 128-byte swizzle, 8-row groups 1024 bytes apart, descriptor version 1. `lead`: for a
-// tile whose rows run along K (Q, K) not used (1); for V, whose rows run along N, the distance of its two 64-value parts.
-__device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lead) {
-  return uint64_t((addr & 0x3FFFFu) >> 4) | (uint64_t(lead) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
-         (uint64_t(2) << 61);
 }
 
 // Bounded wait. A wait that ran out is recorded, and every later one ends at once.

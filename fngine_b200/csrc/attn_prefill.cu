@@ -5,9 +5,10 @@
 // One pass over the keys per query tile with a running maximum and sum. A block takes 256 queries of one head as two tiles of
 // 128 (TMEM lanes) and goes through the keys 128 at a time:
 //   S = Q K^T   tcgen05 kind::f16, both operands in shared memory, fp32 S in tensor memory (128 columns per tile)
-//   P = 2^(c S - c m) in the type of v, written over S by the tile's four softmax warps, a thread per row: no shuffles
+//   P = 2^(c S - c m) in the type of v, to tensor memory by the tile's four softmax warps, a thread per row: no shuffles
 //   O += P V    P from tensor memory, V as it lies in memory (keys x head_dim: the operand's N-major form), fp32 O in tensor memory
-// The two tiles are half a step apart: while one is in its softmax, the tensor core has the other's two products.
+// The two tiles are half a step apart and take turns with S, which a softmax thread has in registers 70 cycles after it is complete:
+// from then on the other tile's scores are made there, so neither softmax waits for the tensor core.
 // m is the maximum that the exponents refer to, not the latest one: it moves up (and O is multiplied) only when a row's scores
 // rise above it by more than 2^8, which leaves every weight at most 256 and the sum in fp32 range. Normally that is
 // the first block alone, so O stays in tensor memory untouched.
@@ -43,7 +44,7 @@ struct PfMaps {
 };
 
 struct PfBars {
-  uint64_t q_full[2], s_full[2], p_full[2], o_done[2], full[8], empty[8], drained;
+  uint64_t q_full[2], s_full[2], s_free[2], p_full[2], o_done[2], full[8], empty[8], drained;
   uint32_t tmem;
   int aborted;
   int issued;  // copies of keys and values
@@ -110,6 +111,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->q_full[i], 1);
       mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->s_free[i], kPfRows);
       mbar_init(&bars->p_full[i], kPfRows);
       mbar_init(&bars->o_done[i], 1);
     }
@@ -127,9 +129,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
   tc_fence_after();
   // (not before the allocation: a block of the next kernel that took tensor memory and then waited for this one would hold it up)
   pdl_launch_dependents();
-  const uint32_t tmem = bars->tmem;
-  constexpr uint32_t kS = 0, kO = 256;  // tile i: S in columns 128 i, O in 256 + 128 i
+  // All 512 columns: their address is 0, and every address in tensor memory a constant.
+  if (bars->tmem != 0 && tid == 0 && a.status) atomicMax(a.status, uint32_t(FB_STATUS_BAD_WORK));
+  constexpr uint32_t kS = 0, kP = 128, kO = 256;  // S; tile i: P in columns 128 + 64 i, O in 256 + 128 i
 
+  // 256 threads x 208 and 128 x 88 registers are the 384 x 168 of the launch.
+  if (warp >= 8) {
+  regs_down<88>();
   if (warp == 9) {
     // ------------------------------------------------------------------ copies
     if (lane == 0) {
@@ -157,17 +163,21 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       ok = ok && bounded_wait_warp(&bars->aborted, a.status, bar, parity);
     };
+    int held_by = -1, held_at = 0;  // whose scores S holds
     auto scores = [&](int t, int j) {
       const int slot = (2 * j) % kStages;
+      if (held_by >= 0) wait(&bars->s_free[held_by], uint32_t(held_at) & 1);
+      held_by = t;
+      held_at = j;
       wait(&bars->full[slot], uint32_t(2 * j / kStages) & 1);
       if (!ok) return;
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t qd = umma_desc(smem_u32(q_tiles + t * S::kTileBytes), 1), kd = umma_desc(smem_u32(ring + slot * S::kTileBytes), 1);
+        const uint32_t qd = umma_desc_lo(smem_u32(q_tiles + t * S::kTileBytes), 1), kd = umma_desc_lo(smem_u32(ring + slot * S::kTileBytes), 1);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint32_t at = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
-          umma_ss(tmem + kS + 128 * t, qd + at, kd + at, kIdescQk, k > 0);
+          umma_ss<kIdescQk>(kS, qd + at, kd + at, k > 0);
         }
         umma_commit(&bars->s_full[t]);
       }
@@ -192,10 +202,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
       }
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t vd = umma_desc(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
+        const uint32_t vd = umma_desc_lo(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4), d = kO + 128 * t, p = kP + 64 * t;
+        umma_ts<kIdescPv>(d, p, vd, j > 0);
 #pragma unroll
-        for (int k = 0; k < kPfRows / 16; ++k)
-          umma_ts(tmem + kO + 128 * t, tmem + kS + 128 * t + 8 * k, vd + k * (2048 >> 4), kIdescPv, j > 0 || k > 0);
+        for (int k = 1; k < kPfRows / 16; ++k) umma_ts<kIdescPv>(d, p + 8 * k, vd + k * (2048 >> 4), true);
         umma_commit(&bars->o_done[t]);
       }
       __syncwarp();
@@ -211,29 +221,29 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
       scores(1, 0);
     }
     release(0);
+    // The next scores of a tile are made while its softmax still works on the last ones, as soon as the other tile has taken its own.
     for (int j = 0; j < blocks && ok; ++j) {
-      if (j < blocks0) {
-        outputs(0, j);
-        if (j + 1 < blocks0) scores(0, j + 1);
-      }
-      if (j < blocks1) {
-        outputs(1, j);
-        if (j + 1 < blocks1) scores(1, j + 1);
-      }
-      release(2 * j + 1);
+      if (j + 1 < blocks0) scores(0, j + 1);
+      if (j < blocks0) outputs(0, j);
+      if (j + 1 < blocks1) scores(1, j + 1);
       if (j + 1 < blocks) release(2 * j + 2);
+      if (j < blocks1) outputs(1, j);
+      release(2 * j + 1);
     }
     // Nothing issued here is still running when the tensor memory is given back.
     if (elect_one()) umma_commit(&bars->drained);
     __syncwarp();
     for (uint32_t n = 0; n < (1u << 16) && !__all_sync(0xffffffffu, mbar_try_wait_hint(&bars->drained, 0)); ++n) {}
-  } else if (warp < 8) {
+  }
+  } else {
+    regs_up<208>();
     // ------------------------------------------------------------------ softmax
     const int t = warp >> 2, row = tid & 127;
     const int n = t ? blocks1 : blocks0;
     const uint32_t lanes = uint32_t(warp & 3) << 21;  // (32 (warp % 4)) << 16
-    const uint32_t s_at = tmem + lanes + kS + 128 * t, o_at = tmem + lanes + kO + 128 * t;
+    const uint32_t s_at = lanes + kS, p_at = lanes + kP + 64 * t, o_at = lanes + kO + 128 * t;
     const bool real = row0 + t * kPfRows + row < length;
+    const uint64_t scale = pair_of(a.scale_log2, a.scale_log2);
     float top = -INFINITY, sum = 0.f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
@@ -246,6 +256,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
       tmem_ld_wait();
 #pragma unroll
       for (int i = 0; i < 4; ++i) tmem_landed(s[i]);
+      tc_fence_before();
+      mbar_arrive(&bars->s_free[t]);
       if (j == n - 1) {  // the diagonal
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -253,25 +265,21 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
           for (int c = 0; c < 32; ++c)
             if (32 * i + c > row) s[i][c] = -INFINITY;
       }
-      float m[4];
+      float latest = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        m[i] = s[i][0];
-#pragma unroll
-        for (int c = 1; c < 32; ++c) m[i] = fmaxf(m[i], s[i][c]);
-      }
-      const float latest = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+      for (int i = 0; i < 4; ++i) latest = scores_max(s[i], latest);
       // (always in the first block; rows behind the sequence are nobody's and decide nothing)
       const bool rises = real && (latest - top) * a.scale_log2 > kPfSlack;
+      // P and O are free: the block before's product is done.
+      if (j > 0) ok = bounded_wait_warp(&bars->aborted, a.status, &bars->o_done[t], uint32_t(j - 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
       if (__any_sync(0xffffffffu, rises)) {
         const float up = fmaxf(latest, top);
         const float fade = exp2_approx((top - up) * a.scale_log2);
         top = up;
         sum *= fade;
         if (j > 0) {
-          ok = bounded_wait_warp(&bars->aborted, a.status, &bars->o_done[t], uint32_t(j - 1) & 1);
-          if (!ok) break;
-          tc_fence_after();
 #pragma unroll 1
           for (int i = 0; i < D / 32; ++i) {
             float o[32];
@@ -284,24 +292,27 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
             tmem_st16(o_at + 32 * i, r);
             tmem_st16(o_at + 32 * i + 16, r + 16);
           }
-          tmem_st_wait();
         }
       }
       const float base = top * a.scale_log2;
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t minus = pair_of(-base, -base);
+      uint64_t part[2] = {0, 0};
+      if (j == n - 1) {  // (masked scores stay with the exponential unit: exactly zero)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t p[16];
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const float x = exp2_approx(fmaf(s[i][2 * c], a.scale_log2, -base));
-          const float y = exp2_approx(fmaf(s[i][2 * c + 1], a.scale_log2, -base));
-          part[c & 3] += x + y;
-          p[c] = pack2<T>(x, y);  // rounded to the type of v: half a step of each weight, averaged over the keys
+        for (int i = 0; i < 4; ++i) {
+          uint32_t p[16];
+          scores_exp<T, false>(s[i], scale, minus, p, part);
+          tmem_st16(p_at + 16 * i, p);
         }
-        tmem_st16(s_at + 16 * i, p);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t p[16];
+          scores_exp<T, true>(s[i], scale, minus, p, part);
+          tmem_st16(p_at + 16 * i, p);
+        }
       }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      sum += pairs_sum(part);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&bars->p_full[t]);
@@ -351,7 +362,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
     for (int i = 0; i < (blocks1 ? 2 : 1); ++i)
       for (uint32_t n = 0; n < (1u << 16) && !mbar_try_wait_hint(&bars->q_full[i], 0); ++n) {}
   }
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars->tmem), "r"(512) : "memory");
 }
 
 // [tokens][heads][dim] in boxes of 128 tokens x 64 values of one head; tokens behind the last one read as zeros.

@@ -228,7 +228,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
   tc_fence_after();
   // (not before the allocation: a block of the next kernel that took tensor memory and then waited for this one would hold it up)
   pdl_launch_dependents();
-  const uint32_t tmem = bars->tmem;
+  // All 512 columns: their address is 0, and every address in tensor memory a constant.
+  if (bars->tmem != 0 && tid == 0) atomicMax(a.status, uint32_t(FB_STATUS_BAD_WORK));
   constexpr uint32_t kS = 0, kO = 256;  // stream t: S in columns 128 t, O in 256 + 128 t
 
   if (warp >= 8 && warp < 12) {
@@ -346,11 +347,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
         fence_proxy_async();  // (the copies were made by the generic proxy, the product reads through the other)
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t qd = umma_desc(smem_u32(q_tiles + b * S::kTileBytes), 1), kd = umma_desc(smem_u32(ring + slot * S::kTileBytes), 1);
+          const uint32_t qd = umma_desc_lo(smem_u32(q_tiles + b * S::kTileBytes), 1), kd = umma_desc_lo(smem_u32(ring + slot * S::kTileBytes), 1);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t at = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
-            umma_ss(tmem + kS + 128 * (it & 1), qd + at, kd + at, kIdescQk, k > 0);
+            umma_ss<kIdescQk>(kS + 128 * (it & 1), qd + at, kd + at, k > 0);
           }
           umma_commit(&bars->s_full[it & 1]);
           umma_commit(&bars->empty[slot]);
@@ -375,10 +376,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
       fence_proxy_async();
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t vd = umma_desc(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
+        const uint32_t vd = umma_desc_lo(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
+        const uint32_t d = kO + 128 * (it & 1), p = kS + 128 * (it & 1);
+        umma_ts<kIdescPv>(d, p, vd, it - piece >= 2);
 #pragma unroll
-        for (int k = 0; k < kTreeKeys / 16; ++k)
-          umma_ts(tmem + kO + 128 * (it & 1), tmem + kS + 128 * (it & 1) + 8 * k, vd + k * (2048 >> 4), kIdescPv, it - piece >= 2 || k > 0);
+        for (int k = 1; k < kTreeKeys / 16; ++k) umma_ts<kIdescPv>(d, p + 8 * k, vd + k * (2048 >> 4), true);
         umma_commit(&bars->o_done[it & 1]);
         umma_commit(&bars->empty[slot]);
       }
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
     // ------------------------------------------------------------------ softmax: thread = row, warps 4 t .. 4 t + 3 take stream t
     const int t = warp >> 2, row = tid & (kTreeRows - 1), lane_row = 32 * (warp & 3);
     const uint32_t lanes = uint32_t(lane_row) << 16;
-    const uint32_t s_at = tmem + lanes + kS + 128 * t, o_at = tmem + lanes + kO + 128 * t;
+    const uint32_t s_at = lanes + kS + 128 * t, o_at = lanes + kO + 128 * t;
     const uint64_t scale = pair_of(a.scale_log2, a.scale_log2);
     bool ok = true, fresh = true;
     float top = -INFINITY, sum = 0.f;
@@ -480,7 +482,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
             if (i < 3) tmem_ld32(s_at + 32 * (i + 1), s[(i + 1) & 1]);
             unseen(i, s[i & 1]);
             uint32_t p[16];
-            scores_exp<T>(s[i & 1], scale, minus, p, part);
+            scores_exp<T, false>(s[i & 1], scale, minus, p, part);
             tmem_st16(s_at + 16 * i, p);  // (over scores that have been read)
           }
           sum += pairs_sum(part);
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
               if (it == piece && w != (it & 1)) continue;  // one block: one stream
-              tmem_ld32(tmem + lanes + kO + 128 * w + 32 * i, o);
+              tmem_ld32(lanes + kO + 128 * w + 32 * i, o);
               tmem_ld_wait();
               tmem_landed(o);
 #pragma unroll
@@ -609,7 +611,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
     for (int i = q_issued > 2 ? q_issued - 2 : 0; i < q_issued; ++i)
       for (uint32_t n = 0; n < (1u << 16) && !mbar_try_wait_hint(&bars->q_full[i & 1], uint32_t(i / 2) & 1); ++n) {}
   }
-  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars->tmem), "r"(512) : "memory");
 }
 
 template <class T, int D>
