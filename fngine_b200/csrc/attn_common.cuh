@@ -193,7 +193,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
 
 // Bounded wait. A wait that ran out is recorded, and every later one ends at once.
 __device__ __forceinline__ bool bounded_wait(int* aborted, uint32_t* status, uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
+  // (a plain probe first: a try that may suspend takes some 200 cycles longer even when the phase is complete)
+  if (mbar_test_wait(bar, parity)) return true;
   for (uint32_t i = 0; i < (1u << 21); ++i) {
     if (mbar_try_wait_hint(bar, parity)) return true;
     if ((i & 31u) == 0u && *static_cast<volatile int*>(aborted)) return false;
@@ -206,6 +207,7 @@ __device__ __forceinline__ bool bounded_wait(int* aborted, uint32_t* status, uin
 // The same for a whole warp: one answer for all lanes. What stands behind a wait (barriers, tensor memory, elections) needs the
 // warp converged, and lanes that left a polling loop one by one are not.
 __device__ __forceinline__ bool bounded_wait_warp(int* aborted, uint32_t* status, uint64_t* bar, uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
   const bool ok = __all_sync(0xffffffffu, bounded_wait(aborted, status, bar, parity));
   __syncwarp();
   return ok;
