@@ -83,16 +83,16 @@ __device__ __forceinline__ void exp2_poly(uint64_t x2, float& x, float& y) {
   y = __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23));
 }
 // 32 weights 2^(scale s - base) as pairs of T (rounded to the type of v: half a step of each weight, averaged over the keys) and, before
-// that rounding, added to `sum` (a pair of partial sums). MIXED: six of sixteen pairs by exp2_poly. The exponential unit takes eight
-// cycles per warp and instruction, 2048 for the two softmax warps of a scheduler per block of 128 keys; with six of sixteen
-// elsewhere it and the issue slots are both done in about 1300.
+// that rounding, added to `sum` (a pair of partial sums). MIXED: two of sixteen pairs by exp2_poly, which takes work off the exponential
+// unit (eight cycles per warp and instruction, 2048 of some 2600 cycles that two softmax warps of a scheduler have for a block of keys)
+// at nine instructions a pair: 8192 tokens 624 us with none, 616 with two, 619 with four, 653 with six.
 template <class T, bool MIXED>
 __device__ __forceinline__ void scores_exp(const float (&s)[32], uint64_t scale, uint64_t minus_base, uint32_t (&p)[16], uint64_t (&sum)[2]) {
 #pragma unroll
   for (int c = 0; c < 16; ++c) {
     float x, y;
     const uint64_t x2 = fma2(pair_of(s[2 * c], s[2 * c + 1]), scale, minus_base);
-    if (MIXED && (c % 8 == 1 || c % 8 == 4 || c % 8 == 6)) {
+    if (MIXED && c % 8 == 4) {
       exp2_poly(x2, x, y);
     } else {
       unpair(x2, x, y);

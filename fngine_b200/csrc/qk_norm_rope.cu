@@ -4,8 +4,8 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w                                   per head of q and k
 //   (a, b) -> (a cos p - b sin p, b cos p + a sin p),  p = position[axis(j)] * inv_freq[j]     frequency j's pair
 //
-// Bound by memory: every value is read once and written once. A block takes a token (or a share of its heads); D / 8 lanes
-// hold a head, 16 bytes each, and a thread's kRows heads are all asked for before the first is used. The angles of a
+// Bound by memory: every value is read once and written once. A block takes a token (or a share of its heads) after the other; D / 8
+// lanes hold a head, 16 bytes each, and the next token's values are on their way while this one's are worked on. The angles of a
 // token are made once per block: the product of position and frequency in 64 bits, reduced to a part of a turn there
 // (a position of a million leaves fp32 no more than four correct digits of the angle), the sine and cosine of the rest in fp32.
 #include "common.cuh"
@@ -19,7 +19,8 @@ namespace fb {
 namespace {
 
 constexpr int kQkThreads = 256;
-constexpr int kQkRows = 4;  // heads a thread has in flight
+constexpr int kQkRows = 4;    // heads a thread works on at a time, and as many are in flight behind them
+constexpr int kQkBlocks = 2;  // per multiprocessor
 
 struct QkArgs {
   const void* in[3];     // q, k, v
@@ -35,6 +36,7 @@ struct QkArgs {
   float eps;
   int weight_dtype, heads, kv_heads, half, adjacent;
   int rows;              // heads of all tensors
+  int tokens;
   int first[3];          // first row of q, k, v
   int section_end[4];
 };
@@ -78,105 +80,137 @@ __device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
 template <class T, int D>
 __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a) {
   constexpr int kLanes = D / 8;                    // lanes of a head
-  constexpr int kPerPass = kQkThreads / kLanes;    // heads of a block per pass
-  __shared__ float cs[2][D / 2];
+  constexpr int kPerPass = kQkThreads / kLanes;    // heads of a block per row of a thread
+  __shared__ float cs[2][2][D / 2];
   pdl_wait_prior();
   pdl_launch_dependents();
-  const int64_t token = blockIdx.x;
   const int l = threadIdx.x % kLanes, e0 = 8 * l, slot_row = threadIdx.x / kLanes;
-  const int step = kPerPass * gridDim.y;
-  // Every thread stays for the shuffles; a row behind the last one is not loaded and not stored.
+  const int step = kPerPass * gridDim.y, first_row = blockIdx.y * kPerPass + slot_row;
   auto which = [&](int row) { return row >= a.first[2] ? 2 : row >= a.first[1] ? 1 : 0; };
-  int64_t kv_row = token;
-  if (a.slots) {
-    kv_row = a.slots[token];
-    if (kv_row < 0 || kv_row >= a.n_slots) kv_row = -1;  // not stored
-  }
-  uint4 raw[kQkRows];
-  auto load = [&](int row0) {
+  // Every thread stays for the shuffles; a row behind the last one is not loaded and not stored.
+  auto load = [&](int64_t token, int row0, uint4 (&raw)[kQkRows]) {
 #pragma unroll
     for (int i = 0; i < kQkRows; ++i) {
       const int row = row0 + i * step;
       if (row < a.rows) {
         const int w = which(row);
-        raw[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.in[w]) + token * a.in_stride[w] +
-                                                 (row - a.first[w]) * D + e0);
+        raw[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.in[w]) + token * a.in_stride[w] + (row - a.first[w]) * D + e0);
+      } else {
+        raw[i] = make_uint4(0, 0, 0, 0);
       }
     }
   };
-  int row0 = blockIdx.y * kPerPass + slot_row;
-  load(row0);
-  for (int j = threadIdx.x; j < a.half; j += kQkThreads) {
+  int64_t token = blockIdx.x;
+  int row0 = first_row;
+  uint4 raw[kQkRows];
+  load(token, row0, raw);
+  // Thread j makes frequency j's sine and cosine.
+  const int j = threadIdx.x;
+  const bool turns_one = j < a.half;
+  const int32_t* positions = nullptr;
+  double turns_per = 0.0;
+  int position = 0;
+  if (turns_one) {
     const int axis = (j >= a.section_end[0]) + (j >= a.section_end[1]) + (j >= a.section_end[2]);
-    const double angle = double(a.positions[axis * a.axis_stride + token]) * double(a.inv_freq[j]);
-    const double turns = angle * 0.15915494309189533577;  // 1 / (2 pi)
-    float s, c;
-    sincospif(2.f * float(turns - rint(turns)), &s, &c);
-    cs[0][j] = c;
-    cs[1][j] = s;
+    positions = a.positions + axis * a.axis_stride;
+    position = positions[token];
+    turns_per = double(a.inv_freq[j]) * 0.15915494309189533577;  // 1 / (2 pi)
   }
-  __syncthreads();
-  // This lane's cosines and sines, one per element: the sine carries the sign of the partner's product.
-  float co[8], si[8];
-  const bool turned = e0 < 2 * a.half;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    co[i] = 1.f;
-    si[i] = 0.f;
-    if (turned) {
-      const int e = e0 + i, j = a.adjacent ? e >> 1 : e < a.half ? e : e - a.half;
-      const bool low = a.adjacent ? !(e & 1) : e < a.half;
-      co[i] = cs[0][j];
-      si[i] = low ? -cs[1][j] : cs[1][j];
-    }
-  }
-  // The lane that holds the partners of an element pair (i, i + rot / 2), in this head's lanes.
-  const int lane = threadIdx.x & 31;
-  const int partner = !turned || a.adjacent ? lane : e0 < a.half ? lane + a.half / 8 : lane - a.half / 8;
+  int64_t slot = a.slots ? a.slots[token] : token;
   float wt[2][8];
 #pragma unroll
   for (int w = 0; w < 2; ++w)
 #pragma unroll
     for (int i = 0; i < 8; ++i) wt[w][i] = a.weight[w] ? weight_at(a.weight[w], a.weight_dtype, e0 + i) : 1.f;
-
-  for (; row0 - slot_row < a.rows; row0 += kQkRows * step) {
-    if (row0 - slot_row != int(blockIdx.y) * kPerPass) load(row0);
+  const bool turned = e0 < 2 * a.half;
+  // The lane that holds the partners of an element pair (i, i + rot / 2), in this head's lanes.
+  const int lane = threadIdx.x & 31;
+  const int partner = !turned || a.adjacent ? lane : e0 < a.half ? lane + a.half / 8 : lane - a.half / 8;
+  float co[8], si[8];
+  int buffer = 0;
+  bool fresh = true;
+  for (;;) {
+    if (fresh) {
+      // This lane's cosines and sines, one per element: the sine carries the sign of the partner's product.
+      if (turns_one) {
+        const double turns = double(position) * turns_per;
+        float s, c;
+        sincospif(2.f * float(turns - rint(turns)), &s, &c);
+        cs[buffer][0][j] = c;
+        cs[buffer][1][j] = s;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        co[i] = 1.f;
+        si[i] = 0.f;
+        if (turned) {
+          const int e = e0 + i, f = a.adjacent ? e >> 1 : e < a.half ? e : e - a.half;
+          const bool low = a.adjacent ? !(e & 1) : e < a.half;
+          co[i] = cs[buffer][0][f];
+          si[i] = low ? -cs[buffer][1][f] : cs[buffer][1][f];
+        }
+      }
+      buffer ^= 1;
+    }
+    // What comes after these rows is asked for before they are worked on.
+    int64_t next_token = token, next_slot = slot;
+    int next_row = row0 + kQkRows * step;
+    fresh = next_row - slot_row >= a.rows;  // (block-uniform)
+    if (fresh) {
+      next_token += gridDim.x;
+      next_row = first_row;
+    }
+    const bool more = next_token < a.tokens;
+    uint4 next_raw[kQkRows];
+    if (more) {
+      load(next_token, next_row, next_raw);
+      if (fresh) {
+        if (turns_one) position = positions[next_token];
+        next_slot = a.slots ? a.slots[next_token] : next_token;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kQkRows; ++i) {
       const int row = row0 + i * step;
       if (row - slot_row >= a.rows) break;  // (block-uniform)
       const int w = row < a.rows ? which(row) : 2;
       float x[8];
-      uint4 packed = raw[i];
-      if (row >= a.rows) packed = make_uint4(0, 0, 0, 0);
-      unpack8<T>(packed, x);
+      unpack8<T>(raw[i], x);
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(x[j], x[j], sum);
+      for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
 #pragma unroll
       for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
       const bool norm = w < 2 && a.weight[w];
       const float r = norm ? rsqrtf(sum * (1.f / D) + a.eps) : 1.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= r * (w == 1 ? wt[1][j] : wt[0][j]);
+      for (int e = 0; e < 8; ++e) x[e] *= r * (w == 1 ? wt[1][e] : wt[0][e]);
       float y[8];
       if (a.adjacent) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = fmaf(x[j], co[j], x[j ^ 1] * si[j]);
+        for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], co[e], x[e ^ 1] * si[e]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float p = __shfl_sync(0xffffffffu, x[j], partner);
-          y[j] = fmaf(x[j], co[j], turned ? p * si[j] : 0.f);
+        for (int e = 0; e < 8; ++e) {
+          const float p = __shfl_sync(0xffffffffu, x[e], partner);
+          y[e] = fmaf(x[e], co[e], turned ? p * si[e] : 0.f);
         }
       }
       if (row < a.rows) {
-        const uint4 v = w == 2 ? packed : pack8<T>(y);
-        const int64_t to = w == 0 ? token : kv_row;
+        const uint4 v = w == 2 ? raw[i] : pack8<T>(y);
+        // (a slot outside of the cache is not stored)
+        const int64_t to = w == 0 ? token : !a.slots || (slot >= 0 && slot < a.n_slots) ? slot : -1;
         if (to >= 0)
           *reinterpret_cast<uint4*>(static_cast<T*>(a.out[w]) + to * a.out_stride[w] + (row - a.first[w]) * D + e0) = v;
       }
     }
+    if (!more) break;
+#pragma unroll
+    for (int i = 0; i < kQkRows; ++i) raw[i] = next_raw[i];
+    token = next_token;
+    slot = next_slot;
+    row0 = next_row;
   }
 }
 
@@ -272,11 +306,13 @@ int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm
   if (a.slots && a.n_slots <= 0) return invalid("qk_norm_rope: slots without n_slots");
   a.heads = in->heads;
   a.kv_heads = in->kv_heads;
-  // A block per token with up to kQkRows heads per thread and pass; few tokens share their heads among more blocks.
-  const int per_pass = kQkThreads / (dim / 8), passes = (a.rows + per_pass - 1) / per_pass;
+  a.tokens = tokens;
+  // A block per token with up to kQkRows heads per thread and pass, kQkBlocks of them per multiprocessor, each with every so many of
+  // the tokens; few tokens share their heads among more blocks.
+  const int per_pass = kQkThreads / (dim / 8), passes = (a.rows + per_pass - 1) / per_pass, most = kQkBlocks * sm_count();
   int share = 1;
   while (share < passes && tokens * share < sm_count()) share *= 2;
-  const dim3 grid(unsigned(tokens), unsigned(share < passes ? share : passes));
+  const dim3 grid(unsigned(tokens < most ? tokens : most), unsigned(share < passes ? share : passes));
   const cudaError_t e = in->dtype == FB_DT_BF16 ? launch_qk<__nv_bfloat16>(a, dim, grid, as_stream(stream))
                                                 : launch_qk<__half>(a, dim, grid, as_stream(stream));
   const int32_t st = check_launch("qk_norm_rope");
