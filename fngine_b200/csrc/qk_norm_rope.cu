@@ -20,7 +20,8 @@ namespace {
 
 constexpr int kQkThreads = 256;
 constexpr int kQkRows = 4;    // heads a thread works on at a time, and as many are in flight behind them
-constexpr int kQkBlocks = 2;  // per multiprocessor
+constexpr int kQkBlocks = 3;  // per multiprocessor
+constexpr int kQkTile = 4;    // tokens whose angles are made together
 
 struct QkArgs {
   const void* in[3];     // q, k, v
@@ -36,7 +37,7 @@ struct QkArgs {
   float eps;
   int weight_dtype, heads, kv_heads, half, adjacent;
   int rows;              // heads of all tensors
-  int tokens;
+  int tokens, tile;
   int first[3];          // first row of q, k, v
   int section_end[4];
 };
@@ -77,140 +78,155 @@ __device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
   return __half2float(static_cast<const __half*>(w)[i]);
 }
 
+// Norm weight and rotation of a value are two factors, of itself and of its partner in the pair, the same for all heads of a token:
+//   y[e] = r (x[e] own[e] + x[partner(e)] other[e]),   r = rsqrt(mean(x^2) + eps)
+// A block keeps them for the tokens of a tile, in the order in which a warp's lanes read them: 16-byte pieces side by side.
+template <int D>
+struct QkFactors {
+  float4 piece[4][D / 8];  // own 0-3, own 4-7, other 0-3, other 4-7 of each lane's eight values
+  __device__ __forceinline__ void set(int e, float own, float other) {
+    reinterpret_cast<float*>(&piece[(e >> 2) & 1][e >> 3])[e & 3] = own;
+    reinterpret_cast<float*>(&piece[2 + ((e >> 2) & 1)][e >> 3])[e & 3] = other;
+  }
+};
+
 template <class T, int D>
-__global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(const QkArgs a) {
+__global__ void __launch_bounds__(kQkThreads, kQkBlocks) qk_norm_rope_kernel(const QkArgs a) {
   constexpr int kLanes = D / 8;                    // lanes of a head
   constexpr int kPerPass = kQkThreads / kLanes;    // heads of a block per row of a thread
-  __shared__ float cs[2][2][D / 2];
+  constexpr int kAngles = (kQkTile * (D / 2) + kQkThreads - 1) / kQkThreads;  // per thread and tile
+  __shared__ QkFactors<D> factors[2][kQkTile][2];  // of q and k; the next tile's are made while this one's are in use
+  __shared__ float weights[2][D];
   pdl_wait_prior();
   pdl_launch_dependents();
   const int l = threadIdx.x % kLanes, e0 = 8 * l, slot_row = threadIdx.x / kLanes;
-  const int step = kPerPass * gridDim.y, first_row = blockIdx.y * kPerPass + slot_row;
-  auto which = [&](int row) { return row >= a.first[2] ? 2 : row >= a.first[1] ? 1 : 0; };
-  // Every thread stays for the shuffles; a row behind the last one is not loaded and not stored.
-  auto load = [&](int64_t token, int row0, uint4 (&raw)[kQkRows]) {
+  const int tile = a.tile;
+  // This thread's rows, the same of every token. Every thread stays for the shuffles; a row behind the last one is not loaded and not
+  // stored.
+  int kind[kQkRows], off[kQkRows];  // 0 q, 1 k, 2 v, 3 none; values from the token's first
+  bool copies = true;               // nothing but values of v in this warp
 #pragma unroll
-    for (int i = 0; i < kQkRows; ++i) {
-      const int row = row0 + i * step;
-      if (row < a.rows) {
-        const int w = which(row);
-        raw[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.in[w]) + token * a.in_stride[w] + (row - a.first[w]) * D + e0);
-      } else {
-        raw[i] = make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < kQkRows; ++i) {
+    const int row = (i * gridDim.y + blockIdx.y) * kPerPass + slot_row;
+    kind[i] = row >= a.rows ? 3 : row >= a.first[2] ? 2 : row >= a.first[1] ? 1 : 0;
+    off[i] = (row - (kind[i] == 0 ? a.first[0] : kind[i] == 1 ? a.first[1] : a.first[2])) * D + e0;
+    copies &= kind[i] >= 2;
+  }
+  copies = __all_sync(0xffffffffu, copies);
+  auto load = [&](int64_t token, uint4 (&raw)[kQkRows]) {
+    const T* q = static_cast<const T*>(a.in[0]) + token * a.in_stride[0];
+    const T* k = static_cast<const T*>(a.in[1]) + token * a.in_stride[1];
+    const T* v = static_cast<const T*>(a.in[2]) + token * a.in_stride[2];
+#pragma unroll
+    for (int i = 0; i < kQkRows; ++i)
+      raw[i] = kind[i] < 3 ? *reinterpret_cast<const uint4*>((kind[i] == 0 ? q : kind[i] == 1 ? k : v) + off[i]) : make_uint4(0, 0, 0, 0);
+  };
+  int64_t token0 = int64_t(blockIdx.x) * tile;
+  uint4 raw[kQkRows];
+  load(token0, raw);
+  // Thread and index i take an angle of the tile: (token, frequency), the positions asked for a tile ahead.
+  int position[kAngles];
+  auto ask = [&](int64_t first) {
+#pragma unroll
+    for (int i = 0; i < kAngles; ++i) {
+      const int id = threadIdx.x + i * kQkThreads, t = a.half ? id / a.half : tile, f = id - t * a.half;
+      position[i] = 0;
+      if (t < tile && first + t < a.tokens) {
+        const int axis = (f >= a.section_end[0]) + (f >= a.section_end[1]) + (f >= a.section_end[2]);
+        position[i] = a.positions[axis * a.axis_stride + first + t];
       }
     }
   };
-  int64_t token = blockIdx.x;
-  int row0 = first_row;
-  uint4 raw[kQkRows];
-  load(token, row0, raw);
-  // Thread j makes frequency j's sine and cosine.
-  const int j = threadIdx.x;
-  const bool turns_one = j < a.half;
-  const int32_t* positions = nullptr;
-  double turns_per = 0.0;
-  int position = 0;
-  if (turns_one) {
-    const int axis = (j >= a.section_end[0]) + (j >= a.section_end[1]) + (j >= a.section_end[2]);
-    positions = a.positions + axis * a.axis_stride;
-    position = positions[token];
-    turns_per = double(a.inv_freq[j]) * 0.15915494309189533577;  // 1 / (2 pi)
+  ask(token0);
+  for (int e = threadIdx.x; e < 2 * D; e += kQkThreads) {
+    const int w = e / D;
+    weights[w][e % D] = a.weight[w] ? weight_at(a.weight[w], a.weight_dtype, e % D) : 1.f;
   }
-  int64_t slot = a.slots ? a.slots[token] : token;
-  float wt[2][8];
-#pragma unroll
-  for (int w = 0; w < 2; ++w)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) wt[w][i] = a.weight[w] ? weight_at(a.weight[w], a.weight_dtype, e0 + i) : 1.f;
+  __syncthreads();
+  for (int id = threadIdx.x; id < 2 * kQkTile * 2 * D; id += kQkThreads) {  // values that are not turned: once for all
+    const int e = id % D, w = id / D % 2, t = id / (2 * D) % kQkTile;
+    if (e >= 2 * a.half) factors[id / (2 * D * kQkTile)][t][w].set(e, weights[w][e], 0.f);
+  }
   const bool turned = e0 < 2 * a.half;
   // The lane that holds the partners of an element pair (i, i + rot / 2), in this head's lanes.
   const int lane = threadIdx.x & 31;
   const int partner = !turned || a.adjacent ? lane : e0 < a.half ? lane + a.half / 8 : lane - a.half / 8;
-  float co[8], si[8];
   int buffer = 0;
-  bool fresh = true;
-  for (;;) {
-    if (fresh) {
-      // This lane's cosines and sines, one per element: the sine carries the sign of the partner's product.
-      if (turns_one) {
-        const double turns = double(position) * turns_per;
+  for (; token0 < a.tokens; token0 += int64_t(gridDim.x) * tile, buffer ^= 1) {
+#pragma unroll
+    for (int i = 0; i < kAngles; ++i) {
+      const int id = threadIdx.x + i * kQkThreads, t = a.half ? id / a.half : tile, f = id - t * a.half;
+      if (t < tile) {
+        const double turns = double(position[i]) * (double(a.inv_freq[f]) * 0.15915494309189533577);  // 1 / (2 pi)
         float s, c;
         sincospif(2.f * float(turns - rint(turns)), &s, &c);
-        cs[buffer][0][j] = c;
-        cs[buffer][1][j] = s;
-      }
-      __syncthreads();
+        const int lo = a.adjacent ? 2 * f : f, hi = a.adjacent ? 2 * f + 1 : f + a.half;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        co[i] = 1.f;
-        si[i] = 0.f;
-        if (turned) {
-          const int e = e0 + i, f = a.adjacent ? e >> 1 : e < a.half ? e : e - a.half;
-          const bool low = a.adjacent ? !(e & 1) : e < a.half;
-          co[i] = cs[buffer][0][f];
-          si[i] = low ? -cs[buffer][1][f] : cs[buffer][1][f];
+        for (int w = 0; w < 2; ++w) {
+          const float wl = weights[w][lo], wh = weights[w][hi];
+          factors[buffer][t][w].set(lo, wl * c, -wh * s);
+          factors[buffer][t][w].set(hi, wh * c, wl * s);
         }
       }
-      buffer ^= 1;
     }
-    // What comes after these rows is asked for before they are worked on.
-    int64_t next_token = token, next_slot = slot;
-    int next_row = row0 + kQkRows * step;
-    fresh = next_row - slot_row >= a.rows;  // (block-uniform)
-    if (fresh) {
-      next_token += gridDim.x;
-      next_row = first_row;
-    }
-    const bool more = next_token < a.tokens;
-    uint4 next_raw[kQkRows];
-    if (more) {
-      load(next_token, next_row, next_raw);
-      if (fresh) {
-        if (turns_one) position = positions[next_token];
-        next_slot = a.slots ? a.slots[next_token] : next_token;
+    ask(token0 + int64_t(gridDim.x) * tile);
+    __syncthreads();
+    const int here = a.tokens - token0 < tile ? int(a.tokens - token0) : tile;
+    for (int t = 0; t < here; ++t) {
+      const int64_t token = token0 + t, next = t + 1 < here ? token + 1 : token0 + int64_t(gridDim.x) * tile;
+      uint4 next_raw[kQkRows];
+      if (next < a.tokens) load(next, next_raw);
+      int64_t slot = token;
+      bool kept = true;
+      if (a.slots) {
+        slot = a.slots[token];
+        kept = slot >= 0 && slot < a.n_slots;
       }
-    }
+      T* q = static_cast<T*>(a.out[0]) + token * a.out_stride[0];
+      T* k = static_cast<T*>(a.out[1]) + slot * a.out_stride[1];
+      T* v = static_cast<T*>(a.out[2]) + slot * a.out_stride[2];
 #pragma unroll
-    for (int i = 0; i < kQkRows; ++i) {
-      const int row = row0 + i * step;
-      if (row - slot_row >= a.rows) break;  // (block-uniform)
-      const int w = row < a.rows ? which(row) : 2;
-      float x[8];
-      unpack8<T>(raw[i], x);
-      float sum = 0.f;
+      for (int i = 0; i < kQkRows; ++i) {
+        uint4 result = raw[i];
+        if (!copies) {
+          const QkFactors<D>& f = factors[buffer][t][kind[i] == 1];
+          float x[8], p[8];
+          unpack8<T>(raw[i], x);
+          float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+          for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
 #pragma unroll
-      for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-      const bool norm = w < 2 && a.weight[w];
-      const float r = norm ? rsqrtf(sum * (1.f / D) + a.eps) : 1.f;
+          for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+          const float r = a.weight[kind[i] & 1] ? rsqrtf(sum * (1.f / D) + a.eps) : 1.f;
+          if (a.adjacent) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= r * (w == 1 ? wt[1][e] : wt[0][e]);
-      float y[8];
-      if (a.adjacent) {
+            for (int e = 0; e < 8; ++e) p[e] = x[e ^ 1];
+          } else {
+            uint4 other;
+            other.x = __shfl_sync(0xffffffffu, raw[i].x, partner);
+            other.y = __shfl_sync(0xffffffffu, raw[i].y, partner);
+            other.z = __shfl_sync(0xffffffffu, raw[i].z, partner);
+            other.w = __shfl_sync(0xffffffffu, raw[i].w, partner);
+            unpack8<T>(other, p);
+          }
+          const float4 o0 = f.piece[0][l], o1 = f.piece[1][l];
+          float y[8] = {x[0] * o0.x, x[1] * o0.y, x[2] * o0.z, x[3] * o0.w, x[4] * o1.x, x[5] * o1.y, x[6] * o1.z, x[7] * o1.w};
+          if (turned) {
+            const float4 t0 = f.piece[2][l], t1 = f.piece[3][l];
+            const float other[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], co[e], x[e ^ 1] * si[e]);
-      } else {
+            for (int e = 0; e < 8; ++e) y[e] = fmaf(p[e], other[e], y[e]);
+          }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float p = __shfl_sync(0xffffffffu, x[e], partner);
-          y[e] = fmaf(x[e], co[e], turned ? p * si[e] : 0.f);
+          for (int e = 0; e < 8; ++e) y[e] *= r;
+          if (kind[i] < 2) result = pack8<T>(y);
         }
+        if (kind[i] == 0 || (kind[i] < 3 && kept))
+          *reinterpret_cast<uint4*>((kind[i] == 0 ? q : kind[i] == 1 ? k : v) + off[i]) = result;
       }
-      if (row < a.rows) {
-        const uint4 v = w == 2 ? raw[i] : pack8<T>(y);
-        // (a slot outside of the cache is not stored)
-        const int64_t to = w == 0 ? token : !a.slots || (slot >= 0 && slot < a.n_slots) ? slot : -1;
-        if (to >= 0)
-          *reinterpret_cast<uint4*>(static_cast<T*>(a.out[w]) + to * a.out_stride[w] + (row - a.first[w]) * D + e0) = v;
-      }
-    }
-    if (!more) break;
 #pragma unroll
-    for (int i = 0; i < kQkRows; ++i) raw[i] = next_raw[i];
-    token = next_token;
-    slot = next_slot;
-    row0 = next_row;
+      for (int i = 0; i < kQkRows; ++i) raw[i] = next_raw[i];
+    }
   }
 }
 
@@ -306,13 +322,14 @@ int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm
   if (a.slots && a.n_slots <= 0) return invalid("qk_norm_rope: slots without n_slots");
   a.heads = in->heads;
   a.kv_heads = in->kv_heads;
+  // Up to kQkRows heads per thread, the others to more blocks; few tokens share their heads among blocks, many go to a block in tiles.
+  const int per_pass = kQkThreads / (dim / 8), passes = (a.rows + per_pass - 1) / per_pass, room = kQkBlocks * sm_count();
+  int share = (passes + kQkRows - 1) / kQkRows;
+  while (share < passes && int64_t(tokens) * share < sm_count()) share = 2 * share < passes ? 2 * share : passes;
   a.tokens = tokens;
-  // A block per token with up to kQkRows heads per thread and pass, kQkBlocks of them per multiprocessor, each with every so many of
-  // the tokens; few tokens share their heads among more blocks.
-  const int per_pass = kQkThreads / (dim / 8), passes = (a.rows + per_pass - 1) / per_pass, most = kQkBlocks * sm_count();
-  int share = 1;
-  while (share < passes && tokens * share < sm_count()) share *= 2;
-  const dim3 grid(unsigned(tokens < most ? tokens : most), unsigned(share < passes ? share : passes));
+  a.tile = int64_t(tokens) * share >= 2 * int64_t(kQkTile) * room ? kQkTile : 1;
+  const int tiles = (tokens + a.tile - 1) / a.tile, across = room / share > 0 ? room / share : 1;
+  const dim3 grid(unsigned(tiles < across ? tiles : across), unsigned(share));
   const cudaError_t e = in->dtype == FB_DT_BF16 ? launch_qk<__nv_bfloat16>(a, dim, grid, as_stream(stream))
                                                 : launch_qk<__half>(a, dim, grid, as_stream(stream));
   const int32_t st = check_launch("qk_norm_rope");
