@@ -10,6 +10,11 @@ _DTYPES = {torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
 _WEIGHT_DTYPES = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
 
 
+def _device():
+    """Index of the current device; a number that no tensor's device has while there is none in use."""
+    return torch._C._cuda_getDevice() if torch.cuda.is_initialized() else -2
+
+
 def _heads(x, tokens, heads, dim, dtype, dev, what):
     """(address, stride between tokens) of a [tokens][heads][head_dim] tensor whose heads lie side by side, on the current device
     (whose stream the call goes to)."""
@@ -67,7 +72,7 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, eps, rope, positions, q_out, k_out
         raise ValueError("qk_norm_rope: k_out has another number of tokens than k")
     if (v is None) != (v_out is None):
         raise ValueError("qk_norm_rope: v and v_out are given together, or neither")
-    dev = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
+    dev = _device()
     q_at, q_stride = _heads(q, tokens, heads, dim, dtype, dev, "q")
     k_at, k_stride = _heads(k, tokens, kv_heads, dim, dtype, dev, "k")
     qo_at, qo_stride = _heads(q_out, tokens, heads, dim, dtype, dev, "q_out")
@@ -99,7 +104,7 @@ def attn_prefill(q, k, v, cu_seqlens, out, scale=None, status=None):
         raise ValueError("attn_prefill: bf16 or fp16")
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError("attn_prefill: cu_seqlens int32 [n_seqs + 1]")
-    dev = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
+    dev = _device()
     q_at, q_stride = _heads(q, tokens, heads, dim, dtype, dev, "q")
     k_at, k_stride = _heads(k, tokens, kv_heads, dim, dtype, dev, "k")
     v_at, v_stride = _heads(v, tokens, kv_heads, dim, dtype, dev, "v")
@@ -151,7 +156,7 @@ def attn_tree_decode(q, cache, block_table, contexts, out, workspace, mask=None,
     n_seqs, drafted, heads, dim = q.shape
     if q.dtype is not cache.dtype or out.dtype is not q.dtype or out.shape != q.shape or dim != cache.head_dim:
         raise ValueError("attn_tree_decode: q and out [n_seqs][drafted][heads][head_dim] of the cache's type")
-    dev = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
+    dev = _device()
     strides = []
     for x in (q, out):
         s = x.stride()
