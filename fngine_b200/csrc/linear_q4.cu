@@ -115,18 +115,20 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
   auto seek = [&] {
     if (pu < a.units) {
 #pragma unroll
-      for (int i = 0; i < 2 * MT; ++i) src[i] = a.codes + size_t(row_of(pu, 8 * i + g)) * row_bytes + t * 16;
+      for (int i = 0; i < 2 * MT; ++i) src[i] = a.codes + size_t(row_of(pu, 8 * i + g)) * row_bytes + ps * 64 + t * 16;
     }
   };
   const uint32_t ring_addr = smem_u32(ring);
   // 16-byte chunk c of row r lies at r * 64 + (c ^ (r / 2 % 4)) * 16: eight rows of a chunk in eight bank groups.
-  const uint32_t put = uint32_t(g * 64 + ((t ^ ((g >> 1) & 3)) << 4));
-  int put_stage = 0;
+  const uint32_t put0 = ring_addr + uint32_t(g * 64 + ((t ^ ((g >> 1) & 3)) << 4)), ring_end = put0 + kStages * MT * 1024;
+  uint32_t put = put0;
   auto copy_step = [&] {
     if (pu < a.units) {
 #pragma unroll
       for (int i = 0; i < 2 * MT; ++i)
-        cp_async16(ring_addr + put_stage * (MT * 1024) + i * 512 + put, src[i] + size_t(ps) * 64);
+        cp_async16(put + i * 512, src[i]);
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) src[i] += split * 64;
       ps += split;
       if (ps >= ksteps) {
         ps = wk;
@@ -135,44 +137,62 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
       }
     }
     cp_async_commit();
-    put_stage = put_stage + 1 == kStages ? 0 : put_stage + 1;
+    put += MT * 1024;
+    if (put == ring_end) put = put0;
   };
 
   // Scales and zero points of the step after the current one.
   uint32_t s_raw[2 * MT][kScaleWords], z_raw[2 * MT];
   int su = first, ss = wk;
+  uint32_t s_at[2 * MT];  // group of the step in each row
+  auto seek_scales = [&] {
+    if (su < a.units) {
+#pragma unroll
+      for (int i = 0; i < 2 * MT; ++i) s_at[i] = uint32_t(row_of(su, 8 * i + g)) * uint32_t(row_groups) + uint32_t(ss * kGroups);
+    }
+  };
   auto load_scales = [&] {
     if (su >= a.units) return;
 #pragma unroll
     for (int i = 0; i < 2 * MT; ++i) {
-      const size_t at = size_t(row_of(su, 8 * i + g)) * row_groups + ss * kGroups;
       if (SF32) {
-        const float* p = static_cast<const float*>(a.scales) + at;
-#pragma unroll
-        for (int j = 0; j < kGroups; ++j) s_raw[i][j] = __float_as_uint(p[j]);
-      } else {
-        const uint16_t* p = static_cast<const uint16_t*>(a.scales) + at;
-        if (kGroups == 1) {
-          s_raw[i][0] = *p;
+        const float* p = static_cast<const float*>(a.scales) + s_at[i];
+        if (kGroups == 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(p);
+          s_raw[i][0] = v.x, s_raw[i][1 % kScaleWords] = v.y, s_raw[i][2 % kScaleWords] = v.z, s_raw[i][3 % kScaleWords] = v.w;
+        } else if (kGroups == 2) {
+          const uint2 v = *reinterpret_cast<const uint2*>(p);
+          s_raw[i][0] = v.x, s_raw[i][1 % kScaleWords] = v.y;
         } else {
-#pragma unroll
-          for (int j = 0; j < kScaleWords; ++j) s_raw[i][j] = reinterpret_cast<const uint32_t*>(p)[j];
+          s_raw[i][0] = __float_as_uint(*p);
+        }
+      } else {
+        const uint16_t* p = static_cast<const uint16_t*>(a.scales) + s_at[i];
+        if (kGroups == 4) {
+          const uint2 v = *reinterpret_cast<const uint2*>(p);
+          s_raw[i][0] = v.x, s_raw[i][1 % kScaleWords] = v.y;
+        } else if (kGroups == 2) {
+          s_raw[i][0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+          s_raw[i][0] = *p;
         }
       }
       if (a.zeros) {
-        const uint8_t* z = a.zeros + at;
+        const uint8_t* z = a.zeros + s_at[i];
         z_raw[i] = kGroups == 1 ? *z : kGroups == 2 ? *reinterpret_cast<const uint16_t*>(z) : *reinterpret_cast<const uint32_t*>(z);
-        z_raw[i] &= 0x0f0f0f0fu;
       }
+      s_at[i] += split * kGroups;
     }
     ss += split;
     if (ss >= ksteps) {
       ss = wk;
       su += stride;
+      seek_scales();
     }
   };
 
   seek();
+  seek_scales();
   pdl_wait_prior();
   pdl_launch_dependents();
 #pragma unroll
@@ -191,8 +211,10 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
   }
   // ldmatrix row addresses: lanes 0-7 rows 0-7 of a chunk, 8-15 rows 8-15, 16-31 the same of the next chunk.
   const int lr = (lane & 7) + ((lane >> 3) & 1) * 8, lc = lane >> 4;
-  const uint32_t get = uint32_t(lr * 64), get_x = uint32_t((lr >> 1) & 3);
-  int get_stage = 0;
+  // Chunk pairs (0, 1) and (2, 3) of a row: where this lane's lies in a stage.
+  const uint32_t get_x = uint32_t((lr >> 1) & 3), get0 = ring_addr + uint32_t(lr * 64), get_end = get0 + kStages * MT * 1024;
+  const uint32_t chunk[2] = {(uint32_t(lc) ^ get_x) << 4, (uint32_t(2 + lc) ^ get_x) << 4};
+  uint32_t get = get0;
 
   float acc[MT][NT][4];
   bool loaded = false;
@@ -230,21 +252,22 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
         for (int i = 0; i < 2 * MT; ++i) {
 #pragma unroll
           for (int j = 0; j < kScaleWords; ++j) s_now[i][j] = s_raw[i][j];
-          z_now[i] = z_raw[i];
+          z_now[i] = z_raw[i] & 0x0f0f0f0fu;
         }
         load_scales();
         cp_async_wait<kStages - 2>();
         __syncwarp();
         copy_step();  // into the stage that the step before has read
-        const uint32_t stage = ring_addr + get_stage * (MT * 1024) + get;
-        get_stage = get_stage + 1 == kStages ? 0 : get_stage + 1;
+        const uint32_t stage = get;
+        get += MT * 1024;
+        if (get == get_end) get = get0;
         const uint32_t x_step = uint32_t((step - c0) * (kQ4Step * 2));
         float part[MT][NT][4];
 #pragma unroll
         for (int b2 = 0; b2 < 2; ++b2) {
           uint32_t w[MT][4];
 #pragma unroll
-          for (int m = 0; m < MT; ++m) ldmatrix_x4(w[m], stage + m * 1024 + (((2 * b2 + lc) ^ get_x) << 4));
+          for (int m = 0; m < MT; ++m) ldmatrix_x4(w[m], stage + chunk[b2] + m * 1024);
 #pragma unroll
           for (int ci = 0; ci < 2; ++ci) {
             constexpr int kBlocks = GROUP / 32;  // blocks of 32 values per group
@@ -378,6 +401,7 @@ int32_t fb_linear_q4_decode(const void* x_bf16, int32_t tokens, const fb_q4_weig
   const int n = weight->n, k = weight->k, group = weight->group, kind = epilogue->kind;
   if (n <= 0 || k <= 0 || k % kQ4Step) return invalid("linear_q4_decode: unsupported shape (k %% 128)");
   if (group != 32 && group != 64 && group != 128) return invalid("linear_q4_decode: groups of 32, 64 or 128 values");
+  if (int64_t(n) * (k / group) > INT32_MAX) return invalid("linear_q4_decode: more than 2^31 - 1 groups");
   if (weight->scales_dtype != FB_DT_F32 && weight->scales_dtype != FB_DT_BF16 && weight->scales_dtype != FB_DT_F16)
     return invalid("linear_q4_decode: scales are fp32, bf16 or fp16");
   if (kind < FB_EPI_STORE_BF16 || kind > FB_EPI_SHARED_SCALE) return invalid("linear_q4_decode: unknown epilogue");

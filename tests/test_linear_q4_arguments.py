@@ -16,7 +16,7 @@ def test_refusals(fb_built):
     lib = L.load()
     for bad, word in [(dict(tokens=0), b"1..16"), (dict(tokens=17), b"1..16"), (dict(tokens=-1), b"1..16"), (dict(k=192), b"k % 128"),
                       (dict(k=0), b"shape"), (dict(n=0), b"shape"), (dict(n=-8), b"shape"), (dict(group=16), b"groups"), (dict(group=256), b"groups"),
-                      (dict(group=0), b"groups"), (dict(sdtype=7), b"scales"), (dict(kind=5), b"epilogue"), (dict(kind=-1), b"epilogue"),
+                      (dict(group=0), b"groups"), (dict(n=2 ** 25, k=2048, group=32), b"2^31"), (dict(sdtype=7), b"scales"), (dict(kind=5), b"epilogue"), (dict(kind=-1), b"epilogue"),
                       (dict(kind=L.EPI_GR_WRITE), b"inj"), (dict(kind=L.EPI_SHARED_SCALE), b"gate_logit"), (dict(kind=L.EPI_SWIGLU, n=33), b"SwiGlu"),
                       (dict(codes=0x100008), b"aligned"), (dict(scales=0x200002), b"aligned"), (dict(zeros=0x500001), b"aligned"),
                       (dict(x=0x300008), b"aligned"), (dict(out=0x400002), b"aligned"), (dict(out=0x400001, kind=L.EPI_STORE_BF16), b"aligned"),
