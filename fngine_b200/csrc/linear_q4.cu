@@ -2,14 +2,21 @@
 //
 //   acc[t][r] = sum over groups g of  s[r][g] * sum_{i in g} (c[r][i] - z[r][g]) * x[t][i],   then the epilogue.
 //
-// c - z is a whole number of magnitude <= 15, exact in bf16, and so is x: the tensor core forms the inner sums of a group
-// from exact products in fp32, and one multiply-add per group and output applies the scale. Nothing is rounded but sums.
+// The code bits are the tensor core's operand as they stand: bits 0-7 of a bf16 number whose other bits are zero count in steps of
+// 2^-133 (the subnormal numbers and the first normal ones have the same spacing), so a code in bits 0-3 is c 2^-133 and one in bits
+// 4-7 is 16 c 2^-133, both exact, and eight codes cost one shift and four ANDs. (As whole bf16 numbers, by an exponent under the bits
+// and a subtraction of 128 + z, they cost eleven instructions, and their issue bound the kernel: 110 us for 248320 x 2560 at 16 tokens.)
+// The activations bring the scale back: they are multiplied by 2^64, those of the codes in bits 4-7 by 2^60, exactly; or by 1 and 1/16
+// in a token that has one of 2^63 or more. Products are exact, the tensor core adds them in fp32; what is below 2^-57 (2^7 in such a
+// token, of more than 2^63) counts as zero. What a zero
+// point takes off, z sum(x) of a group, comes from sums of the activations that are made once:
+//   acc += s (P - z X),   P = sum of c x 2^-69 over the group, X = sum of x 2^-69.
+// Nothing is rounded but sums.
 //
 // The weights are the only large operand, so the kernel is built around their stream. A warp takes 16 MT rows (the M
 // side of mma.sync m16n8k16, the tokens are the N side) through K in steps of 128: its own ring of cp.async stages in
-// shared memory, no barrier between warps. ldmatrix gives lane (g, t) of a quad eight consecutive codes of row g, of
-// which every second MMA operand pair is one AND-OR: the nibbles of 0x000f000f under the bf16 exponent of 128, minus
-// 128 + z. The activations lie in shared memory in the order (0 4 1 5 2 6 3 7) that those pairs come in. S warps share
+// shared memory, no barrier between warps. ldmatrix gives lane (g, t) of a quad eight consecutive codes of row g. The activations lie
+// in shared memory in the order (0 4 1 5 2 6 3 7) that the masked codes come in. S warps share
 // the K steps of a row tile and add their tiles in shared memory in warp order, so results do not depend on timing.
 #include "common.cuh"
 
@@ -23,7 +30,7 @@ constexpr int kQ4Warps = 16;
 constexpr int kQ4Threads = 32 * kQ4Warps;
 constexpr int kQ4Step = 128;    // K values per step of a warp: 64 bytes of a row
 constexpr int kQ4MaxTok = 16;
-constexpr int kQ4SmemLimit = 227 * 1024;
+constexpr int kQ4SmemLimit = 226 * 1024;  // (beside the static part)
 
 struct Q4Args {
   const __nv_bfloat16* x;
@@ -61,13 +68,13 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Two codes (bits 0-3 and 16-19 of w) minus their zero point, as a bf16 pair: 128 + c is exact, and so is the difference.
-__device__ __forceinline__ uint32_t codes_to_bf16(uint32_t w, uint32_t zero) {
-  uint32_t v, r;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(v) : "r"(w));  // (w & mask) | 128.0
-  asm("sub.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(zero));
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
+// Code 0..15 as fp32, without the conversion unit.
+__device__ __forceinline__ float code_to_float(uint32_t c) { return __uint_as_float(0x4b000000u | c) - 8388608.f; }
 
 // Stages of a warp's ring. One more costs 16 or 32 KB of the activations' room.
 template <int MT>
@@ -86,10 +93,13 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
   constexpr int kScaleWords = SF32 ? kGroups : (kGroups + 1) / 2;    // 32-bit words of a row's scales per step
   constexpr int kPitch = kQ4RowPitch<MT>;
   extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ uint32_t large_tokens;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (threadIdx.x == 0) large_tokens = 0;
   uint8_t* ring = smem + warp * (kStages * MT * 1024);
   float* tile = reinterpret_cast<float*>(smem + kQ4Warps * kStages * MT * 1024) + warp * (8 * NT * kPitch);
-  uint8_t* xs = smem + q4_fixed_smem<MT, NT>();
+  float* group_sums = reinterpret_cast<float*>(smem + q4_fixed_smem<MT, NT>());  // [groups of a chunk][8 NT]
+  uint8_t* xs = reinterpret_cast<uint8_t*>(group_sums + a.chunk * (kGroups * 8 * NT));
   const int split = a.split, per_cta = kQ4Warps / split;
   const int wk = warp % split, wu = warp / split;
   const int ksteps = a.k / kQ4Step;
@@ -217,6 +227,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
   uint32_t get = get0;
 
   float acc[MT][NT][4];
+  uint32_t large = 0;  // tokens whose activations are not multiplied by 2^64, and their sums smaller by it
   bool loaded = false;
   for (int base = blockIdx.x * per_cta; base < a.units; base += stride) {
     const int unit = base + wu;
@@ -231,20 +242,51 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
     for (int c0 = 0; c0 < ksteps; c0 += a.chunk) {
       const int c1 = c0 + a.chunk < ksteps ? c0 + a.chunk : ksteps;
       if (!loaded || a.chunk < ksteps) {  // (block-uniform)
-        if (loaded) __syncthreads();
+        __syncthreads();
         const int per_row = (c1 - c0) * (kQ4Step / 8);
-        for (int i = threadIdx.x; i < per_row * a.tokens; i += kQ4Threads) {
-          const int tok = i / per_row, j = i - tok * per_row;
-          const uint4 v = *reinterpret_cast<const uint4*>(a.x + size_t(tok) * a.k + size_t(c0) * kQ4Step + j * 8);
-          uint4 w;
-          w.x = __byte_perm(v.x, v.z, 0x5410);
-          w.y = __byte_perm(v.x, v.z, 0x7632);
-          w.z = __byte_perm(v.y, v.w, 0x5410);
-          w.w = __byte_perm(v.y, v.w, 0x7632);
-          *reinterpret_cast<uint4*>(xs + tok * x_pitch + j * 16) = w;
+        auto stage_x = [&] {
+          for (int i = threadIdx.x; i < per_row * a.tokens; i += kQ4Threads) {
+            const int tok = i / per_row, j = i - tok * per_row;
+            const bool plain = (large >> tok) & 1;
+            const uint32_t up = plain ? 0x3f803f80u : 0x5f805f80u, up16 = plain ? 0x3d803d80u : 0x5d805d80u;  // 1, 2^64; 1/16, 2^60
+            const uint4 v = *reinterpret_cast<const uint4*>(a.x + size_t(tok) * a.k + size_t(c0) * kQ4Step + j * 8);
+            const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+            bool found = false;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t lo = in[e] & 0x7fffu, hi = (in[e] >> 16) & 0x7fffu;
+              found |= (lo >= 0x5f00u && lo < 0x7f80u) || (hi >= 0x5f00u && hi < 0x7f80u);  // 2^63 and more, and finite
+              sum += __uint_as_float(in[e] << 16) * 0x1p-69f + __uint_as_float(in[e] & 0xffff0000u) * 0x1p-69f;
+            }
+            if (found) atomicOr(&large_tokens, 1u << tok);
+#pragma unroll
+            for (int m = GROUP / 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffu << (lane & 16), sum, m);  // (16 lanes have 128 values)
+            if (j % (GROUP / 8) == 0) group_sums[j / (GROUP / 8) * (8 * NT) + tok] = plain ? sum * 0x1p-64f : sum;
+            uint4 w;
+            w.x = mul_bf16x2(__byte_perm(v.x, v.z, 0x5410), up);
+            w.y = mul_bf16x2(__byte_perm(v.x, v.z, 0x7632), up16);
+            w.z = mul_bf16x2(__byte_perm(v.y, v.w, 0x5410), up);
+            w.w = mul_bf16x2(__byte_perm(v.y, v.w, 0x7632), up16);
+            *reinterpret_cast<uint4*>(xs + tok * x_pitch + j * 16) = w;
+          }
+          __syncthreads();
+        };
+        stage_x();
+        const uint32_t more = large_tokens & ~large;  // (the same for all)
+        if (more) {
+          __syncthreads();
+          large |= more;
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if ((more >> (nt * 8 + 2 * t + (i & 1))) & 1) acc[m][nt][i] *= 0x1p-64f;
+          stage_x();
         }
         loaded = true;
-        __syncthreads();
       }
       for (; step < c1; step += split) {
         uint32_t s_now[2 * MT][kScaleWords], z_now[2 * MT];
@@ -252,7 +294,7 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
         for (int i = 0; i < 2 * MT; ++i) {
 #pragma unroll
           for (int j = 0; j < kScaleWords; ++j) s_now[i][j] = s_raw[i][j];
-          z_now[i] = z_raw[i] & 0x0f0f0f0fu;
+          z_now[i] = z_raw[i];
         }
         load_scales();
         cp_async_wait<kStages - 2>();
@@ -289,13 +331,9 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
                            : "memory");
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-              const uint32_t za = 0x43004300u + ((z_now[2 * m] >> (8 * group)) & 0xffu) * 0x00010001u;
-              const uint32_t zb = 0x43004300u + ((z_now[2 * m + 1] >> (8 * group)) & 0xffu) * 0x00010001u;
-              const uint32_t wa = w[m][2 * ci], wb = w[m][2 * ci + 1];
-              const uint32_t a0 = codes_to_bf16(wa, za), a1 = codes_to_bf16(wb, zb);
-              const uint32_t a2 = codes_to_bf16(wa >> 4, za), a3 = codes_to_bf16(wb >> 4, zb);
-              const uint32_t a4 = codes_to_bf16(wa >> 8, za), a5 = codes_to_bf16(wb >> 8, zb);
-              const uint32_t a6 = codes_to_bf16(wa >> 12, za), a7 = codes_to_bf16(wb >> 12, zb);
+              const uint32_t wa = w[m][2 * ci], wb = w[m][2 * ci + 1], va = wa >> 8, vb = wb >> 8;
+              const uint32_t a0 = wa & 0x000f000fu, a1 = wb & 0x000f000fu, a2 = wa & 0x00f000f0u, a3 = wb & 0x00f000f0u;
+              const uint32_t a4 = va & 0x000f000fu, a5 = vb & 0x000f000fu, a6 = va & 0x00f000f0u, a7 = vb & 0x00f000f0u;
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 mma_bf16(part[m][nt], a0, a1, a2, a3, xv[nt].x, xv[nt].y);
@@ -303,9 +341,13 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
               }
             }
             if (b % kBlocks == kBlocks - 1) {
+              float2 xsum[NT];
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                xsum[nt] = *reinterpret_cast<const float2*>(group_sums + ((step - c0) * kGroups + group) * (8 * NT) + nt * 8 + 2 * t);
 #pragma unroll
               for (int m = 0; m < MT; ++m) {
-                float sc[2];
+                float sc[2], z[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                   if (SF32) {
@@ -314,11 +356,15 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
                     const uint32_t h = (s_now[2 * m + i][group / 2] >> (16 * (group % 2))) & 0xffffu;
                     sc[i] = a.scale_f16 ? __half2float(__ushort_as_half(uint16_t(h))) : __uint_as_float(h << 16);
                   }
+                  z[i] = code_to_float((z_now[2 * m + i] >> (8 * group)) & 15u);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) acc[m][nt][i] = fmaf(sc[i >> 1], part[m][nt][i], acc[m][nt][i]);
+                  for (int i = 0; i < 4; ++i) {
+                    float v = fmaf(-z[i >> 1], i & 1 ? xsum[nt].y : xsum[nt].x, part[m][nt][i]);
+                    acc[m][nt][i] = fmaf(sc[i >> 1], v, acc[m][nt][i]);
+                  }
               }
             }
           }
@@ -333,7 +379,8 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          tile[(nt * 8 + 2 * t + (i & 1)) * kPitch + m * 16 + g + (i >> 1) * 8] = acc[m][nt][i];
+          tile[(nt * 8 + 2 * t + (i & 1)) * kPitch + m * 16 + g + (i >> 1) * 8] =
+              acc[m][nt][i] * 0x1p69f * ((large >> (nt * 8 + 2 * t + (i & 1))) & 1 ? 0x1p64f : 1.f);
     __syncwarp();
     if (split > 1) named_bar_sync(1 + wu, 32 * split);
     if (unit < a.units) {
@@ -455,10 +502,11 @@ int32_t fb_linear_q4_decode(const void* x_bf16, int32_t tokens, const fb_q4_weig
   const int grid = int(ctas < sms ? ctas : sms);
   const int fixed = mt == 1 ? (nt == 1 ? q4_fixed_smem<1, 1>() : q4_fixed_smem<1, 2>())
                             : (nt == 1 ? q4_fixed_smem<2, 1>() : q4_fixed_smem<2, 2>());
-  const int room = (kQ4SmemLimit - fixed) / tokens;  // bytes of a token's activations
-  a.chunk = (room - 64) / (kQ4Step * 2);
+  // Per K step: a token's activations, and the sums of its groups for all token columns.
+  const int per_step = tokens * kQ4Step * 2 + (kQ4Step / group) * 8 * nt * 4;
+  a.chunk = (kQ4SmemLimit - fixed - tokens * 64) / per_step;
   if (a.chunk > ksteps) a.chunk = ksteps;
-  const size_t smem = size_t(fixed) + size_t(tokens) * (size_t(a.chunk) * kQ4Step * 2 + 64);
+  const size_t smem = size_t(fixed) + size_t(tokens) * 64 + size_t(a.chunk) * per_step;
   const bool f32 = weight->scales_dtype == FB_DT_F32;
   cudaStream_t s = as_stream(stream);
   const cudaError_t e = mt == 1 ? launch_q4_group<1, 1>(a, group, f32, grid, smem, s)

@@ -112,6 +112,19 @@ def test_epilogues(kind, n, k, group, sdtype, zeros, T):
         assert torch.equal(run(torch, kind, codes, scales, z, x, extra), got)
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+def test_activations_of_any_size(zeros):
+    """Activations from 2^-56 to the largest bf16 numbers, tokens of both kinds in one call: the kernel scales them by powers of two."""
+    torch = _torch()
+    codes, scales, z, x = make(torch, 70, 1024, 32, torch.float32, zeros, 5, True, 8)
+    scales = scales * 2.0 ** -14
+    x = x * torch.tensor([2.0 ** -50, 1.0, 2.0 ** 62, 2.0 ** 100, 2.0 ** 124], device="cuda")[:, None].to(torch.bfloat16)
+    want = x.double() @ weight64(torch, codes, scales, z, 32).T
+    assert torch.equal(run(torch, "store_f32", codes, scales, z, x).double(), want)
+    assert torch.equal(run(torch, "store_f32", codes, scales, z, x[:3].contiguous()).double(), want[:3])
+    assert torch.equal(run(torch, "store_f32", codes, scales, z, x[3:].contiguous()).double(), want[3:])
+
+
 def test_zero_points_count_their_low_four_bits():
     torch = _torch()
     codes, scales, z, x = make(torch, 50, 256, 32, torch.float32, True, 3, True, 5)
