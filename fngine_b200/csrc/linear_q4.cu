@@ -385,31 +385,61 @@ __global__ void __launch_bounds__(kQ4Threads, 1) q4_kernel(const Q4Args a) {
     if (split > 1) named_bar_sync(1 + wu, 32 * split);
     if (unit < a.units) {
       const float* tiles = tile - wk * (8 * NT * kPitch);
-      const int rows = swiglu ? 16 : 16 * MT, shift = rows == 16 ? 4 : 5;
-      const int row0 = unit * rows, row_end = swiglu ? half : a.n;
-      for (int i = wk * 32 + lane; i < rows * a.tokens; i += 32 * split) {
-        const int r = i & (rows - 1), tok = i >> shift;
-        const float* p = tiles + tok * kPitch + r;
-        float v = 0.f, u = 0.f;
-        for (int w = 0; w < split; ++w) v += p[w * (8 * NT * kPitch)];
-        if (swiglu) {
-          for (int w = 0; w < split; ++w) u += p[w * (8 * NT * kPitch) + 16];
-        }
-        const int row = row0 + r;
+      // Four rows of a token per thread and step.
+      const int quads = swiglu ? 4 : 4 * MT, shift = quads == 4 ? 2 : 3;
+      const int row_end = swiglu ? half : a.n;
+      for (int i = wk * 32 + lane; i < quads * a.tokens; i += 32 * split) {
+        const int r = 4 * (i & (quads - 1)), tok = i >> shift, row = unit * (4 * quads) + r;
         if (row >= row_end) continue;
-        if (a.kind == FB_EPI_STORE_BF16) {
-          static_cast<__nv_bfloat16*>(a.out)[size_t(tok) * a.n + row] = __float2bfloat16_rn(v);
-        } else if (a.kind == FB_EPI_STORE_F32) {
-          static_cast<float*>(a.out)[size_t(tok) * a.n + row] = v;
-        } else if (swiglu) {
-          static_cast<__nv_bfloat16*>(a.out)[size_t(tok) * half + row] = __float2bfloat16_rn(v / (1.f + expf(-v)) * u);
-        } else if (a.kind == FB_EPI_SHARED_SCALE) {
-          const float gate = a.gate_logit[size_t(tok) * a.gate_stride];
-          static_cast<float*>(a.out)[size_t(tok) * a.n + row] = v / (1.f + expf(-gate));
-        } else {  // GrWrite: four residual streams
-          float* X = static_cast<float*>(a.out) + size_t(tok) * 4 * a.n + row;
+        const float* p = tiles + tok * kPitch + r;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < split; ++w) {
+          const float4 f = *reinterpret_cast<const float4*>(p + w * (8 * NT * kPitch));
+          v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+        }
+        if (swiglu) {
+          float u[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int w = 0; w < split; ++w) {
+            const float4 f = *reinterpret_cast<const float4*>(p + w * (8 * NT * kPitch) + 16);
+            u[0] += f.x, u[1] += f.y, u[2] += f.z, u[3] += f.w;
+          }
 #pragma unroll
-          for (int s = 0; s < 4; ++s) X[size_t(s) * a.n] += a.inj[tok * 4 + s] * v;
+          for (int e = 0; e < 4; ++e) v[e] = v[e] / (1.f + expf(-v[e])) * u[e];
+        } else if (a.kind == FB_EPI_SHARED_SCALE) {
+          const float gate = 1.f + expf(-a.gate_logit[size_t(tok) * a.gate_stride]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] /= gate;
+        }
+        const int here = row_end - row < 4 ? row_end - row : 4;
+        const size_t at = size_t(tok) * row_end + row;
+        if (a.kind == FB_EPI_GR_WRITE) {  // four residual streams
+#pragma unroll
+          for (int s = 0; s < 4; ++s) {
+            float* X = static_cast<float*>(a.out) + (size_t(tok) * 4 + s) * a.n + row;
+            const float inj = a.inj[tok * 4 + s];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e < here) X[e] += inj * v[e];
+          }
+        } else if (a.kind == FB_EPI_STORE_BF16 || swiglu) {
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + at;
+          if (here == 4 && !(reinterpret_cast<uintptr_t>(out) & 7)) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+            *reinterpret_cast<uint2*>(out) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e < here) out[e] = __float2bfloat16_rn(v[e]);
+          }
+        } else {
+          float* out = static_cast<float*>(a.out) + at;
+          if (here == 4 && !(reinterpret_cast<uintptr_t>(out) & 15)) {
+            *reinterpret_cast<float4*>(out) = make_float4(v[0], v[1], v[2], v[3]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (e < here) out[e] = v[e];
+          }
         }
       }
     }
@@ -484,8 +514,10 @@ int32_t fb_linear_q4_decode(const void* x_bf16, int32_t tokens, const fb_q4_weig
   a.scale_f16 = weight->scales_dtype == FB_DT_F16;
 
   const int sms = sm_count(), ksteps = k / kQ4Step, nt = tokens > 8 ? 2 : 1;
-  // Two row tiles of 16 per warp halve the reads of activations per weight.
-  const int mt = kind == FB_EPI_SWIGLU || nt == 2 ? 2 : 1;
+  // Two row tiles of 16 per warp halve the reads of activations and the steps per weight (248320 x 2560, one token: 99 us by 16 rows, 67
+  // by 32), where every warp has at least two such steps (2560 x 640: 4.1 us by 16, 5.0 by 32).
+  const long long steps32 = (n + 31LL) / 32 * ksteps;
+  const int mt = kind == FB_EPI_SWIGLU || nt == 2 || steps32 >= 2LL * kQ4Warps * sms ? 2 : 1;
   const long long units = kind == FB_EPI_SWIGLU ? (n / 2 + 15) / 16 : (n + 16 * mt - 1LL) / (16 * mt);
   // The number of warps per row tile that ends first, by the steps that the busiest warp takes.
   long long best = -1;
