@@ -204,7 +204,17 @@ __device__ __forceinline__ bool bounded_wait(int* aborted, uint32_t* status, uin
   return false;
 }
 
-// The same for a whole warp: one answer for all lanes. What stands behind a wait (barriers, tensor memory, elections) needs the
+// For a single thread that issues products: it polls, since waking up from a try takes longer than a product's share of the time.
+__device__ __forceinline__ bool bounded_spin(int* aborted, uint32_t* status, uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < (1u << 26); ++i) {
+    if (mbar_test_wait(bar, parity)) return true;
+    if ((i & 1023u) == 1023u && *static_cast<volatile int*>(aborted)) return false;
+  }
+  *static_cast<volatile int*>(aborted) = 1;
+  if (status) atomicMax(status, uint32_t(FB_STATUS_PIPELINE_TIMEOUT));
+  return false;
+}
+// bounded_wait for a whole warp: one answer for all lanes. What stands behind a wait (barriers, tensor memory, elections) needs the
 // warp converged, and lanes that left a polling loop one by one are not.
 __device__ __forceinline__ bool bounded_wait_warp(int* aborted, uint32_t* status, uint64_t* bar, uint32_t parity) {
   if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;

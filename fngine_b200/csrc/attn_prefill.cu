@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
     constexpr uint32_t kIdescPv = kIdesc | (uint32_t(D >> 3) << 17) | (1u << 16);  // V runs along N
     if (elect_one()) {
       bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && bounded_wait(&bars->aborted, a.status, bar, parity); };
+      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && bounded_spin(&bars->aborted, a.status, bar, parity); };
       if (warp == 8) {
         int held_by = -1, held_at = 0;  // whose scores S holds
         for (int j = 0; j < blocks && ok; ++j) {

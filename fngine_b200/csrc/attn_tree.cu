@@ -25,7 +25,7 @@
 namespace fb {
 namespace {
 
-constexpr int kTreeThreads = 416;        // two streams of four softmax warps, four warps that copy, one that issues products
+constexpr int kTreeThreads = 448;        // two streams of four softmax warps, four that copy, one each that issues scores and outputs
 constexpr int kTreeWarps = kTreeThreads / 32;
 constexpr int kTreeRows = 128;           // rows of a tile
 constexpr int kTreeKeys = 128;           // keys of a block
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
       mbar_init(&bars->full[i], kTreeKeys);
       mbar_init(&bars->empty[i], 1);
     }
-    mbar_init(&bars->drained, 1);
+    mbar_init(&bars->drained, 2);
     bars->aborted = 0;
     bars->q_issued = 0;
     bars->in_flight = 0;
@@ -326,69 +326,57 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
       if (!boxes) warps_sync(2, kTreeKeys);  // the slots have been read
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == 12) {
-    // ------------------------------------------------------------------ products
+  } else if (warp >= 12) {
+    // ------------------------------------------------------------------ products: a thread for the scores, one for the outputs
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kTreeRows >> 4) << 24);
     constexpr uint32_t kIdescQk = kIdesc | (uint32_t(kTreeKeys >> 3) << 17);
     constexpr uint32_t kIdescPv = kIdesc | (uint32_t(D >> 3) << 17) | (1u << 16);  // V runs along N
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      ok = ok && bounded_wait_warp(&bars->aborted, a.status, bar, parity);
-    };
-    TreeCursor next = now;  // of the scores, a block ahead of the outputs
-    int segment = 0;
-    auto scores = [&](int it, bool first) {
-      const int slot = (2 * it) % kStages, b = segment & 1;
-      if (first) wait(&bars->q_full[b], uint32_t(segment / 2) & 1);
-      wait(&bars->full[slot], uint32_t(2 * it / kStages) & 1);
-      const bool last = next.tile + 1 == next.tiles;
-      if (ok) {
-        fence_proxy_async();  // (the copies were made by the generic proxy, the product reads through the other)
-        tc_fence_after();
-        if (elect_one()) {
+    if (elect_one()) {
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && bounded_spin(&bars->aborted, a.status, bar, parity); };
+      int segment = 0, piece = 0;  // piece: first block of the segment in this block's share
+      for (int it = 0; it < n_tiles && ok; ++it) {
+        const bool first = it == piece, last = now.tile + 1 == now.tiles;
+        const uint32_t t = uint32_t(it & 1);
+        if (warp == 12) {
+          const int slot = (2 * it) % kStages, b = segment & 1;
+          if (first) wait(&bars->q_full[b], uint32_t(segment / 2) & 1);
+          wait(&bars->full[slot], uint32_t(2 * it / kStages) & 1);
+          if (it >= 2) wait(&bars->o_done[t], uint32_t((it >> 1) - 1) & 1);  // the stream's last weights, which lie over S, are used
+          if (!ok) break;
+          fence_proxy_async();  // (cp.async writes by the generic proxy, the product reads through the other)
+          tc_fence_after();
           const uint32_t qd = umma_desc_lo(smem_u32(q_tiles + b * S::kTileBytes), 1), kd = umma_desc_lo(smem_u32(ring + slot * S::kTileBytes), 1);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t at = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
-            umma_ss<kIdescQk>(kS + 128 * (it & 1), qd + at, kd + at, k > 0);
+            umma_ss<kIdescQk>(kS + 128 * t, qd + at, kd + at, k > 0);
           }
-          umma_commit(&bars->s_full[it & 1]);
+          umma_commit(&bars->s_full[t]);
           umma_commit(&bars->empty[slot]);
           if (last) umma_commit(&bars->q_empty[b]);
-        }
-        __syncwarp();
-      }
-      if (last) ++segment;
-    };
-    scores(0, true);
-    int piece = 0;  // first block of the segment in this block's share
-    for (int it = 0; it < n_tiles && ok; ++it) {
-      bool next_first = false;
-      if (it + 1 < n_tiles) {
-        next_first = advance(next);
-        scores(it + 1, next_first);
-      }
-      const int slot = (2 * it + 1) % kStages;
-      wait(&bars->p_full[it & 1], uint32_t(it >> 1) & 1);
-      wait(&bars->full[slot], uint32_t((2 * it + 1) / kStages) & 1);
-      if (!ok) break;
-      fence_proxy_async();
-      tc_fence_after();
-      if (elect_one()) {
-        const uint32_t vd = umma_desc_lo(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
-        const uint32_t d = kO + 128 * (it & 1), p = kS + 128 * (it & 1);
-        umma_ts<kIdescPv>(d, p, vd, it - piece >= 2);
+        } else {
+          const int slot = (2 * it + 1) % kStages;
+          wait(&bars->full[slot], uint32_t((2 * it + 1) / kStages) & 1);
+          wait(&bars->p_full[t], uint32_t(it >> 1) & 1);
+          if (!ok) break;
+          fence_proxy_async();
+          tc_fence_after();
+          const uint32_t vd = umma_desc_lo(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
+          const uint32_t d = kO + 128 * t, p = kS + 128 * t;
+          umma_ts<kIdescPv>(d, p, vd, it - piece >= 2);
 #pragma unroll
-        for (int k = 1; k < kTreeKeys / 16; ++k) umma_ts<kIdescPv>(d, p + 8 * k, vd + k * (2048 >> 4), true);
-        umma_commit(&bars->o_done[it & 1]);
-        umma_commit(&bars->empty[slot]);
+          for (int k = 1; k < kTreeKeys / 16; ++k) umma_ts<kIdescPv>(d, p + 8 * k, vd + k * (2048 >> 4), true);
+          umma_commit(&bars->o_done[t]);
+          umma_commit(&bars->empty[slot]);
+        }
+        if (last) ++segment;
+        if (it + 1 < n_tiles && advance(now)) piece = it + 1;
       }
-      __syncwarp();
-      if (next_first) piece = it + 1;
+      // Nothing issued here is still running when the tensor memory is given back.
+      umma_commit(&bars->drained);
     }
-    // Nothing issued here is still running when the tensor memory is given back.
-    if (elect_one()) umma_commit(&bars->drained);
     __syncwarp();
     for (uint32_t n = 0; n < (1u << 16) && !__all_sync(0xffffffffu, mbar_try_wait_hint(&bars->drained, 0)); ++n) {}
   } else {
@@ -456,7 +444,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
             const float fade = up == -INFINITY ? 1.f : exp2_approx((top - up) * a.scale_log2);
             top = up;
             sum *= fade;
-            if (it - piece >= 2) {  // (the stream's last outputs are done: these scores were issued behind them)
+            if (it - piece >= 2) {  // (the stream's last outputs are done: these scores were issued after that)
 #pragma unroll 1
               for (int i = 0; i < D / 32; ++i) {
                 float o[32];
@@ -493,7 +481,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
       }
 
       if (piece_ends) {
-        // The stream's last block of this segment, if it has one. Its scores were issued behind the outputs of the block before it, so
+        // The stream's last block of this segment, if it has one. Its scores were issued when the outputs of the one before were done, so
         // the barrier is not two phases behind, and not ahead: the next outputs need this warp's weights.
         const int last_own = (it & 1) == t ? it : it - 1;
         if (last_own >= piece) ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->o_done[t], uint32_t(last_own >> 1) & 1);
@@ -566,29 +554,47 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
           warps_sync(1, 2 * kTreeRows);
           if (bars->last_block) {
             __threadfence();
-            for (int i = tid; i < rows * (D / 4); i += 2 * kTreeRows) {
-              const int r = i % rows, c = i / rows;
+            // 256 / rows threads to a row, rows along the lanes, up to four 16-byte pieces of it at a time.
+            const int per_row = 2 * kTreeRows / rows, r = tid % rows, sub = tid / rows;
+            if (sub < per_row) {
               // Piece b of the segment is block b's: the first begins with the segment, the others do not.
-              float up = __ldcg(a.partial + (2 * size_t(first) + 1) * S::kSlot + D * kTreeRows + r);
+              const float* head_piece = a.partial + (2 * size_t(first) + 1) * S::kSlot;
+              const float* piece0 = a.partial + 2 * size_t(first) * S::kSlot;
+              float up = __ldcg(head_piece + D * kTreeRows + r);
 #pragma unroll 8
-              for (int b = first + 1; b <= last; ++b) up = fmaxf(up, __ldcg(a.partial + 2 * size_t(b) * S::kSlot + D * kTreeRows + r));
+              for (int b = 1; b <= last - first; ++b) up = fmaxf(up, __ldcg(piece0 + size_t(2 * b) * S::kSlot + D * kTreeRows + r));
               if (up == -INFINITY) up = 0.f;  // a row that sees nothing
-              float l = 0.f;
-              float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+              T* to = static_cast<T*>(a.out) + (token0 + r / a.group) * a.out_stride + int64_t(head0 + r % a.group) * D;
+              for (int c0 = sub; c0 < D / 4; c0 += 4 * per_row) {
+                float l = 0.f;
+                float4 x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-              for (int b = first; b <= last; ++b) {
-                const float* from = a.partial + (2 * size_t(b) + (b == first ? 1 : 0)) * S::kSlot;
-                const float4 o = __ldcg(reinterpret_cast<const float4*>(from + (c * kTreeRows + r) * 4));
-                const float f = exp2_approx((__ldcg(from + D * kTreeRows + r) - up) * a.scale_log2);
-                l = fmaf(__ldcg(from + (D + 1) * kTreeRows + r), f, l);
-                x.x = fmaf(o.x, f, x.x);
-                x.y = fmaf(o.y, f, x.y);
-                x.z = fmaf(o.z, f, x.z);
-                x.w = fmaf(o.w, f, x.w);
+                for (int b = 0; b <= last - first; ++b) {
+                  const float* from = b ? piece0 + size_t(2 * b) * S::kSlot : head_piece;
+                  const float f = exp2_approx((__ldcg(from + D * kTreeRows + r) - up) * a.scale_log2);
+                  l = fmaf(__ldcg(from + (D + 1) * kTreeRows + r), f, l);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const int c = c0 + e * per_row;
+                    if (c < D / 4) {
+                      const float4 o = __ldcg(reinterpret_cast<const float4*>(from + (c * kTreeRows + r) * 4));
+                      x[e].x = fmaf(o.x, f, x[e].x);
+                      x[e].y = fmaf(o.y, f, x[e].y);
+                      x[e].z = fmaf(o.z, f, x[e].z);
+                      x[e].w = fmaf(o.w, f, x[e].w);
+                    }
+                  }
+                }
+                const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int c = c0 + e * per_row;
+                  if (c < D / 4)
+                    *reinterpret_cast<uint2*>(to + 4 * c) = make_uint2(pack2<T>(x[e].x * inv, x[e].y * inv), pack2<T>(x[e].z * inv, x[e].w * inv));
+                }
               }
-              const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-              T* to = static_cast<T*>(a.out) + (token0 + r / a.group) * a.out_stride + int64_t(head0 + r % a.group) * D + 4 * c;
-              *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
             }
           }
         }
