@@ -5,6 +5,7 @@ import ctypes
 import torch
 
 from . import lib as L
+from . import linear
 
 _DTYPES = {torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
 _WEIGHT_DTYPES = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
@@ -180,3 +181,76 @@ def attn_tree_decode(q, cache, block_table, contexts, out, workspace, mask=None,
                                       workspace.numel(), L.stream())
     if st:
         L.check(st, "attn_tree_decode")
+
+
+def kv_store(k, v, cache, slots):
+    """Copies keys and values of packed tokens ([tokens][kv_heads][head_dim]) to slots of a paged cache (int64 [tokens]; one outside of
+    the cache stores nothing): fb_qk_norm_rope without queries, norms and rotation."""
+    tokens, dev = k.shape[0], _device()
+    k_at, k_stride = _heads(k, tokens, cache.kv_heads, cache.head_dim, cache.dtype, dev, "k")
+    v_at, v_stride = _heads(v, tokens, cache.kv_heads, cache.head_dim, cache.dtype, dev, "v")
+    slot = cache.kv_heads * cache.head_dim
+    st = L.load().fb_qk_norm_rope(L.Qkv(None, k_at, v_at, 0, k_stride, v_stride, _DTYPES[cache.dtype], 0, cache.kv_heads, cache.head_dim), tokens,
+                                  None, None, L.QkvOut(None, cache.c.k, cache.c.v, 0, slot, slot, _plain(slots, (tokens,), torch.int64, dev, "slots"),
+                                                       cache.n_pages * cache.page_size), L.stream())
+    if st:
+        L.check(st, "kv_store")
+
+
+class AttentionBranch:
+    """The attention branch of one layer: qkv = a weight of (heads + 2 kv_heads) head_dim rows, out = one of hidden rows, both
+    linear.Fp8RowWeight (any number of tokens) or linear.Q4GroupWeight (up to 16), the norms' weights, the rotation. Owns the workspaces
+    and the intermediate buffers (bf16) of up to max_tokens tokens; calls that overlap need a branch each."""
+
+    def __init__(self, qkv, out, q_weight, k_weight, eps, rope, heads, kv_heads, head_dim, max_tokens):
+        if qkv.n != (heads + 2 * kv_heads) * head_dim or out.k != heads * head_dim:
+            raise ValueError("AttentionBranch: the projections do not fit the heads")
+        self.qkv, self.out, self.q_weight, self.k_weight, self.eps, self.rope = qkv, out, q_weight, k_weight, eps, rope
+        self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
+        device = qkv.codes.device
+        self.rows = torch.empty(max_tokens, qkv.n, dtype=torch.bfloat16, device=device)
+        self.o = torch.empty(max_tokens, heads, head_dim, dtype=torch.bfloat16, device=device)
+        self._work = [linear.linear_fp8_workspace(w, max_tokens, device) if isinstance(w, linear.Fp8RowWeight) else None for w in (qkv, out)]
+
+    def parts(self, tokens):
+        """q, k and v of the projection's output, [tokens][heads or kv_heads][head_dim]."""
+        q, k, v = self.rows[:tokens].split([self.heads * self.head_dim, self.kv_heads * self.head_dim, self.kv_heads * self.head_dim], dim=1)
+        return tuple(x.unflatten(1, (-1, self.head_dim)) for x in (q, k, v))
+
+    def project(self, x, which, epilogue):
+        w = self.out if which else self.qkv
+        if isinstance(w, linear.Q4GroupWeight):
+            linear.linear_q4_decode(x, w, epilogue)
+        else:
+            linear.linear_fp8(x, w, epilogue, self._work[which])
+
+
+def forward_attention_prefill(branch, x, cu_seqlens, positions, X, inj, cache=None, slots=None):
+    """The attention branch over packed prompts: projection, norms and rotation, causal attention, projection with the residual write X
+    += inj * y (X fp32 [T][4][hidden], inj [T][4]). x bf16 [T][hidden]. With `cache` the keys and values are put to `slots` for
+    forward_attention_decode."""
+    tokens = x.shape[0]
+    branch.project(x, 0, linear.store_bf16(branch.rows[:tokens]))
+    q, k, v = branch.parts(tokens)
+    qk_norm_rope(q, k, None, branch.q_weight, branch.k_weight, branch.eps, branch.rope, positions, q, k, None)
+    if cache is not None:
+        kv_store(k, v, cache, slots)
+    o = branch.o[:tokens]
+    attn_prefill(q, k, v, cu_seqlens, o)
+    branch.project(o.flatten(1), 1, linear.gr_write(X, inj))
+
+
+def forward_attention_decode(branch, x, drafted, cache, block_table, contexts, slots, positions, workspace, X, inj, mask=None):
+    """The attention branch of a decode step: x bf16 [n_seqs * drafted][hidden], the tokens of a sequence one after another; their
+    keys and values go to `slots` of the cache, which are positions contexts[s] .. contexts[s] + drafted - 1 of sequence s. `workspace` of
+    attn_tree_workspace; `mask` as in attn_tree_decode (one token per sequence: plain decoding)."""
+    tokens = x.shape[0]
+    n_seqs = contexts.shape[0]
+    if tokens != n_seqs * drafted:
+        raise ValueError("forward_attention_decode: x holds another number of tokens than contexts say")
+    branch.project(x, 0, linear.store_bf16(branch.rows[:tokens]))
+    q, k, v = branch.parts(tokens)
+    qk_norm_rope(q, k, v, branch.q_weight, branch.k_weight, branch.eps, branch.rope, positions, q, cache.k_rows, cache.v_rows, slots=slots)
+    o = branch.o[:tokens]
+    attn_tree_decode(q.unflatten(0, (n_seqs, drafted)), cache, block_table, contexts, o.unflatten(0, (n_seqs, drafted)), workspace, mask=mask)
+    branch.project(o.flatten(1), 1, linear.gr_write(X, inj))
