@@ -8,12 +8,7 @@
 // lanes hold a head, 16 bytes each, and the next token's values are on their way while this one's are worked on. The angles of a
 // token are made once per block: the product of position and frequency in 64 bits, reduced to a part of a turn there
 // (a position of a million leaves fp32 no more than four correct digits of the angle), the sine and cosine of the rest in fp32.
-#include "common.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include <type_traits>
+#include "attn_common.cuh"
 
 namespace fb {
 namespace {
@@ -42,33 +37,28 @@ struct QkArgs {
   int section_end[4];
 };
 
+// Eight values as pairs of fp32, and back with one rounding each.
 template <class T>
-__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+__device__ __forceinline__ void unpack8(const uint4& v, uint64_t (&f)[4]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (std::is_same<T, __nv_bfloat16>::value) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      f[i] = pair_of(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     } else {
       const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = p.x;
-      f[2 * i + 1] = p.y;
+      f[i] = pair_of(p.x, p.y);
     }
   }
 }
 template <class T>
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+__device__ __forceinline__ uint4 pack8(const uint64_t (&f)[4]) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (std::is_same<T, __nv_bfloat16>::value) {
-      const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&p);
-    } else {
-      const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&p);
-    }
+    float a, b;
+    unpair(f[i], a, b);
+    w[i] = pack2<T>(a, b);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -83,7 +73,7 @@ __device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
 // A block keeps them for the tokens of a tile, in the order in which a warp's lanes read them: 16-byte pieces side by side.
 template <int D>
 struct QkFactors {
-  float4 piece[4][D / 8];  // own 0-3, own 4-7, other 0-3, other 4-7 of each lane's eight values
+  ulonglong2 piece[4][D / 8];  // own 0-3, own 4-7, other 0-3, other 4-7 of each lane's eight values
   __device__ __forceinline__ void set(int e, float own, float other) {
     reinterpret_cast<float*>(&piece[(e >> 2) & 1][e >> 3])[e & 3] = own;
     reinterpret_cast<float*>(&piece[2 + ((e >> 2) & 1)][e >> 3])[e & 3] = other;
@@ -104,15 +94,15 @@ __global__ void __launch_bounds__(kQkThreads, kQkBlocks) qk_norm_rope_kernel(con
   // This thread's rows, the same of every token. Every thread stays for the shuffles; a row behind the last one is not loaded and not
   // stored.
   int kind[kQkRows], off[kQkRows];  // 0 q, 1 k, 2 v, 3 none; values from the token's first
-  bool copies = true;               // nothing but values of v in this warp
+  uint32_t used = 0, turns = 0;     // bit i: the block has rows there; this warp has rows of q or k there
 #pragma unroll
   for (int i = 0; i < kQkRows; ++i) {
     const int row = (i * gridDim.y + blockIdx.y) * kPerPass + slot_row;
     kind[i] = row >= a.rows ? 3 : row >= a.first[2] ? 2 : row >= a.first[1] ? 1 : 0;
     off[i] = (row - (kind[i] == 0 ? a.first[0] : kind[i] == 1 ? a.first[1] : a.first[2])) * D + e0;
-    copies &= kind[i] >= 2;
+    if ((i * int(gridDim.y) + int(blockIdx.y)) * kPerPass < a.rows) used |= 1u << i;
+    if (__any_sync(0xffffffffu, kind[i] < 2)) turns |= 1u << i;
   }
-  copies = __all_sync(0xffffffffu, copies);
   auto load = [&](int64_t token, uint4 (&raw)[kQkRows]) {
     const T* q = static_cast<const T*>(a.in[0]) + token * a.in_stride[0];
     const T* k = static_cast<const T*>(a.in[1]) + token * a.in_stride[1];
@@ -124,6 +114,7 @@ __global__ void __launch_bounds__(kQkThreads, kQkBlocks) qk_norm_rope_kernel(con
   int64_t token0 = int64_t(blockIdx.x) * tile;
   uint4 raw[kQkRows];
   load(token0, raw);
+  int64_t next_slot = a.slots ? a.slots[token0] : 0;
   // Thread and index i take an angle of the tile: (token, frequency), the positions asked for a tile ahead.
   int position[kAngles];
   auto ask = [&](int64_t first) {
@@ -147,6 +138,7 @@ __global__ void __launch_bounds__(kQkThreads, kQkBlocks) qk_norm_rope_kernel(con
     const int e = id % D, w = id / D % 2, t = id / (2 * D) % kQkTile;
     if (e >= 2 * a.half) factors[id / (2 * D * kQkTile)][t][w].set(e, weights[w][e], 0.f);
   }
+  const bool normed[2] = {a.weight[0] != nullptr, a.weight[1] != nullptr};
   const bool turned = e0 < 2 * a.half;
   // The lane that holds the partners of an element pair (i, i + rot / 2), in this head's lanes.
   const int lane = threadIdx.x & 31;
@@ -175,32 +167,38 @@ __global__ void __launch_bounds__(kQkThreads, kQkBlocks) qk_norm_rope_kernel(con
     for (int t = 0; t < here; ++t) {
       const int64_t token = token0 + t, next = t + 1 < here ? token + 1 : token0 + int64_t(gridDim.x) * tile;
       uint4 next_raw[kQkRows];
-      if (next < a.tokens) load(next, next_raw);
-      int64_t slot = token;
-      bool kept = true;
-      if (a.slots) {
-        slot = a.slots[token];
-        kept = slot >= 0 && slot < a.n_slots;
+      const int64_t slot = a.slots ? next_slot : token;
+      const bool kept = !a.slots || (slot >= 0 && slot < a.n_slots);
+      if (next < a.tokens) {
+        load(next, next_raw);
+        if (a.slots) next_slot = a.slots[next];
       }
       T* q = static_cast<T*>(a.out[0]) + token * a.out_stride[0];
       T* k = static_cast<T*>(a.out[1]) + slot * a.out_stride[1];
       T* v = static_cast<T*>(a.out[2]) + slot * a.out_stride[2];
 #pragma unroll
       for (int i = 0; i < kQkRows; ++i) {
+        if (!((used >> i) & 1)) break;
         uint4 result = raw[i];
-        if (!copies) {
+        if ((turns >> i) & 1) {
           const QkFactors<D>& f = factors[buffer][t][kind[i] == 1];
-          float x[8], p[8];
+          uint64_t x[4], p[4];
           unpack8<T>(raw[i], x);
-          float sum = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+          uint64_t sum2 = fma2(x[1], x[1], fma2(x[0], x[0], 0));
+          sum2 = add2(sum2, fma2(x[3], x[3], fma2(x[2], x[2], 0)));
+          float sum, high;
+          unpair(sum2, sum, high);
+          sum += high;
 #pragma unroll
           for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-          const float r = a.weight[kind[i] & 1] ? rsqrtf(sum * (1.f / D) + a.eps) : 1.f;
+          const float r = normed[kind[i] == 1] ? rsqrtf(fmaf(sum, 1.f / D, a.eps)) : 1.f;
           if (a.adjacent) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = x[e ^ 1];
+            for (int e = 0; e < 4; ++e) {
+              float lo, hi;
+              unpair(x[e], lo, hi);
+              p[e] = pair_of(hi, lo);
+            }
           } else {
             uint4 other;
             other.x = __shfl_sync(0xffffffffu, raw[i].x, partner);
@@ -209,16 +207,18 @@ __global__ void __launch_bounds__(kQkThreads, kQkBlocks) qk_norm_rope_kernel(con
             other.w = __shfl_sync(0xffffffffu, raw[i].w, partner);
             unpack8<T>(other, p);
           }
-          const float4 o0 = f.piece[0][l], o1 = f.piece[1][l];
-          float y[8] = {x[0] * o0.x, x[1] * o0.y, x[2] * o0.z, x[3] * o0.w, x[4] * o1.x, x[5] * o1.y, x[6] * o1.z, x[7] * o1.w};
+          const ulonglong2 o0 = f.piece[0][l], o1 = f.piece[1][l];
+          const uint64_t rr = pair_of(r, r);
+          uint64_t y[4] = {fma2(x[0], o0.x, 0), fma2(x[1], o0.y, 0), fma2(x[2], o1.x, 0), fma2(x[3], o1.y, 0)};
           if (turned) {
-            const float4 t0 = f.piece[2][l], t1 = f.piece[3][l];
-            const float other[8] = {t0.x, t0.y, t0.z, t0.w, t1.x, t1.y, t1.z, t1.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = fmaf(p[e], other[e], y[e]);
+            const ulonglong2 t0 = f.piece[2][l], t1 = f.piece[3][l];
+            y[0] = fma2(p[0], t0.x, y[0]);
+            y[1] = fma2(p[1], t0.y, y[1]);
+            y[2] = fma2(p[2], t1.x, y[2]);
+            y[3] = fma2(p[3], t1.y, y[3]);
           }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] *= r;
+          for (int e = 0; e < 4; ++e) y[e] = fma2(y[e], rr, 0);
           if (kind[i] < 2) result = pack8<T>(y);
         }
         if (kind[i] == 0 || (kind[i] < 3 && kept))
@@ -327,8 +327,10 @@ int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm
   int share = (passes + kQkRows - 1) / kQkRows;
   while (share < passes && int64_t(tokens) * share < sm_count()) share = 2 * share < passes ? 2 * share : passes;
   a.tokens = tokens;
+  // (tiles of four tokens where every block gets two of them: 8192 tokens of 48 heads 61 us in tiles of four or two, 67 one by one)
   a.tile = int64_t(tokens) * share >= 2 * int64_t(kQkTile) * room ? kQkTile : 1;
-  const int tiles = (tokens + a.tile - 1) / a.tile, across = room / share > 0 ? room / share : 1;
+  const int across = room / share > 0 ? room / share : 1;
+  const int tiles = (tokens + a.tile - 1) / a.tile;
   const dim3 grid(unsigned(tiles < across ? tiles : across), unsigned(share));
   const cudaError_t e = in->dtype == FB_DT_BF16 ? launch_qk<__nv_bfloat16>(a, dim, grid, as_stream(stream))
                                                 : launch_qk<__half>(a, dim, grid, as_stream(stream));
