@@ -120,6 +120,8 @@ __device__ __forceinline__ void regs_down() {
 }
 
 // ------------------------------------------------------------------------------ copies and products
+// Brings a tensor map (a kernel parameter) to where copies look for it.
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
                    dst),

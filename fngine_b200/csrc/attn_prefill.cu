@@ -61,6 +61,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
   uint8_t* ring = smem + 2 * S::kTileBytes;
   PfBars* bars = reinterpret_cast<PfBars*>(ring + kStages * S::kTileBytes);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 9 * 32) {
+    prefetch_map(&maps.q);
+    prefetch_map(&maps.k);
+    prefetch_map(&maps.v);
+  }
   pdl_wait_prior();
 
   // Which sequence and which 256 queries: item blockIdx.y counts the items of the sequences in order, each from its end.
@@ -107,7 +112,18 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (tid == 0) {
+  // (the copying thread makes the barriers and begins, while the others are on their way)
+  constexpr int kCopier = 9 * 32, kEarly = 3;  // copies of keys and values before the barrier
+  auto copy = [&](uint8_t* dst, const CUtensorMap* map, int h, int row, uint64_t* bar) {
+    mbar_expect_tx(bar, S::kTileBytes);
+    for (int p = 0; p < kParts; ++p) tma_load_3d(smem_u32(dst) + p * S::kHalf, map, p * 64, h, row, bar);
+  };
+  auto copy_block = [&](int i) {  // K_0 V_0 K_1 V_1 ...
+    const int slot = i % kStages;
+    copy(ring + slot * S::kTileBytes, i & 1 ? &maps.v : &maps.k, kv_head, start + (i >> 1) * kPfRows, &bars->full[slot]);
+    bars->issued = i + 1;
+  };
+  if (tid == kCopier) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->q_full[i], 1);
       mbar_init(&bars->s_full[i], 1);
@@ -124,6 +140,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
     bars->aborted = 0;
     bars->issued = 0;
     mbar_fence_init();
+    copy(q_tiles, &maps.q, head, start + row0, &bars->q_full[0]);
+    copy_block(0);
+    if (blocks1) copy(q_tiles + S::kTileBytes, &maps.q, head, start + row0 + kPfRows, &bars->q_full[1]);
+    for (int i = 1; i < kEarly && i < 2 * blocks; ++i) copy_block(i);
   }
   tc_fence_before();
   __syncthreads();
@@ -140,18 +160,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
   if (warp == 9) {
     // ------------------------------------------------------------------ copies
     if (lane == 0) {
-      auto tile = [&](uint8_t* dst, const CUtensorMap* map, int h, int row, uint64_t* bar) {
-        mbar_expect_tx(bar, S::kTileBytes);
-        for (int p = 0; p < kParts; ++p) tma_load_3d(smem_u32(dst) + p * S::kHalf, map, p * 64, h, row, bar);
-      };
-      tile(q_tiles, &maps.q, head, start + row0, &bars->q_full[0]);
-      for (int i = 0; i < 2 * blocks; ++i) {  // K_0 V_0 K_1 V_1 ...
-        const int slot = i % kStages;
-        if (i >= kStages && !bounded_wait(&bars->aborted, a.status, &bars->empty[slot], uint32_t(i / kStages - 1) & 1)) break;
-        tile(ring + slot * S::kTileBytes, i & 1 ? &maps.v : &maps.k, kv_head, start + (i >> 1) * kPfRows, &bars->full[slot]);
-        bars->issued = i + 1;
-        if (i == 0 && blocks1)
-          tile(q_tiles + S::kTileBytes, &maps.q, head, start + row0 + kPfRows, &bars->q_full[1]);
+      for (int i = kEarly; i < 2 * blocks; ++i) {
+        if (i >= kStages && !bounded_wait(&bars->aborted, a.status, &bars->empty[i % kStages], uint32_t(i / kStages - 1) & 1)) break;
+        copy_block(i);
       }
     }
     __syncwarp();
