@@ -476,13 +476,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
             uint32_t p[16];
             tmem_ld32(s_at + 32 * (i + 1), s1);
             unseen(i, s0);
-            scores_exp<T, D == 128>(s0, scale, minus, p, part);
+            scores_exp<T, false>(s0, scale, minus, p, part);
             tmem_st16(s_at + 16 * i, p);  // (over scores that have been read)
             tmem_ld_wait();
             tmem_landed(s1);
             tmem_ld32(s_at + 64, s0);  // (of no use in the second turn, whose weights begin at column 32)
             unseen(i + 1, s1);
-            scores_exp<T, D == 128>(s1, scale, minus, p, part);
+            scores_exp<T, false>(s1, scale, minus, p, part);
             tmem_st16(s_at + 16 * (i + 1), p);
             tmem_ld_wait();
             tmem_landed(s0);

@@ -215,3 +215,38 @@ def test_captured_calls_follow_the_contexts():
             graph.replay()
             s.synchronize()
             compare(out, *reference(torch, q, kc, vc, table, contexts, None))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_that_see_nothing_and_rows_that_see_one_key(dim, dtype):
+    """Exact zeros and exact copies: a weight of a hidden key that is not zero, however small, would show in both."""
+    torch = _torch()
+    from fngine_b200 import attention as A
+    q, kc, vc, table, ctx = setup(torch, 2, 64, 4, 2, dim, 16, [0, 0], dtype, 12)
+    mask = torch.tensor([[0 if i % 3 else 1 << i if i < 63 else -(1 << 63) for i in range(64)]] * 2, device="cuda")
+    ws, out = A.attn_tree_workspace(2, 64, 4, 2, dim), torch.full_like(q, float("nan"))
+    A.attn_tree_decode(q, A.KvCache(kc, vc), table, ctx, out, ws, mask=mask)
+    torch.cuda.synchronize()
+    for s in range(2):
+        for i in range(64):
+            v = vc[int(table[s, i // 16]), i % 16].repeat_interleave(2, 0)
+            assert torch.equal(out[s, i], v if i % 3 == 0 else torch.zeros_like(v))
+    vc[int(table[1, 0]), 6] = float("nan")  # a key that one row sees: NaN in that row
+    A.attn_tree_decode(q, A.KvCache(kc, vc), table, ctx, out, ws, mask=mask)
+    torch.cuda.synchronize()
+    assert bool(torch.isnan(out[1, 6]).all()) and not bool(torch.isnan(out[0]).any())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_not_a_number_reaches_the_rows_that_see_it(dim):
+    """A key of the context that is not a number: every row of its sequence and key head, and no other."""
+    torch = _torch()
+    from fngine_b200 import attention as A
+    for at in range(0, 300, 37):
+        q, kc, vc, table, ctx = setup(torch, 2, 3, 4, 2, dim, 16, [300, 200], "bfloat16", 13)
+        kc[int(table[0, at // 16]), at % 16, 1] = float("nan")
+        ws, out = A.attn_tree_workspace(2, 3, 4, 2, dim), torch.zeros_like(q)
+        A.attn_tree_decode(q, A.KvCache(kc, vc), table, ctx, out, ws)
+        torch.cuda.synchronize()
+        assert bool(torch.isnan(out[0, :, 2:]).all()) and not bool(torch.isnan(out[0, :, :2]).any()) and not bool(torch.isnan(out[1]).any())
