@@ -28,9 +28,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // ------------------------------------------------------------------------------ a row's scores, 32 at a time
+// (NaN wins over numbers)
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ uint64_t pair_of(float a, float b) {
@@ -62,12 +63,12 @@ __device__ __forceinline__ float scores_max(const float (&s)[32], float m) {
 }
 // 2^x of a pair on the multiply-add pipe: x = n + f with n whole and |f| <= 1/2 (adding 1.5 * 2^23 rounds to whole numbers and leaves
 // n in the low bits), a polynomial of degree four for 2^f (minimax by Remez exchange, relative error 2.7e-6), n into the exponent.
-// Below -126 it stays at 2^-126, so not for scores that are masked; NaN does not turn into a number that passes for a weight.
+// Below -126 it stays at 2^-126, so not for scores that are masked. NaN does not stay NaN: the row's maximum has to show it.
 __device__ __forceinline__ void exp2_poly(uint64_t x2, float& x, float& y) {
   float a, b;
   unpair(x2, a, b);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  a = fmaxf(a, -126.f);
+  b = fmaxf(b, -126.f);
   x2 = pair_of(a, b);
   constexpr float kRound = 12582912.f;
   const uint64_t t = add2(x2, pair_of(kRound, kRound));

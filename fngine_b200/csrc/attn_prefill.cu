@@ -272,14 +272,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
       float latest = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i) latest = scores_max(s[i], latest);
-      // (always in the first block; rows behind the sequence are nobody's and decide nothing)
-      const bool rises = real && (latest - top) * a.scale_log2 > kPfSlack;
+      // (always in the first block; from a score that is NaN on, with the maximum, the sum and the outputs NaN; rows behind the sequence
+      // are nobody's and decide nothing)
+      const bool rises = real && !((latest - top) * a.scale_log2 <= kPfSlack);
       // P and O are free: the block before's product is done.
       if (j > 0) ok = bounded_wait_warp(&bars->aborted, a.status, &bars->o_done[t], uint32_t(j - 1) & 1);
       if (!ok) break;
       tc_fence_after();
       if (__any_sync(0xffffffffu, rises)) {
-        const float up = fmaxf(latest, top);
+        const float up = max3(latest, top, top);
         const float fade = exp2_approx((top - up) * a.scale_log2);
         top = up;
         sum *= fade;

@@ -181,3 +181,20 @@ def test_lengths_that_make_no_sense_stay_within_the_tensors():
     torch.cuda.synchronize()
     check(torch, out, q, k, v, 0, 50)
     assert bool((out[50:100] == 5).all())
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_key_that_is_not_a_number_reaches_the_rows_that_see_it(dim):
+    """One key that is not a number, at every place of a group of 32: NaN in the rows from it on, and in no other."""
+    torch = _torch()
+    from fngine_b200 import attention as A
+    g = torch.Generator(device="cuda").manual_seed(5)
+    q, k, v = (torch.randn(300, 2, dim, generator=g, device="cuda").bfloat16() for _ in range(3))
+    cu = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    for at in list(range(32)) + [33, 101, 127, 128, 140, 172, 255, 256, 299]:
+        bad, out = k.clone(), torch.zeros_like(q)
+        bad[at, 1, dim // 2] = float("nan")
+        A.attn_prefill(q, bad, v, cu, out)
+        torch.cuda.synchronize()
+        nan = torch.isnan(out)
+        assert not bool(nan[:, 0].any()) and not bool(nan[:at, 1].any()) and bool(nan[at:, 1].all()), at
