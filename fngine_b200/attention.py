@@ -137,7 +137,8 @@ class KvCache:
 
 
 def attn_tree_workspace(n_seqs, drafted, heads, kv_heads, head_dim, device="cuda"):
-    """Zero-filled workspace of attn_tree_decode for up to n_seqs sequences of these shapes; every call leaves it ready for the next."""
+    """Zero-filled workspace of attn_tree_decode for up to n_seqs sequences of these shapes, and for all others that need no more bytes;
+    every call leaves it ready for the next."""
     n = L.load().fb_attn_tree_workspace_bytes(n_seqs, drafted, heads, kv_heads, head_dim)
     if not n:
         raise ValueError("attn_tree_workspace: unsupported shape")

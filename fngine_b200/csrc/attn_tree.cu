@@ -651,6 +651,8 @@ int tree_row_tiles(int drafted, int group) {
   const int t = tree_tile_tokens(drafted, group);
   return (drafted + t - 1) / t;
 }
+// Partial results lie in front of the counters, at one size for all shapes: what one call leaves there is no counter of another.
+constexpr size_t kTreePartialBytes = size_t(2 * kTreeMaxSms) * kTreeRows * (128 + 2) * 4;
 size_t tree_counter_bytes(int64_t n_seqs, int drafted, int heads, int kv_heads) {
   return (size_t(n_seqs) * kv_heads * tree_row_tiles(drafted, heads / kv_heads) * 4 + 255) & ~size_t(255);
 }
@@ -688,7 +690,7 @@ extern "C" {
 
 size_t fb_attn_tree_workspace_bytes(int32_t n_seqs, int32_t drafted, int32_t heads, int32_t kv_heads, int32_t head_dim) {
   if (!tree_shape_ok(n_seqs, drafted, heads, kv_heads, head_dim)) return 0;
-  return 256 + tree_counter_bytes(n_seqs, drafted, heads, kv_heads) + size_t(2 * kTreeMaxSms) * kTreeRows * (head_dim + 2) * 4;
+  return 256 + kTreePartialBytes + tree_counter_bytes(n_seqs, drafted, heads, kv_heads);
 }
 
 int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int32_t n_seqs, int32_t drafted,
@@ -736,8 +738,8 @@ int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int3
   a.table_stride = table_stride;
   uint8_t* base = static_cast<uint8_t*>(workspace);
   a.status = reinterpret_cast<uint32_t*>(base);
-  a.counters = reinterpret_cast<int32_t*>(base + 256);
-  a.partial = reinterpret_cast<float*>(base + 256 + tree_counter_bytes(n_seqs, drafted, heads, kv));
+  a.partial = reinterpret_cast<float*>(base + 256);
+  a.counters = reinterpret_cast<int32_t*>(base + 256 + kTreePartialBytes);
   a.scale_log2 = scale * 1.4426950408889634f;  // scores are kept in powers of two
   a.n_pages = int(cache->n_pages);
   a.n_seqs = n_seqs;

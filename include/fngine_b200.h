@@ -509,7 +509,7 @@ typedef struct fb_qk_norm {
 typedef struct fb_rope {
   const float* inv_freq;     /* [rot_dim / 2] */
   const int32_t* positions;  /* [axes][tokens] */
-  int64_t axis_stride;       /* elements between the positions of two axes */
+  int64_t axis_stride;       /* elements between the positions of two axes; 0: one row of positions for all */
   int32_t rot_dim;           /* leading values of a head that are turned: a multiple of 16 */
   int32_t axes;              /* 1..4 */
   int32_t sections[4];       /* frequencies of each axis, in their order; they add up to rot_dim / 2 (not read for one axis) */
@@ -529,7 +529,7 @@ typedef struct fb_qkv_out {
 /* y = x * rsqrt(mean(x^2) + eps) * weight per head of q and k (norm NULL or a weight NULL: y = x), then the rotation
  * (a, b) -> (a cos p - b sin p, b cos p + a sin p) of every pair, p = position * inv_freq of the pair's frequency, formed in 64
  * bits (rope NULL: none); v is copied. One pass, fp32 arithmetic, one rounding. With `slots` k and v go to rows of a
- * cache (page * page_size + offset of a paged one): slots that differ from token to token; a negative one or one behind n_slots
+ * cache (page * page_size + offset of a paged one): slots that differ from token to token (of two tokens with one slot, parts of either stay); a negative one or one behind n_slots
  * stores nothing, q is stored all the same. Any of q, k, v may be NULL together with its output. An output may be its input
  * exactly (same address and stride, no slots) or lie apart from all inputs. head_dim 64, 128 or 256; everything 16-byte
  * aligned, strides multiples of 8 elements. */
@@ -543,7 +543,7 @@ int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm
  * of all sequences are left as they were. A sequence's result does not depend on what lies beside it; its own keys and values are to
  * be finite. Softmax statistics and sums are fp32, the weights are rounded to the type of v; repeated calls are bitwise
  * identical. cu_seqlens is read on the device. `status` (one device word, may be NULL) is set to FB_STATUS_PIPELINE_TIMEOUT when a bounded
- * wait ran out. No workspace. head_dim 64 or 128; everything 16-byte aligned, strides multiples of 8 elements. */
+ * wait ran out. No workspace. out lies apart from q, k and v. head_dim 64 or 128; everything 16-byte aligned, strides multiples of 8 elements. */
 int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seqlens, int32_t n_seqs, float scale, void* out,
                         int64_t out_stride, uint32_t* status, void* stream);
 
@@ -571,8 +571,8 @@ typedef struct fb_kv_cache {
  * work are in a fixed order: repeated calls are bitwise identical.
  * `workspace`: fb_attn_tree_workspace_bytes() bytes (0 for an unsupported shape), 256-byte aligned, zero-filled once; the
  * call leaves its counters clear. Its first word is a status (FB_STATUS_*): FB_STATUS_PIPELINE_TIMEOUT once a bounded wait has run out,
- * after which it is to be zero-filled again. Calls that share one must not overlap, captured ones included, and have the
- * same shapes or are separated by a zero-fill. head_dim 64 or 128, up to 128 query heads per key head, up to 2^31 - 1 slots. */
+ * after which it is to be zero-filled again. Calls that share one must not overlap, captured ones included; their shapes may
+ * differ. out lies apart from q and the cache. head_dim 64 or 128, up to 128 query heads per key head, up to 2^31 - 1 slots. */
 size_t fb_attn_tree_workspace_bytes(int32_t n_seqs, int32_t drafted, int32_t heads, int32_t kv_heads, int32_t head_dim);
 int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int32_t n_seqs, int32_t drafted,
                             const fb_kv_cache* cache, const int32_t* block_table, int64_t table_stride, const int32_t* contexts,

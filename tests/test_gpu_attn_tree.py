@@ -250,3 +250,27 @@ def test_not_a_number_reaches_the_rows_that_see_it(dim):
         A.attn_tree_decode(q, A.KvCache(kc, vc), table, ctx, out, ws)
         torch.cuda.synchronize()
         assert bool(torch.isnan(out[0, :, 2:]).all()) and not bool(torch.isnan(out[0, :, :2]).any()) and not bool(torch.isnan(out[1]).any())
+
+
+def test_calls_of_different_shapes_share_a_workspace():
+    """More sequences, fewer, another head_dim, another number of row tiles, one after another and back."""
+    torch = _torch()
+    from fngine_b200 import attention as A
+    shapes = [(2, 3, 8, 2, 128, [9000, 12000]), (300, 2, 4, 2, 64, [(53 * j) % 700 for j in range(300)]), (3, 16, 48, 2, 128, [4000, 2000, 77]),
+              (1, 1, 4, 4, 64, [30000])]
+    size = max((A.attn_tree_workspace(*s[:5]) for s in shapes), key=lambda w: w.numel())
+    ws = torch.zeros(size.numel() + 256, dtype=torch.uint8, device="cuda")
+    ws = ws[-ws.data_ptr() % 256:][:size.numel()]
+    first = []
+    for turn in range(2):
+        for i, (seqs, drafted, heads, kv, dim, contexts) in enumerate(shapes if not turn else shapes[::-1]):
+            q, kc, vc, table, ctx = setup(torch, seqs, drafted, heads, kv, dim, 16, contexts, "bfloat16", dim + seqs)
+            out = torch.full_like(q, float("nan"))
+            A.attn_tree_decode(q, A.KvCache(kc, vc), table, ctx, out, ws)
+            torch.cuda.synchronize()
+            if turn:
+                assert torch.equal(out, first[-1 - i])
+            else:
+                compare(out, *reference(torch, q, kc, vc, table, contexts, None))
+                first.append(out)
+    assert A.attn_tree_status(ws) == 0
