@@ -309,7 +309,7 @@ int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm
       a.section_end[i] = end += n;
     }
     if (end != a.half) return invalid("qk_norm_rope: the sections do not add up to rot_dim / 2");
-    if (rope->axes > 1 && rope->axis_stride < tokens) return invalid("qk_norm_rope: axis_stride is smaller than tokens");
+    if (rope->axes > 1 && rope->axis_stride && rope->axis_stride < tokens) return invalid("qk_norm_rope: axis_stride is smaller than tokens");
     // (axes behind the last one are never reached: a frequency is below the last section's end)
     a.adjacent = rope->adjacent != 0;
     a.inv_freq = rope->inv_freq;

@@ -158,3 +158,43 @@ def test_captured_and_chained():
         graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def test_one_row_of_positions_for_all_axes():
+    """A position row that is expanded to the axes (no memory of its own) is the same as three equal rows, and as one axis."""
+    torch = _torch()
+    from fngine_b200 import attention as A
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    q, k = torch.randn(50, 4, 64, generator=gen, device="cuda").bfloat16(), torch.randn(50, 2, 64, generator=gen, device="cuda").bfloat16()
+    pos = torch.randint(0, 5000, (1, 50), generator=gen, device="cuda", dtype=torch.int32)
+    inv = (1e4 ** (-torch.arange(32, device="cuda") / 32)).float()
+    outs = []
+    for sections, p in (((10, 12, 10), pos.expand(3, 50)), ((10, 12, 10), pos.repeat(3, 1)), (None, pos)):
+        qo, ko = torch.empty_like(q), torch.empty_like(k)
+        A.qk_norm_rope(q, k, None, None, None, 0.0, A.Rope(inv, sections), p, qo, ko, None)
+        outs.append((qo, ko))
+    torch.cuda.synchronize()
+    for a, b in outs[1:]:
+        assert torch.equal(a, outs[0][0]) and torch.equal(b, outs[0][1])
+
+
+def test_offsets_beyond_32_bits():
+    """Tokens some 10 GB behind the first one, into slots as far behind the first one."""
+    torch = _torch()
+    from fngine_b200 import attention as A
+    tokens, H, K, D = 200000, 2, 1, 128
+    wide = torch.zeros(tokens, 24576, dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    wide[-300:] = torch.randn(300, 24576, generator=gen, device="cuda").bfloat16()
+    q, k, v = wide[:, 128:384].unflatten(1, (H, D)), wide[:, 1024:1152].unflatten(1, (K, D)), wide[:, 24448:].unflatten(1, (K, D))
+    ko, vo = (wide[:, c:c + D].unflatten(1, (K, D)) for c in (8192, 16384))
+    slots = torch.full((tokens,), -1, device="cuda")
+    slots[-300:] = torch.arange(tokens - 1, tokens - 301, -1, device="cuda")
+    pos = torch.arange(tokens, device="cuda", dtype=torch.int32)
+    inv = (1e4 ** (-torch.arange(64, device="cuda") / 64)).float()
+    want = [reference(torch, x[-300:], None, 0.0, inv, pos[None, -300:], (64,), False) for x in (q, k)]
+    A.qk_norm_rope(q, k, v, None, None, 0.0, A.Rope(inv), pos, q, ko, vo, slots=slots)
+    torch.cuda.synchronize()
+    check(torch, q[-300:], *want[0])
+    check(torch, ko[-300:].flip(0), *want[1])
+    assert torch.equal(vo[-300:].flip(0), v[-300:]) and not bool(ko[:-300].any())
