@@ -218,6 +218,18 @@ class AttentionBranch:
         q, k, v = self.rows[:tokens].split([self.heads * self.head_dim, self.kv_heads * self.head_dim, self.kv_heads * self.head_dim], dim=1)
         return tuple(x.unflatten(1, (-1, self.head_dim)) for x in (q, k, v))
 
+    def check(self, x, X, inj):
+        """Number of tokens of x [tokens][hidden], once everything that the calls behind go by fits it."""
+        tokens, hidden = x.shape
+        if tokens > self.o.shape[0]:
+            raise ValueError("AttentionBranch: %d tokens, made for up to %d" % (tokens, self.o.shape[0]))
+        if hidden != self.qkv.k or X.shape != (tokens, 4, self.out.n) or inj.shape != (tokens, 4):
+            raise ValueError("AttentionBranch: x [tokens][%d], X [tokens][4][%d], inj [tokens][4]" % (self.qkv.k, self.out.n))
+        dev = _device()
+        if not (x.get_device() == X.get_device() == inj.get_device() == self.o.get_device() == dev):
+            raise ValueError("AttentionBranch: not on the current device")
+        return tokens
+
     def project(self, x, which, epilogue):
         w = self.out if which else self.qkv
         if isinstance(w, linear.Q4GroupWeight):
@@ -230,7 +242,9 @@ def forward_attention_prefill(branch, x, cu_seqlens, positions, X, inj, cache=No
     """The attention branch over packed prompts: projection, norms and rotation, causal attention, projection with the residual write X
     += inj * y (X fp32 [T][4][hidden], inj [T][4]). x bf16 [T][hidden]. With `cache` the keys and values are put to `slots` for
     forward_attention_decode."""
-    tokens = x.shape[0]
+    tokens = branch.check(x, X, inj)
+    if not tokens:
+        return
     branch.project(x, 0, linear.store_bf16(branch.rows[:tokens]))
     q, k, v = branch.parts(tokens)
     qk_norm_rope(q, k, None, branch.q_weight, branch.k_weight, branch.eps, branch.rope, positions, q, k, None)
@@ -245,10 +259,12 @@ def forward_attention_decode(branch, x, drafted, cache, block_table, contexts, s
     """The attention branch of a decode step: x bf16 [n_seqs * drafted][hidden], the tokens of a sequence one after another; their
     keys and values go to `slots` of the cache, which are positions contexts[s] .. contexts[s] + drafted - 1 of sequence s. `workspace` of
     attn_tree_workspace; `mask` as in attn_tree_decode (one token per sequence: plain decoding)."""
-    tokens = x.shape[0]
+    tokens = branch.check(x, X, inj)
     n_seqs = contexts.shape[0]
     if tokens != n_seqs * drafted:
         raise ValueError("forward_attention_decode: x holds another number of tokens than contexts say")
+    if not tokens:
+        return
     branch.project(x, 0, linear.store_bf16(branch.rows[:tokens]))
     q, k, v = branch.parts(tokens)
     qk_norm_rope(q, k, v, branch.q_weight, branch.k_weight, branch.eps, branch.rope, positions, q, cache.k_rows, cache.v_rows, slots=slots)

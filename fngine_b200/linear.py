@@ -122,11 +122,16 @@ class Q4GroupWeight:
 _DTYPES = {torch.float32: L.DT_F32, torch.bfloat16: L.DT_BF16, torch.float16: L.DT_F16}
 
 
+_VALUES = {L.EPI_GR_WRITE: 4, L.EPI_SWIGLU: 0.5}  # of an output per row and token
+
+
 def linear_q4_decode(x, weight, epilogue):
     """fb_linear_q4_decode: x bf16 [T][k], T <= 16; the output is whatever `epilogue` (store_bf16, store_f32, gr_write,
     swiglu, shared_scale) names. Products are exact and sums fp32."""
     assert x.dtype == torch.bfloat16 and x.is_contiguous() and x.shape[1] == weight.k
     assert x.get_device() == weight.codes.get_device() == torch._C._cuda_getDevice()
+    out, values = epilogue._keep[0], x.shape[0] * weight.n
+    assert out.get_device() == x.get_device() and out.numel() == _VALUES.get(epilogue.kind, 1) * values
     st = L.load().fb_linear_q4_decode(x.data_ptr(), x.shape[0], weight.ref, ctypes.byref(epilogue), L.stream())
     if st:
         L.check(st, "linear_q4_decode")

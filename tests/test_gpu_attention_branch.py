@@ -158,3 +158,60 @@ def test_arguments():
     q = torch.zeros(4, HEADS, DIM, dtype=torch.bfloat16)  # not on the GPU
     with pytest.raises(ValueError):
         A.attn_prefill(q, q, q, torch.tensor([0, 4], dtype=torch.int32), q)
+
+
+def test_a_branch_refuses_what_does_not_fit():
+    """More tokens than its buffers hold, streams or inj of other shapes; no tokens at all are not an error."""
+    torch = _torch()
+    from fngine_b200 import attention as A
+    branch = make_branch(torch, "fp8", 32)
+    make = lambda t: (torch.zeros(t, HIDDEN, device="cuda", dtype=torch.bfloat16), torch.zeros(t, 4, HIDDEN, device="cuda"), torch.ones(t, 4, device="cuda"))
+    cu, pos = torch.tensor([0, 0], device="cuda", dtype=torch.int32), torch.zeros(33, device="cuda", dtype=torch.int32)
+    for x, X, inj in (make(33), (make(4)[0], make(3)[1], make(4)[2]), (make(4)[0], make(4)[1], make(5)[2]), (make(4)[0][:, :640].contiguous(), *make(4)[1:]),
+                      (make(4)[0], make(4)[1].cpu(), make(4)[2])):
+        with pytest.raises(ValueError):
+            A.forward_attention_prefill(branch, x, cu, pos[:x.shape[0]], X, inj)
+        with pytest.raises(ValueError):
+            A.forward_attention_decode(branch, x, 1, None, None, torch.zeros(x.shape[0], device="cuda", dtype=torch.int32), None, pos[:x.shape[0]], None, X, inj)
+    x, X, inj = make(0)
+    A.forward_attention_prefill(branch, x, cu, pos[:0], X, inj)
+    A.forward_attention_decode(branch, x, 1, None, None, torch.zeros(0, device="cuda", dtype=torch.int32), None, pos[:0], None, X, inj)
+
+
+def test_a_captured_decode_step_follows_its_inputs():
+    """A step captured once and replayed as the sequences grow, on another stream than it was captured on, against steps without a graph."""
+    torch = _torch()
+    from fngine_b200 import attention as A
+    seqs, page = 3, 16
+    branch = make_branch(torch, "q4", 16)
+    gen = torch.Generator(device="cuda").manual_seed(23)
+    kc, vc = (torch.randn(40, page, KV, DIM, generator=gen, device="cuda").bfloat16() for _ in "kv")
+    table = torch.randperm(39, generator=gen, device="cuda").int().view(3, 13)
+    cache, ws = A.KvCache(kc, vc), A.attn_tree_workspace(seqs, 1, HEADS, KV, DIM)
+    x, inj = torch.randn(seqs, HIDDEN, generator=gen, device="cuda").bfloat16(), torch.randn(seqs, 4, generator=gen, device="cuda")
+    X, ctx, slots = torch.zeros(seqs, 4, HIDDEN, device="cuda"), torch.zeros(seqs, dtype=torch.int32, device="cuda"), torch.zeros(seqs, dtype=torch.int64, device="cuda")
+    step = lambda: A.forward_attention_decode(branch, x, 1, cache, table, ctx, slots, ctx, ws, X, inj)
+
+    def at(contexts):
+        ctx.copy_(torch.tensor(contexts, dtype=torch.int32))
+        slots.copy_(torch.tensor([int(table[s, c // page]) * page + c % page for s, c in enumerate(contexts)]))
+        X.zero_()
+
+    at([0, 5, 100])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        step()
+        with torch.cuda.graph(graph, stream=s):
+            step()
+    torch.cuda.synchronize()
+    for contexts in ([0, 5, 100], [1, 6, 101], [200, 31, 32]):
+        at(contexts)
+        graph.replay()
+        got = X.clone()
+        at(contexts)
+        step()
+        assert torch.equal(got, X) and bool(got.any())
+    torch.cuda.synchronize()
+    assert A.attn_tree_status(ws) == 0

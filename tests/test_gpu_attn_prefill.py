@@ -2,8 +2,8 @@
 
 The tolerance: weights are rounded once to the type of v (half a step h of each: bf16 2^-8, fp16 2^-11), so an output is off by at most h
 sum_j w_j |v_j| = h B; scores are fp32 sums of D products (D 2^-23 sum |scale q k|, which moves a weight by that relative part, and the
-exponential another 2^-21): 2 (D 2^-23 S + 2^-21) B with S the row's largest sum |scale q k|; sums over the keys 2^-18 B; and
-half a step of the output. Weights below fp16's normal range are off by 2^-25 of the largest at most (the largest in use is at
+exponential another 2^-18, of which a polynomial's 2.7e-6 < 2^-18.4 is the most, its roundings and the scaled score's 2^-21): 2 (D
+2^-23 S + 2^-18) B with S the row's largest sum |scale q k|; sums over the keys 2^-18 B; and half a step of the output. Weights below fp16's normal range are off by 2^-25 of the largest at most (the largest in use is at
 least 2^-8 of the one that the exponents refer to, which loses eight bits there: 2^-17): 2^-17 sum |v| w_max over the keys."""
 import pytest
 
@@ -35,7 +35,7 @@ def check(torch, out, q, k, v, a, b, scale=None):
         w = torch.softmax((qq @ kk.T * scale).masked_fill_(later, -float("inf")), 1)
         want, B = w @ vv, w @ vv.abs()
         S = ((qq.abs() @ kk.abs().T) * scale).masked_fill_(later, 0).amax(1, keepdim=True)
-        tol = (h + 2 * (D * 2.0 ** -23 * S + 2.0 ** -21) + 2.0 ** -18) * B
+        tol = (h + 2 * (D * 2.0 ** -23 * S + 2.0 ** -18) + 2.0 ** -18) * B
         least = 0.0
         if q.dtype == torch.float16:
             tol = tol + 2.0 ** -17 * w.amax(1, keepdim=True) * vv.abs().cumsum(0)
@@ -198,3 +198,21 @@ def test_a_key_that_is_not_a_number_reaches_the_rows_that_see_it(dim):
         torch.cuda.synchronize()
         nan = torch.isnan(out)
         assert not bool(nan[:, 0].any()) and not bool(nan[:at, 1].any()) and bool(nan[at:, 1].all()), at
+
+
+def test_offsets_beyond_32_bits():
+    """Tokens that lie some 10 GB behind the first one."""
+    torch = _torch()
+    from fngine_b200 import attention as A
+    tokens, H, K, D = 200000, 2, 1, 128
+    wide = torch.empty(tokens, 24576, dtype=torch.bfloat16, device="cuda")
+    first = tokens - 700
+    wide[first:] = torch.randn(700, 24576, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").bfloat16()
+    q, k, v, out = wide[:, 128:128 + H * D].unflatten(1, (H, D)), wide[:, 1024:1024 + D].unflatten(1, (K, D)), wide[:, 24448:].unflatten(1, (K, D)), None
+    out = wide[:, 4096:4096 + H * D].unflatten(1, (H, D))
+    cu = torch.tensor([first, tokens - 200, tokens], dtype=torch.int32, device="cuda")
+    A.attn_prefill(q, k, v, cu, out)
+    torch.cuda.synchronize()
+    last = lambda x: x[first:]
+    check(torch, last(out), last(q), last(k), last(v), 0, 500)
+    check(torch, last(out), last(q), last(k), last(v), 500, 700)

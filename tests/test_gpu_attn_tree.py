@@ -274,3 +274,26 @@ def test_calls_of_different_shapes_share_a_workspace():
                 compare(out, *reference(torch, q, kc, vc, table, contexts, None))
                 first.append(out)
     assert A.attn_tree_status(ws) == 0
+
+
+@pytest.mark.parametrize("page", [16, 5])
+def test_offsets_beyond_32_bits(page):
+    """A cache of some 10 GB each of keys and values, with pages from both of its ends; pages of no power of two go the other way."""
+    torch = _torch()
+    from fngine_b200 import attention as A
+    kv, dim, contexts = 8, 128, [700, 333]
+    n = 5 * 2 ** 30 // (page * kv * dim)
+    kc, vc = (torch.empty(n, page, kv, dim, dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    need = [-(-(c + 4) // page) for c in contexts]
+    table = torch.zeros(2, max(need), dtype=torch.int32, device="cuda")
+    table[0] = n - 1 - torch.arange(max(need), device="cuda", dtype=torch.int32)
+    table[1] = torch.arange(max(need), device="cuda", dtype=torch.int32) * 2 + n // 2
+    for x in (kc, vc):
+        for s in range(2):
+            x[table[s].long()] = torch.randn(max(need), page, kv, dim, generator=gen, device="cuda").bfloat16()
+    q = torch.randn(2, 4, 16, dim, generator=gen, device="cuda").bfloat16()
+    ws, out = A.attn_tree_workspace(2, 4, 16, kv, dim), torch.full_like(q, float("nan"))
+    A.attn_tree_decode(q, A.KvCache(kc, vc), table, torch.tensor(contexts, dtype=torch.int32, device="cuda"), out, ws)
+    torch.cuda.synchronize()
+    compare(out, *reference(torch, q, kc, vc, table, contexts, None))

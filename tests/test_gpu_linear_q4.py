@@ -162,3 +162,23 @@ def test_values_that_are_not_finite_stay_with_their_token():
     got = run(torch, "store_f32", codes, scales, z, x)
     keep = [0, 1, 3, 4, 6]
     assert torch.equal(got[keep], want[keep]) and not bool(torch.isfinite(got[2]).any()) and bool(torch.isnan(got[5]).all())
+
+
+def test_offsets_beyond_32_bits():
+    """Outputs some 4.5 GB behind the first one (sampled rows), and an output of the wrong size."""
+    torch = _torch()
+    from fngine_b200 import linear
+    n, k, T = 70000003, 128, 16
+    codes = torch.empty(n, k // 2, dtype=torch.uint8, device="cuda")
+    codes.view(-1)[: n * 64 // 8 * 8].view(torch.int64).random_(generator=torch.Generator(device="cuda").manual_seed(3))
+    scales = torch.exp2((torch.arange(n, device="cuda") % 7 - 6).float())[:, None].bfloat16()
+    x = torch.randint(-8, 9, (T, k), generator=torch.Generator(device="cuda").manual_seed(4), device="cuda").to(torch.bfloat16)
+    w, out = linear.Q4GroupWeight(codes, scales), torch.empty(T, n, device="cuda")
+    linear.linear_q4_decode(x, w, linear.store_f32(out))
+    torch.cuda.synchronize()
+    rows = torch.cat((torch.arange(0, n, 99991, device="cuda"), torch.arange(n - 300, n, device="cuda")))
+    want = x.double() @ weight64(torch, codes[rows], scales[rows], None, 128).T
+    assert torch.equal(out[:, rows].double(), want)
+    for wrong in (linear.store_f32(out[:15]), linear.store_bf16(torch.empty(T, n - 1, dtype=torch.bfloat16, device="cuda"))):
+        with pytest.raises(AssertionError):
+            linear.linear_q4_decode(x, w, wrong)
