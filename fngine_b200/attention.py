@@ -19,10 +19,10 @@ def _device():
 def _heads(x, tokens, heads, dim, dtype, dev, what):
     """(address, stride between tokens) of a [tokens][heads][head_dim] tensor whose heads lie side by side, on the current device
     (whose stream the call goes to)."""
+    s = x.stride()
     if x.shape != (tokens, heads, dim) or x.dtype is not dtype:
         raise ValueError("%s: [%d tokens][%d heads][%d] of %s" % (what, tokens, heads, dim, dtype))
-    s = x.stride()
-    if s[2] != 1 or (s[1] != dim and heads > 1):
+    if s[1] != dim and heads > 1 or s[2] != 1:
         raise ValueError("%s: [tokens][heads][head_dim] with the heads of a token side by side" % what)
     if x.get_device() != dev:
         raise ValueError("%s: not on the current device" % what)
@@ -47,18 +47,21 @@ class Rope:
         sections = [inv_freq.numel()] if sections is None else [int(s) for s in sections]
         assert 1 <= len(sections) <= 4 and sum(sections) == inv_freq.numel() and min(sections) >= 0
         self.inv_freq, self.axes = inv_freq, len(sections)
-        self._frozen = (inv_freq.data_ptr(), 2 * inv_freq.numel(), self.axes, (ctypes.c_int32 * 4)(*sections), int(bool(adjacent)))
+        self._frozen = bytes(L.RopeArgs(inv_freq.data_ptr(), None, 0, 2 * inv_freq.numel(), self.axes, (ctypes.c_int32 * 4)(*sections),
+                                        int(bool(adjacent)), 0))
 
     def c(self, positions, tokens, dev):
         """fb_rope for int32 positions [axes][tokens] (or [tokens], for one axis)."""
-        if positions.dim() == 1:
-            positions = positions.unsqueeze(0)
-        if positions.dtype is not torch.int32 or positions.shape != (self.axes, tokens) or (tokens > 1 and positions.stride(1) != 1):
+        shape, s = positions.shape, positions.stride()
+        if shape != (self.axes, tokens) and (self.axes > 1 or shape != (tokens,)) or positions.dtype is not torch.int32 or (tokens > 1 and s[-1] != 1):
             raise ValueError("positions: int32 [%d axes][%d tokens], contiguous along the tokens" % (self.axes, tokens))
         if positions.get_device() != dev:
             raise ValueError("positions: not on the current device")
-        f = self._frozen
-        return L.RopeArgs(f[0], positions.data_ptr(), positions.stride(0) if self.axes > 1 else tokens, f[1], f[2], f[3], f[4], 0)
+        r = L.RopeArgs.from_buffer_copy(self._frozen)
+        r.positions = positions.data_ptr()
+        if self.axes > 1:
+            r.axis_stride = s[0]
+        return r
 
 
 def qk_norm_rope(q, k, v, q_weight, k_weight, eps, rope, positions, q_out, k_out, v_out, slots=None):

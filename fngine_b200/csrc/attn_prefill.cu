@@ -13,6 +13,9 @@
 // rise above it by more than 2^8, which leaves every weight at most 256 and the sum in fp32 range. Normally that is
 // the first block alone, so O stays in tensor memory untouched.
 // Blocks are handed out longest first (causal: the last queries of a prompt have the most keys).
+// Bound by the exponentials (16 per clock and multiprocessor) and the tensor core, which are near level, and then by power: 8192
+// tokens of 48 heads of 128 in 616 us = 1.34 PFLOP/s in a burst, 724 under sustained load (a large library product: 1.62 and 1.35). Four prompts of 4000
+// tokens in all take 86: a block of 256 queries has some 7000 cycles of set-up, first scores and epilogue beside 2900 per key block.
 #include "attn_common.cuh"
 
 namespace fb {
@@ -157,88 +160,88 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
   // 256 threads x 208 and 128 x 88 registers are the 384 x 168 of the launch.
   if (warp >= 8) {
     regs_down<88>();
-  if (warp == 9) {
-    // ------------------------------------------------------------------ copies
-    if (lane == 0) {
-      for (int i = kEarly; i < 2 * blocks; ++i) {
-        if (i >= kStages && !bounded_wait(&bars->aborted, a.status, &bars->empty[i % kStages], uint32_t(i / kStages - 1) & 1)) break;
-        copy_block(i);
+    if (warp == 9) {
+      // ------------------------------------------------------------------ copies
+      if (lane == 0) {
+        for (int i = kEarly; i < 2 * blocks; ++i) {
+          if (i >= kStages && !bounded_wait(&bars->aborted, a.status, &bars->empty[i % kStages], uint32_t(i / kStages - 1) & 1)) break;
+          copy_block(i);
+        }
       }
-    }
-    __syncwarp();
-    // Rows of the next sequence in the last block: their weights are zero, but they need not be finite. (The barrier is in the phase of
-    // this last copy: its slot was free before.)
-    const int i = 2 * blocks - 1, slot = i % kStages, there = length - (blocks - 1) * kPfRows;
-    if (there < kPfRows && bounded_wait_warp(&bars->aborted, a.status, &bars->full[slot], uint32_t(i / kStages) & 1)) {
-      for (int c = lane; c < (kPfRows - there) * (D / 8); c += 32) {
-        const int row = there + c / (D / 8), chunk = c % (D / 8);
-        *reinterpret_cast<uint4*>(ring + slot * S::kTileBytes + (chunk / 8) * S::kHalf + row * 128 + (chunk % 8) * 16) = make_uint4(0, 0, 0, 0);
-      }
-      fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->cleared);
-    }
-  } else if (warp != 11) {
-    // ------------------------------------------------------------------ products: a thread for the scores, one for the outputs
-    // (The scores must not wait behind outputs whose weights are not there yet. One thread for all products: 4000 cycles per block of
-    // keys, one for each tile 3650.)
-    constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kPfRows >> 4) << 24);
-    constexpr uint32_t kIdescQk = kIdesc | (uint32_t(kPfRows >> 3) << 17);
-    constexpr uint32_t kIdescPv = kIdesc | (uint32_t(D >> 3) << 17) | (1u << 16);  // V runs along N
-    if (elect_one()) {
-      bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && bounded_spin(&bars->aborted, a.status, bar, parity); };
-      if (warp == 8) {
-        int held_by = -1, held_at = 0;  // whose scores S holds
-        for (int j = 0; j < blocks && ok; ++j) {
-          const int slot = (2 * j) % kStages;
-          wait(&bars->full[slot], uint32_t(2 * j / kStages) & 1);
-          const uint32_t kd = umma_desc_lo(smem_u32(ring + slot * S::kTileBytes), 1);
-#pragma unroll 1
-          for (int t = j < blocks0 ? 0 : 1; t < (j < blocks1 ? 2 : 1); ++t) {
-            if (j == 0) wait(&bars->q_full[t], 0);
-            if (held_by >= 0) wait(&bars->s_free[held_by], uint32_t(held_at) & 1);
-            if (!ok) break;
-            held_by = t;
-            held_at = j;
-            tc_fence_after();
-            const uint32_t qd = umma_desc_lo(smem_u32(q_tiles + t * S::kTileBytes), 1);
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t at = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
-              umma_ss<kIdescQk>(kS, qd + at, kd + at, k > 0);
-            }
-            umma_commit(&bars->s_full[t]);
-          }
-          if (ok) umma_commit(&bars->empty[slot]);
+      // Rows of the next sequence in the last block: their weights are zero, but they need not be finite. (The barrier is in the phase of
+      // this last copy: its slot was free before.)
+      const int i = 2 * blocks - 1, slot = i % kStages, there = length - (blocks - 1) * kPfRows;
+      if (there < kPfRows && bounded_wait_warp(&bars->aborted, a.status, &bars->full[slot], uint32_t(i / kStages) & 1)) {
+        for (int c = lane; c < (kPfRows - there) * (D / 8); c += 32) {
+          const int row = there + c / (D / 8), chunk = c % (D / 8);
+          *reinterpret_cast<uint4*>(ring + slot * S::kTileBytes + (chunk / 8) * S::kHalf + row * 128 + (chunk % 8) * 16) = make_uint4(0, 0, 0, 0);
         }
-      } else {
-        for (int j = 0; j < blocks && ok; ++j) {
-          const int slot = (2 * j + 1) % kStages;
-          wait(&bars->full[slot], uint32_t((2 * j + 1) / kStages) & 1);
-          if (length - j * kPfRows < kPfRows) wait(&bars->cleared, 0);
-          const uint32_t vd = umma_desc_lo(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
-#pragma unroll 1
-          for (int t = j < blocks0 ? 0 : 1; t < (j < blocks1 ? 2 : 1); ++t) {
-            wait(&bars->p_full[t], uint32_t(j) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t d = kO + 128 * t, p = kP + 64 * t;
-            umma_ts<kIdescPv>(d, p, vd, j > 0);
-#pragma unroll
-            for (int k = 1; k < kPfRows / 16; ++k) umma_ts<kIdescPv>(d, p + 8 * k, vd + k * (2048 >> 4), true);
-            umma_commit(&bars->o_done[t]);
-          }
-          if (ok) umma_commit(&bars->empty[slot]);
-        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->cleared);
       }
-      // Nothing issued here is still running when the tensor memory is given back.
-      umma_commit(&bars->drained);
+    } else if (warp != 11) {
+      // ------------------------------------------------------------------ products: a thread for the scores, one for the outputs
+      // (The scores must not wait behind outputs whose weights are not there yet. One thread for all products: 4000 cycles per block of
+      // keys, one for each tile 3650.)
+      constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kPfRows >> 4) << 24);
+      constexpr uint32_t kIdescQk = kIdesc | (uint32_t(kPfRows >> 3) << 17);
+      constexpr uint32_t kIdescPv = kIdesc | (uint32_t(D >> 3) << 17) | (1u << 16);  // V runs along N
+      if (elect_one()) {
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && bounded_spin(&bars->aborted, a.status, bar, parity); };
+        if (warp == 8) {
+          int held_by = -1, held_at = 0;  // whose scores S holds
+          for (int j = 0; j < blocks && ok; ++j) {
+            const int slot = (2 * j) % kStages;
+            wait(&bars->full[slot], uint32_t(2 * j / kStages) & 1);
+            const uint32_t kd = umma_desc_lo(smem_u32(ring + slot * S::kTileBytes), 1);
+#pragma unroll 1
+            for (int t = j < blocks0 ? 0 : 1; t < (j < blocks1 ? 2 : 1); ++t) {
+              if (j == 0) wait(&bars->q_full[t], 0);
+              if (held_by >= 0) wait(&bars->s_free[held_by], uint32_t(held_at) & 1);
+              if (!ok) break;
+              held_by = t;
+              held_at = j;
+              tc_fence_after();
+              const uint32_t qd = umma_desc_lo(smem_u32(q_tiles + t * S::kTileBytes), 1);
+#pragma unroll
+              for (int k = 0; k < D / 16; ++k) {
+                const uint32_t at = (k / 4) * (S::kHalf >> 4) + (k % 4) * 2;
+                umma_ss<kIdescQk>(kS, qd + at, kd + at, k > 0);
+              }
+              umma_commit(&bars->s_full[t]);
+            }
+            if (ok) umma_commit(&bars->empty[slot]);
+          }
+        } else {
+          for (int j = 0; j < blocks && ok; ++j) {
+            const int slot = (2 * j + 1) % kStages;
+            wait(&bars->full[slot], uint32_t((2 * j + 1) / kStages) & 1);
+            if (length - j * kPfRows < kPfRows) wait(&bars->cleared, 0);
+            const uint32_t vd = umma_desc_lo(smem_u32(ring + slot * S::kTileBytes), S::kHalf >> 4);
+#pragma unroll 1
+            for (int t = j < blocks0 ? 0 : 1; t < (j < blocks1 ? 2 : 1); ++t) {
+              wait(&bars->p_full[t], uint32_t(j) & 1);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t d = kO + 128 * t, p = kP + 64 * t;
+              umma_ts<kIdescPv>(d, p, vd, j > 0);
+#pragma unroll
+              for (int k = 1; k < kPfRows / 16; ++k) umma_ts<kIdescPv>(d, p + 8 * k, vd + k * (2048 >> 4), true);
+              umma_commit(&bars->o_done[t]);
+            }
+            if (ok) umma_commit(&bars->empty[slot]);
+          }
+        }
+        // Nothing issued here is still running when the tensor memory is given back.
+        umma_commit(&bars->drained);
+      }
+      __syncwarp();
+      for (uint32_t i = 0; i < (1u << 16) && !__all_sync(0xffffffffu, mbar_try_wait_hint(&bars->drained, 0)); ++i) {}
     }
-    __syncwarp();
-    for (uint32_t i = 0; i < (1u << 16) && !__all_sync(0xffffffffu, mbar_try_wait_hint(&bars->drained, 0)); ++i) {}
-  }
   } else {
     regs_up<208>();
     // ------------------------------------------------------------------ softmax

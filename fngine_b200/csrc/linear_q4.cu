@@ -13,7 +13,8 @@
 //   acc += s (P - z X),   P = sum of c x 2^-69 over the group, X = sum of x 2^-69.
 // Nothing is rounded but sums.
 //
-// The weights are the only large operand, so the kernel is built around their stream. A warp takes 16 MT rows (the M
+// Bound by the weights' bytes at few tokens and instruction issue at sixteen: 248320 x 2560 in 68 us for one token (4.8 TB/s), 99 for
+// sixteen. The weights are the only large operand, so the kernel is built around their stream. A warp takes 16 MT rows (the M
 // side of mma.sync m16n8k16, the tokens are the N side) through K in steps of 128: its own ring of cp.async stages in
 // shared memory, no barrier between warps. ldmatrix gives lane (g, t) of a quad eight consecutive codes of row g. The activations lie
 // in shared memory in the order (0 4 1 5 2 6 3 7) that the masked codes come in. S warps share

@@ -4,7 +4,7 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w                                   per head of q and k
 //   (a, b) -> (a cos p - b sin p, b cos p + a sin p),  p = position[axis(j)] * inv_freq[j]     frequency j's pair
 //
-// Bound by memory: every value is read once and written once. A block takes a token (or a share of its heads) after the other; D / 8
+// Bound by memory latency: every value is read once and written once, 8192 tokens of 48 heads of 128 in 54 us = 3.7 TB/s (a copy: 6.5). A block takes a token (or a share of its heads) after the other; D / 8
 // lanes hold a head, 16 bytes each, and the next token's values are on their way while this one's are worked on. The angles of a
 // token are made once per block: the product of position and frequency in 64 bits, reduced to a part of a turn there
 // (a position of a million leaves fp32 no more than four correct digits of the angle), the sine and cosine of the rest in fp32.
@@ -327,7 +327,7 @@ int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm
   int share = (passes + kQkRows - 1) / kQkRows;
   while (share < passes && int64_t(tokens) * share < sm_count()) share = 2 * share < passes ? 2 * share : passes;
   a.tokens = tokens;
-  // (tiles of four tokens where every block gets two of them: 8192 tokens of 48 heads 61 us in tiles of four or two, 67 one by one)
+  // (tiles of four tokens where every block gets two of them: 8192 tokens of 48 heads took 61 us in tiles of four or two, 67 one by one; since the pair arithmetic 54 in tiles of four)
   a.tile = int64_t(tokens) * share >= 2 * int64_t(kQkTile) * room ? kQkTile : 1;
   const int across = room / share > 0 ? room / share : 1;
   const int tiles = (tokens + a.tile - 1) / a.tile;

@@ -1,8 +1,9 @@
 /* fngine_b200 -- C ABI of the B200 (sm_100a) quantized-expert kernels.
  *
- * Every entry point replaces one function of the reference engine's kernel interface for the
+ * The entry points replace functions of the reference engine's kernel interface for the
  * routed-expert MoE path and the FP8-row dense projection; the comment above each declaration
- * names the reference declaration it stands in for (paths relative to the reference project).
+ * names the reference declaration it stands in for (paths relative to the reference project). Those without one (the attention
+ * branch of a layer, 4-bit projections, expert parallelism, probes) say so.
  * The reference exposes these as C++ free functions (namespace fngine::kernels); the translation unit
  * fngine_b200/binding/fngine_kernels_b200.cpp defines those C++ names on top of this ABI.
  *
@@ -467,10 +468,11 @@ int32_t fb_linear_fp8_decode(const void* x_bf16, int32_t tokens, const uint8_t* 
  *   out = epilogue(sum over groups of scale[n][g] * sum_{i in g} (code[n][i] - zero[n][g]) * x[t][i])
  * codes [n][k / 2]: value 2j of a row in the low four bits of byte j, value 2j + 1 in the high ones. scales [n][k / group],
  * fp32, bf16 or fp16. zeros [n][k / group]: one byte per group, of which the low four bits count, or NULL: eight everywhere.
- * group 32, 64 or 128; k % 128 == 0; any n (even for SwiGlu). codes, scales, zeros and x are 16-byte aligned.
- * x is bf16 [tokens][k], tokens 1..16; the epilogues are those of fb_linear_fp8. Products are exact, sums are fp32; every
- * output is written once, in an order of additions that the shape fixes: repeated calls are bitwise identical. `out` may not
- * lie in the memory of x. No workspace. */
+ * group 32, 64 or 128; k % 128 == 0; any n (even for SwiGlu) with n * k / group < 2^31. codes, scales, zeros and x are 16-byte aligned.
+ * x is bf16 [tokens][k], tokens 1..16; the epilogues are those of fb_linear_fp8. Products are exact, but activations below
+ * 2^-57 (below 2^7 in a token that has one of 2^63 or more) count as zero; sums are fp32; every output is
+ * written once, in an order of additions that the shape fixes: repeated calls are bitwise identical. `out` may not lie in the
+ * memory of x. No workspace. */
 typedef struct fb_q4_weight {
   const uint8_t* codes;
   const void* scales;
