@@ -4,17 +4,19 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w                                   per head of q and k
 //   (a, b) -> (a cos p - b sin p, b cos p + a sin p),  p = position[axis(j)] * inv_freq[j]     frequency j's pair
 //
-// Bound by memory latency: every value is read once and written once, 8192 tokens of 48 heads of 128 in 54 us = 3.7 TB/s (a copy: 6.5). A block takes a token (or a share of its heads) after the other; D / 8
-// lanes hold a head, 16 bytes each, and the next token's values are on their way while this one's are worked on. The angles of a
-// token are made once per block: the product of position and frequency in 64 bits, reduced to a part of a turn there
-// (a position of a million leaves fp32 no more than four correct digits of the angle), the sine and cosine of the rest in fp32.
+// Every value is read once and written once: 8192 tokens of 48 heads of 128 in 40 us = 5.1 TB/s (a copy: 6.5), 4093 of 64 heads in 30. The
+// issue slots are the next limit (at 54 us, 77 % of them): so a thread takes one head of a tile's tokens after the other, with its
+// addresses made once for the tile, and the next step's 16-byte pieces are on their way while this one's are worked on; D / 8 lanes hold a
+// head. (A token's heads one after the other: 54 us; its values by cp.async two or three tokens ahead: 55 to 63; each block's tokens side by
+// side in memory instead of a tile of every round: 56.) The angles of a tile are made once per block: the product of position and
+// frequency in 64 bits, reduced to a part of a turn there (a position of a million leaves fp32 no more than four correct digits of the
+// angle), the sine and cosine of the rest in fp32.
 #include "attn_common.cuh"
 
 namespace fb {
 namespace {
 
 constexpr int kQkThreads = 256;
-constexpr int kQkRows = 4;    // heads a thread works on at a time, and as many are in flight behind them
 constexpr int kQkBlocks = 3;  // per multiprocessor
 constexpr int kQkTile = 4;    // tokens whose angles are made together
 
@@ -32,7 +34,7 @@ struct QkArgs {
   float eps;
   int weight_dtype, heads, kv_heads, half, adjacent;
   int rows;              // heads of all tensors
-  int tokens, tile;
+  int tiles, shortest, longer;  // tiles of `shortest` tokens, the first `longer` of them with one more
   int first[3];          // first row of q, k, v
   int section_end[4];
 };
@@ -83,52 +85,57 @@ struct QkFactors {
 template <class T, int D>
 __global__ void __launch_bounds__(kQkThreads, kQkBlocks) qk_norm_rope_kernel(const QkArgs a) {
   constexpr int kLanes = D / 8;                    // lanes of a head
-  constexpr int kPerPass = kQkThreads / kLanes;    // heads of a block per row of a thread
+  constexpr int kPerPass = kQkThreads / kLanes;    // heads of a block at a time
   constexpr int kAngles = (kQkTile * (D / 2) + kQkThreads - 1) / kQkThreads;  // per thread and tile
   __shared__ QkFactors<D> factors[2][kQkTile][2];  // of q and k; the next tile's are made while this one's are in use
   __shared__ float weights[2][D];
+  __shared__ int64_t slots[2][kQkTile];
   pdl_wait_prior();
   pdl_launch_dependents();
-  const int l = threadIdx.x % kLanes, e0 = 8 * l, slot_row = threadIdx.x / kLanes;
-  const int tile = a.tile;
-  // This thread's rows, the same of every token. Every thread stays for the shuffles; a row behind the last one is not loaded and not
-  // stored.
-  int kind[kQkRows], off[kQkRows];  // 0 q, 1 k, 2 v, 3 none; values from the token's first
-  uint32_t used = 0, turns = 0;     // bit i: the block has rows there; this warp has rows of q or k there
-#pragma unroll
-  for (int i = 0; i < kQkRows; ++i) {
-    const int row = (i * gridDim.y + blockIdx.y) * kPerPass + slot_row;
-    kind[i] = row >= a.rows ? 3 : row >= a.first[2] ? 2 : row >= a.first[1] ? 1 : 0;
-    off[i] = (row - (kind[i] == 0 ? a.first[0] : kind[i] == 1 ? a.first[1] : a.first[2])) * D + e0;
-    if ((i * int(gridDim.y) + int(blockIdx.y)) * kPerPass < a.rows) used |= 1u << i;
-    if (__any_sync(0xffffffffu, kind[i] < 2)) turns |= 1u << i;
-  }
-  auto load = [&](int64_t token, uint4 (&raw)[kQkRows]) {
-    const T* q = static_cast<const T*>(a.in[0]) + token * a.in_stride[0];
-    const T* k = static_cast<const T*>(a.in[1]) + token * a.in_stride[1];
-    const T* v = static_cast<const T*>(a.in[2]) + token * a.in_stride[2];
-#pragma unroll
-    for (int i = 0; i < kQkRows; ++i)
-      raw[i] = kind[i] < 3 ? *reinterpret_cast<const uint4*>((kind[i] == 0 ? q : kind[i] == 1 ? k : v) + off[i]) : make_uint4(0, 0, 0, 0);
+  const int l = threadIdx.x % kLanes, e0 = 8 * l, mine = threadIdx.x / kLanes, lane = threadIdx.x & 31;
+  const int passes = (a.rows + kPerPass - 1) / kPerPass;
+  // Every gridDim.x-th tile; the first `longer` tiles have one token more than the others.
+  int at = blockIdx.x, token0 = at * a.shortest + (at < a.longer ? at : a.longer), here = a.shortest + (at < a.longer);
+  // A step: one head (of q, k or v: kind 0, 1, 2, or none: 3) of the tile's tokens, one after the other.
+  auto row_of = [&](int pass, int& kind, int& off) {
+    const int row = pass * kPerPass + mine;
+    kind = row >= a.rows ? 3 : row >= a.first[2] ? 2 : row >= a.first[1] ? 1 : 0;
+    off = (row - (kind == 0 ? a.first[0] : kind == 1 ? a.first[1] : a.first[2])) * D + e0;
   };
-  int64_t token0 = int64_t(blockIdx.x) * tile;
-  uint4 raw[kQkRows];
-  load(token0, raw);
-  int64_t next_slot = a.slots ? a.slots[token0] : 0;
-  // Thread and index i take an angle of the tile: (token, frequency), the positions asked for a tile ahead.
-  int position[kAngles];
-  auto ask = [&](int64_t first) {
+  auto load = [&](int token, int there, int kind, int off, uint4 (&raw)[kQkTile]) {
+    const int64_t stride = kind == 0 ? a.in_stride[0] : kind == 1 ? a.in_stride[1] : a.in_stride[2];
+    const T* from = static_cast<const T*>(kind == 0 ? a.in[0] : kind == 1 ? a.in[1] : a.in[2]) + token * stride + off;
 #pragma unroll
-    for (int i = 0; i < kAngles; ++i) {
-      const int id = threadIdx.x + i * kQkThreads, t = a.half ? id / a.half : tile, f = id - t * a.half;
-      position[i] = 0;
-      if (t < tile && first + t < a.tokens) {
-        const int axis = (f >= a.section_end[0]) + (f >= a.section_end[1]) + (f >= a.section_end[2]);
-        position[i] = a.positions[axis * a.axis_stride + first + t];
-      }
+    for (int t = 0; t < kQkTile; ++t) {
+      if (kind < 3 && t < there) raw[t] = *reinterpret_cast<const uint4*>(from);
+      from += stride;
     }
   };
-  ask(token0);
+  uint4 raw[kQkTile] = {};
+  int kind, off;
+  row_of(blockIdx.y, kind, off);
+  load(token0, here, kind, off, raw);
+  // Thread and index i make an angle of the tile, (token, frequency), from positions that are asked for a tile ahead; the first threads
+  // bring the slots.
+  int angle_t[kAngles], angle_f[kAngles], position[kAngles];
+  int64_t slot = 0;
+  double turns_of[kAngles];  // per position
+  auto ask = [&](int first, int there) {
+#pragma unroll
+    for (int i = 0; i < kAngles; ++i) {
+      const int f = angle_f[i], axis = (f >= a.section_end[0]) + (f >= a.section_end[1]) + (f >= a.section_end[2]);
+      position[i] = angle_t[i] < there ? a.positions[axis * a.axis_stride + first + angle_t[i]] : 0;
+    }
+    if (a.slots && int(threadIdx.x) < there) slot = a.slots[first + threadIdx.x];
+  };
+#pragma unroll
+  for (int i = 0; i < kAngles; ++i) {
+    const int id = threadIdx.x + i * kQkThreads;
+    angle_t[i] = a.half ? id / a.half : kQkTile;
+    angle_f[i] = a.half ? id % a.half : 0;
+    turns_of[i] = angle_t[i] < kQkTile ? double(a.inv_freq[angle_f[i]]) * 0.15915494309189533577 : 0.;  // 1 / (2 pi)
+  }
+  ask(token0, here);
   for (int e = threadIdx.x; e < 2 * D; e += kQkThreads) {
     const int w = e / D;
     weights[w][e % D] = a.weight[w] ? weight_at(a.weight[w], a.weight_dtype, e % D) : 1.f;
@@ -138,52 +145,52 @@ __global__ void __launch_bounds__(kQkThreads, kQkBlocks) qk_norm_rope_kernel(con
     const int e = id % D, w = id / D % 2, t = id / (2 * D) % kQkTile;
     if (e >= 2 * a.half) factors[id / (2 * D * kQkTile)][t][w].set(e, weights[w][e], 0.f);
   }
-  const bool normed[2] = {a.weight[0] != nullptr, a.weight[1] != nullptr};
   const bool turned = e0 < 2 * a.half;
   // The lane that holds the partners of an element pair (i, i + rot / 2), in this head's lanes.
-  const int lane = threadIdx.x & 31;
   const int partner = !turned || a.adjacent ? lane : e0 < a.half ? lane + a.half / 8 : lane - a.half / 8;
-  int buffer = 0;
-  for (; token0 < a.tokens; token0 += int64_t(gridDim.x) * tile, buffer ^= 1) {
+  for (int buffer = 0; here > 0; buffer ^= 1) {
 #pragma unroll
     for (int i = 0; i < kAngles; ++i) {
-      const int id = threadIdx.x + i * kQkThreads, t = a.half ? id / a.half : tile, f = id - t * a.half;
-      if (t < tile) {
-        const double turns = double(position[i]) * (double(a.inv_freq[f]) * 0.15915494309189533577);  // 1 / (2 pi)
+      if (angle_t[i] < here) {
+        const double turns = double(position[i]) * turns_of[i];
         float s, c;
         sincospif(2.f * float(turns - rint(turns)), &s, &c);
-        const int lo = a.adjacent ? 2 * f : f, hi = a.adjacent ? 2 * f + 1 : f + a.half;
+        const int f = angle_f[i], lo = a.adjacent ? 2 * f : f, hi = a.adjacent ? 2 * f + 1 : f + a.half;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
           const float wl = weights[w][lo], wh = weights[w][hi];
-          factors[buffer][t][w].set(lo, wl * c, -wh * s);
-          factors[buffer][t][w].set(hi, wh * c, wl * s);
+          factors[buffer][angle_t[i]][w].set(lo, wl * c, -wh * s);
+          factors[buffer][angle_t[i]][w].set(hi, wh * c, wl * s);
         }
       }
     }
-    ask(token0 + int64_t(gridDim.x) * tile);
+    if (threadIdx.x < kQkTile) slots[buffer][threadIdx.x] = slot;
+    at += gridDim.x;
+    const int next_here = at < a.tiles ? a.shortest + (at < a.longer) : 0;
+    const int next0 = next_here ? at * a.shortest + (at < a.longer ? at : a.longer) : 0;
+    ask(next0, next_here);
     __syncthreads();
-    const int here = a.tokens - token0 < tile ? int(a.tokens - token0) : tile;
-    for (int t = 0; t < here; ++t) {
-      const int64_t token = token0 + t, next = t + 1 < here ? token + 1 : token0 + int64_t(gridDim.x) * tile;
-      uint4 next_raw[kQkRows];
-      const int64_t slot = a.slots ? next_slot : token;
-      const bool kept = !a.slots || (slot >= 0 && slot < a.n_slots);
-      if (next < a.tokens) {
-        load(next, next_raw);
-        if (a.slots) next_slot = a.slots[next];
-      }
-      T* q = static_cast<T*>(a.out[0]) + token * a.out_stride[0];
-      T* k = static_cast<T*>(a.out[1]) + slot * a.out_stride[1];
-      T* v = static_cast<T*>(a.out[2]) + slot * a.out_stride[2];
+    for (int pass = blockIdx.y; pass < passes; pass += gridDim.y) {
+      // The next step's values are on their way while this one's are worked on.
+      uint4 next_raw[kQkTile] = {};
+      int next_kind, next_off;
+      const bool last = pass + int(gridDim.y) >= passes;
+      row_of(last ? int(blockIdx.y) : pass + int(gridDim.y), next_kind, next_off);
+      load(last ? next0 : token0, last ? next_here : here, next_kind, next_off, next_raw);
+      // Every thread stays for the shuffles; a head behind the last one is not stored.
+      const bool works = __any_sync(0xffffffffu, kind < 2), normed = (kind == 1 ? a.weight[1] : a.weight[0]) != nullptr;
+      const bool slotted = a.slots && kind != 0;
+      const int64_t stride = kind == 0 ? a.out_stride[0] : kind == 1 ? a.out_stride[1] : a.out_stride[2];
+      T* to = static_cast<T*>(kind == 0 ? a.out[0] : kind == 1 ? a.out[1] : a.out[2]) + off;
+      if (!slotted) to += token0 * stride;
 #pragma unroll
-      for (int i = 0; i < kQkRows; ++i) {
-        if (!((used >> i) & 1)) break;
-        uint4 result = raw[i];
-        if ((turns >> i) & 1) {
-          const QkFactors<D>& f = factors[buffer][t][kind[i] == 1];
+      for (int t = 0; t < kQkTile; ++t) {
+        if (t >= here) break;
+        uint4 result = raw[t];
+        if (works) {
+          const QkFactors<D>& f = factors[buffer][t][kind == 1];
           uint64_t x[4], p[4];
-          unpack8<T>(raw[i], x);
+          unpack8<T>(raw[t], x);
           uint64_t sum2 = fma2(x[1], x[1], fma2(x[0], x[0], 0));
           sum2 = add2(sum2, fma2(x[3], x[3], fma2(x[2], x[2], 0)));
           float sum, high;
@@ -191,7 +198,7 @@ __global__ void __launch_bounds__(kQkThreads, kQkBlocks) qk_norm_rope_kernel(con
           sum += high;
 #pragma unroll
           for (int m = kLanes / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-          const float r = normed[kind[i] == 1] ? rsqrtf(fmaf(sum, 1.f / D, a.eps)) : 1.f;
+          const float r = normed ? rsqrtf(fmaf(sum, 1.f / D, a.eps)) : 1.f;
           if (a.adjacent) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -201,10 +208,10 @@ __global__ void __launch_bounds__(kQkThreads, kQkBlocks) qk_norm_rope_kernel(con
             }
           } else {
             uint4 other;
-            other.x = __shfl_sync(0xffffffffu, raw[i].x, partner);
-            other.y = __shfl_sync(0xffffffffu, raw[i].y, partner);
-            other.z = __shfl_sync(0xffffffffu, raw[i].z, partner);
-            other.w = __shfl_sync(0xffffffffu, raw[i].w, partner);
+            other.x = __shfl_sync(0xffffffffu, raw[t].x, partner);
+            other.y = __shfl_sync(0xffffffffu, raw[t].y, partner);
+            other.z = __shfl_sync(0xffffffffu, raw[t].z, partner);
+            other.w = __shfl_sync(0xffffffffu, raw[t].w, partner);
             unpack8<T>(other, p);
           }
           const ulonglong2 o0 = f.piece[0][l], o1 = f.piece[1][l];
@@ -219,14 +226,23 @@ __global__ void __launch_bounds__(kQkThreads, kQkBlocks) qk_norm_rope_kernel(con
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[e] = fma2(y[e], rr, 0);
-          if (kind[i] < 2) result = pack8<T>(y);
+          if (kind < 2) result = pack8<T>(y);
         }
-        if (kind[i] == 0 || (kind[i] < 3 && kept))
-          *reinterpret_cast<uint4*>((kind[i] == 0 ? q : kind[i] == 1 ? k : v) + off[i]) = result;
+        if (slotted) {
+          const int64_t row = slots[buffer][t];
+          if (kind < 3 && row >= 0 && row < a.n_slots) *reinterpret_cast<uint4*>(to + row * stride) = result;
+        } else {
+          if (kind < 3) *reinterpret_cast<uint4*>(to) = result;
+          to += stride;
+        }
       }
 #pragma unroll
-      for (int i = 0; i < kQkRows; ++i) raw[i] = next_raw[i];
+      for (int t = 0; t < kQkTile; ++t) raw[t] = next_raw[t];
+      kind = next_kind;
+      off = next_off;
     }
+    token0 = next0;
+    here = next_here;
   }
 }
 
@@ -322,16 +338,19 @@ int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm
   if (a.slots && a.n_slots <= 0) return invalid("qk_norm_rope: slots without n_slots");
   a.heads = in->heads;
   a.kv_heads = in->kv_heads;
-  // Up to kQkRows heads per thread, the others to more blocks; few tokens share their heads among blocks, many go to a block in tiles.
+  // Tiles of up to kQkTile tokens where every block gets a step of one; the passes over a token's heads go to as many blocks as it takes to
+  // give each multiprocessor's blocks two tiles (the angles are made once more in each). Tiles as even as they come: all blocks end together.
   const int per_pass = kQkThreads / (dim / 8), passes = (a.rows + per_pass - 1) / per_pass, room = kQkBlocks * sm_count();
-  int share = (passes + kQkRows - 1) / kQkRows;
-  while (share < passes && int64_t(tokens) * share < sm_count()) share = 2 * share < passes ? 2 * share : passes;
-  a.tokens = tokens;
-  // (tiles of four tokens where every block gets two of them: 8192 tokens of 48 heads took 61 us in tiles of four or two, 67 one by one; since the pair arithmetic 54 in tiles of four)
-  a.tile = int64_t(tokens) * share >= 2 * int64_t(kQkTile) * room ? kQkTile : 1;
-  const int across = room / share > 0 ? room / share : 1;
-  const int tiles = (tokens + a.tile - 1) / a.tile;
-  const dim3 grid(unsigned(tiles < across ? tiles : across), unsigned(share));
+  const int longest = (tokens + kQkTile - 1LL) / kQkTile * passes >= room ? kQkTile : 1;
+  const int least = int((tokens + longest - 1LL) / longest);
+  int share = 1;
+  while (share < passes && int64_t(least) * share < 2 * room) share = 2 * share < passes ? 2 * share : passes;
+  const int across = room / share > 0 ? room / share : 1, grid_x = least < across ? least : across;
+  const int64_t even = (least + grid_x - 1LL) / grid_x * grid_x;  // as many for each block
+  a.tiles = int(even < tokens ? even : tokens);
+  a.shortest = tokens / a.tiles;
+  a.longer = tokens % a.tiles;
+  const dim3 grid{unsigned(grid_x), unsigned(share)};
   const cudaError_t e = in->dtype == FB_DT_BF16 ? launch_qk<__nv_bfloat16>(a, dim, grid, as_stream(stream))
                                                 : launch_qk<__half>(a, dim, grid, as_stream(stream));
   const int32_t st = check_launch("qk_norm_rope");
