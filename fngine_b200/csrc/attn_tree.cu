@@ -3,7 +3,7 @@
 //   out[i] = sum_j softmax_j(scale q_i . k_j) v_j over the keys j that token i sees: all ctx keys of the context, and of the
 //   drafted tokens, whose keys follow the context's in the cache, those in its mask.
 //
-// Bound by the cache's bytes and, close behind, the softmax: each key and value is read once for all rows (tokens x query heads of a group) of a key head. The
+// Bound by the cache's bytes: each key and value is read once for all rows (tokens x query heads of a group) of a key head. The
 // rows, up to 128, are the lanes of the products' results in tensor memory, whether they are 4 or 128: a block of 128 keys costs the
 // tensor core 1024 cycles at head_dim 128 and a multiprocessor's share of the memory bandwidth 2800. (Products by mma.sync with
 // fragments in registers, 16 to 128 rows, were bound by the latencies of eight warps: 446 us for 32 sequences of up to 16384 keys
@@ -11,10 +11,12 @@
 //   S = Q K^T   both operands in shared memory, fp32 S in tensor memory
 //   P = 2^(c S - c m) over S in the type of v, by a thread per row; only warps that hold rows read S
 //   O += P V    fp32 in tensor memory; multiplied only when a maximum rises by more than 2^8 above the one in use
-// 32 sequences of up to 16384 keys, four tokens, 32 heads of 128: 300 us = 5.5 TB/s in a burst (274 without the softmax, 287 without
-// the copies), 356 under sustained load; eight of 4096 keys, sixteen tokens, 48 heads: 41 us; one token and 1003 keys: 12.
-// A block of keys keeps its softmax warps for some 2300 cycles and its products for a thousand more, longer than its bytes take. So even and odd blocks are two streams with
+// A block of keys keeps its softmax warps and its products longer than its bytes take. So even and odd blocks are two streams with
 // warps, S, O, maxima and sums of their own, which meet where a segment ends: each O is read there by both, half of the columns each.
+// And a warp reaches only its 32 lanes of tensor memory: up to 32 rows lie there four times (up to 64 twice), and each copy takes a part of a
+// block's keys, with zeros for weights of the others, and a maximum, a sum and an O of its own until the segment ends.
+// 32 sequences of up to 16384 keys, four tokens, 32 heads of 128: 274 us = 6.1 TB/s (302 without the copies of rows; head_dim 64 208
+// and 244); eight of 4096 keys, sixteen tokens, 48 heads: 42 us; one token and 1003 keys: 12.
 // Blocks of context keys come by TMA, a box per run of slots that a page holds (up to 128, the power of two in the page size). The
 // block where the context ends, and all blocks where that power is below kTreeMinBox, come by cp.async, 16 bytes a thread: any slots, and
 // what is not to be read is written as zeros. (cp.async alone moves 4.4 TB/s; TMA gathers of four cache rows took 41 ns each per
@@ -27,7 +29,7 @@
 namespace fb {
 namespace {
 
-constexpr int kTreeThreads = 448;        // two streams of four softmax warps, four that copy, one each that issues scores and outputs
+constexpr int kTreeThreads = 512;        // two streams of four softmax warps, four that copy, one each that issues scores and outputs, two idle
 constexpr int kTreeWarps = kTreeThreads / 32;
 constexpr int kTreeRows = 128;           // rows of a tile
 constexpr int kTreeKeys = 128;           // keys of a block
@@ -57,12 +59,14 @@ struct TreeMaps {
   CUtensorMap q, k, v;
 };
 
-template <int D>
+// C copies of a tile's rows in 128 / C lanes each.
+template <int D, int C>
 struct TreeShape {
   static constexpr int kTileBytes = kTreeKeys * D * 2;
   static constexpr int kHalf = kTreeKeys * 128;  // a tile is D / 64 parts of 128 rows x 128 bytes
-  static constexpr int kStages = D == 128 ? 5 : 10;
-  static constexpr int kSmem = (2 + kStages) * kTileBytes + 3072;
+  static constexpr int kStages = D == 64 ? 10 : C == 1 ? 5 : 4;
+  static constexpr int kMeet = C == 1 ? 0 : 2 * kTreeRows * 32 * 4;  // where copies of rows meet: 32 columns for each stream's warps
+  static constexpr int kSmem = (2 + kStages) * kTileBytes + kMeet + 3072;
   static constexpr int kSlot = (D + 2) * kTreeRows;  // floats of a partial result
 };
 
@@ -83,7 +87,7 @@ struct TreeBars {
   int last_block;
 };
 static_assert(sizeof(TreeBars) <= 3072, "room behind the ring");
-static_assert(TreeShape<128>::kSmem <= 227 * 1024, "all of a multiprocessor's shared memory");
+static_assert(TreeShape<128, 1>::kSmem <= 227 * 1024, "all of a multiprocessor's shared memory");
 
 // Walks through the key blocks of the segments in their order.
 struct TreeCursor {
@@ -91,14 +95,15 @@ struct TreeCursor {
   int tiles, ctx, length;  // of the sequence
 };
 
-template <class T, int D>
+template <class T, int D, int C>
 __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a, const __grid_constant__ TreeMaps maps) {
-  using S = TreeShape<D>;
+  using S = TreeShape<D, C>;
   constexpr int kStages = S::kStages, kParts = D / 64;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* q_tiles = smem;
   uint8_t* ring = smem + 2 * S::kTileBytes;
-  TreeBars* bars = reinterpret_cast<TreeBars*>(ring + kStages * S::kTileBytes);
+  float4* meet = reinterpret_cast<float4*>(ring + kStages * S::kTileBytes);  // [stream][8 pieces of 4 columns][128 rows]
+  TreeBars* bars = reinterpret_cast<TreeBars*>(ring + kStages * S::kTileBytes + S::kMeet);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int parts = a.kv_heads * a.row_tiles;
   const int64_t room = a.table_stride * a.page_size;  // keys that the table can hold
@@ -234,7 +239,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
   if (bars->tmem != 0 && tid == 0) atomicMax(a.status, uint32_t(FB_STATUS_BAD_WORK));
   constexpr uint32_t kS = 0, kO = 256;  // stream t: S in columns 128 t, O in 256 + 128 t
 
+  // 256 threads x 168 and 256 x 88 registers are the 512 x 128 of the launch.
   if (warp >= 8 && warp < 12) {
+    regs_down<88>();
     // ------------------------------------------------------------------ copies
     const int me = tid - 256;  // looks up key `me` of a block
     uint64_t seen = 0;         // drafted tokens that some token of the sequence sees
@@ -270,9 +277,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
         if (segment >= 2) ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->q_empty[b], uint32_t(segment / 2 - 1) & 1);
         if (ok && me == 0) {
           const int token = now.seq * a.drafted + (now.part % a.row_tiles) * a.tile_tokens;
-          mbar_expect_tx(&bars->q_full[b], uint32_t(a.tile_tokens * a.group) * D * 2);
-          for (int p = 0; p < kParts; ++p)
-            tma_load_3d(smem_u32(q_tiles + b * S::kTileBytes) + p * S::kHalf, &maps.q, p * 64, head * a.group, token, &bars->q_full[b]);
+          mbar_expect_tx(&bars->q_full[b], uint32_t(C * a.tile_tokens * a.group) * D * 2);
+          for (int c = 0; c < C; ++c)
+            for (int p = 0; p < kParts; ++p)
+              tma_load_3d(smem_u32(q_tiles + b * S::kTileBytes) + p * S::kHalf + c * (kTreeRows / C) * 128, &maps.q, p * 64, head * a.group, token,
+                          &bars->q_full[b]);
           bars->q_issued = segment + 1;
         }
         ++segment;
@@ -329,12 +338,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp >= 12) {
+    regs_down<88>();
     // ------------------------------------------------------------------ products: a thread for the scores, one for the outputs
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t kIdesc = (1u << 4) | (kType << 7) | (kType << 10) | (uint32_t(kTreeRows >> 4) << 24);
     constexpr uint32_t kIdescQk = kIdesc | (uint32_t(kTreeKeys >> 3) << 17);
     constexpr uint32_t kIdescPv = kIdesc | (uint32_t(D >> 3) << 17) | (1u << 16);  // V runs along N
-    if (elect_one()) {
+    if (warp < 14 && elect_one()) {
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && bounded_spin(&bars->aborted, a.status, bar, parity); };
       int segment = 0, piece = 0;  // piece: first block of the segment in this block's share
@@ -382,11 +392,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
     __syncwarp();
     for (uint32_t n = 0; n < (1u << 16) && !__all_sync(0xffffffffu, mbar_try_wait_hint(&bars->drained, 0)); ++n) {}
   } else {
+    regs_up<168>();
     // ------------------------------------------------------------------ softmax: thread = row, warps 4 t .. 4 t + 3 take stream t
     const int t = warp >> 2, row = tid & (kTreeRows - 1), lane_row = 32 * (warp & 3);
     const uint32_t lanes = uint32_t(lane_row) << 16;
     const uint32_t s_at = lanes + kS + 128 * t, o_at = lanes + kO + 128 * t;
     const uint64_t scale = pair_of(a.scale_log2, a.scale_log2);
+    // Copy c of the rows has its keys: the c-th part of a block's, in steps of 32.
+    constexpr int span = kTreeRows / C, kSteps = 4 / C;
+    const int copy = row / span, place = row % span, step0 = copy * kSteps;
     bool ok = true, fresh = true;
     float top = -INFINITY, sum = 0.f;
     int rows = 0, head0 = 0;
@@ -406,15 +420,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
         head0 = (now.part / a.row_tiles) * a.group;
         token0 = int64_t(now.seq) * a.drafted + first;
         sees = 0;
-        const int token = row / a.group;
-        if (row < rows) sees = a.mask ? a.mask[token0 + token] : first + token == 63 ? ~0ull : (2ull << (first + token)) - 1;
+        const int token = place / a.group;
+        if (place < rows) sees = a.mask ? a.mask[token0 + token] : first + token == 63 ? ~0ull : (2ull << (first + token)) - 1;
         const int there = now.length - now.ctx;  // drafted tokens that the table has room for
         if (there < 64) sees &= (1ull << there) - 1;
       }
       const bool segment_ends = now.tile + 1 == now.tiles, piece_ends = segment_ends || it + 1 == n_tiles;
       if ((it & 1) == t) {
         ok = ok && bounded_wait_warp(&bars->aborted, a.status, &bars->s_full[t], uint32_t(it >> 1) & 1);
-        if (ok && lane_row < rows) {
+        if (ok && lane_row % span < rows) {
           tc_fence_after();
           // (The scores are read twice, once for the maximum and once for the weights: 130 cycles of 3300, for 64 registers.)
           const int off = now.ctx - now.tile * kTreeKeys;  // first column behind the context
@@ -432,24 +446,26 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
           // Loops of two steps of 32 columns, the next on their way: short enough to stay in the instruction cache, where all four steps
           // in a row ran at four cycles per instruction (drafts of 16: 49 us, now 41). What one turn hands to the next has landed.
           float s0[32], s1[32], latest = -INFINITY;
-          tmem_ld32(s_at, s0);
+          tmem_ld32(s_at + 32 * step0, s0);
           tmem_ld_wait();
           tmem_landed(s0);
 #pragma unroll 1
-          for (int i = 0; i < 4; i += 2) {
-            tmem_ld32(s_at + 32 * (i + 1), s1);
+          for (int i = step0; i < step0 + kSteps; i += 2) {
+            if (kSteps > 1) tmem_ld32(s_at + 32 * (i + 1), s1);
             unseen(i, s0);
             latest = scores_max(s0, latest);
-            tmem_ld_wait();
-            tmem_landed(s1);
-            tmem_ld32(s_at + 32 * ((i + 2) & 3), s0);  // (at the end the first columns again: the weights begin with them)
-            unseen(i + 1, s1);
-            latest = scores_max(s1, latest);
-            tmem_ld_wait();
-            tmem_landed(s0);
+            if (kSteps > 1) {
+              tmem_ld_wait();
+              tmem_landed(s1);
+              tmem_ld32(s_at + 32 * (kSteps > 2 ? (i + 2) & 3 : step0), s0);  // (at the end the first columns again: the weights begin with them)
+              unseen(i + 1, s1);
+              latest = scores_max(s1, latest);
+              tmem_ld_wait();
+              tmem_landed(s0);
+            }
           }
           // (no for a row that has seen nothing yet; rows behind the last one are nobody's and decide nothing)
-          const bool rises = row < rows && (latest - top) * a.scale_log2 > kTreeSlack;
+          const bool rises = place < rows && (latest - top) * a.scale_log2 > kTreeSlack;
           if (__any_sync(0xffffffffu, rises)) {
             const float up = fmaxf(latest, top);
             const float fade = up == -INFINITY ? 1.f : exp2_approx((top - up) * a.scale_log2);
@@ -474,20 +490,33 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
           const uint64_t minus = pair_of(-base, -base);
           uint64_t part[2] = {0, 0};
 #pragma unroll 1
-          for (int i = 0; i < 4; i += 2) {
+          for (int i = step0; i < step0 + kSteps; i += 2) {
             uint32_t p[16];
-            tmem_ld32(s_at + 32 * (i + 1), s1);
-            unseen(i, s0);
+            if (kSteps > 1) tmem_ld32(s_at + 32 * (i + 1), s1);
+            if (kSteps > 1) unseen(i, s0);
             scores_exp<T, false>(s0, scale, minus, p, part);
-            tmem_st16(s_at + 16 * i, p);  // (over scores that have been read)
-            tmem_ld_wait();
-            tmem_landed(s1);
-            tmem_ld32(s_at + 64, s0);  // (of no use in the second turn, whose weights begin at column 32)
-            unseen(i + 1, s1);
-            scores_exp<T, false>(s1, scale, minus, p, part);
-            tmem_st16(s_at + 16 * (i + 1), p);
-            tmem_ld_wait();
-            tmem_landed(s0);
+            if (kSteps > 1) {
+              tmem_ld_wait();
+              tmem_landed(s1);
+              tmem_st16(s_at + 16 * i, p);  // (over scores that have been read)
+              if (kSteps > 2) tmem_ld32(s_at + 64, s0);  // (of no use in the second turn, whose weights begin at column 32)
+              unseen(i + 1, s1);
+              scores_exp<T, false>(s1, scale, minus, p, part);
+              tmem_st16(s_at + 16 * (i + 1), p);
+              if (kSteps > 2) {
+                tmem_ld_wait();
+                tmem_landed(s0);
+              }
+            } else {
+              tmem_st16(s_at + 16 * i, p);
+            }
+          }
+          if (C > 1) {  // the other copies' keys
+            const uint32_t none[16] = {};
+#pragma unroll
+            for (int i = 1; i < C; ++i)
+#pragma unroll
+              for (int e = 0; e < kSteps; ++e) tmem_st16(s_at + 16 * (((copy + i) % C) * kSteps + e), none);
           }
           sum += pairs_sum(part);
           tmem_st_wait();
@@ -509,53 +538,123 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
         const bool whole = piece_begin == segment_begin && segment_ends;
         // A block has at most two pieces that are not whole: one that begins with its segment, one that does not.
         float* mine = a.partial + (2 * size_t(blockIdx.x) + (piece_begin == segment_begin ? 1 : 0)) * S::kSlot;
-        if (ok && lane_row < rows) {
-          const float m0 = bars->tops[0][row], m1 = bars->tops[1][row], up = fmaxf(m0, m1), zero = up == -INFINITY ? 0.f : up;
-          float f[2] = {exp2_approx((m0 - zero) * a.scale_log2), exp2_approx((m1 - zero) * a.scale_log2)};
-          const float l = bars->sum_of[0][row] * f[0] + bars->sum_of[1][row] * f[1];
-          if (whole) {
-            const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row that sees nothing: zeros
-            f[0] *= inv;
-            f[1] *= inv;
-          } else if (t == 0) {
-            mine[D * kTreeRows + row] = up;
-            mine[(D + 1) * kTreeRows + row] = l;
-          }
-          T* to = static_cast<T*>(a.out) + (token0 + row / a.group) * a.out_stride + int64_t(head0 + row % a.group) * D;
+        if (C == 1) {
+          if (ok && lane_row < rows) {
+            const float m0 = bars->tops[0][row], m1 = bars->tops[1][row], up = fmaxf(m0, m1), zero = up == -INFINITY ? 0.f : up;
+            float f[2] = {exp2_approx((m0 - zero) * a.scale_log2), exp2_approx((m1 - zero) * a.scale_log2)};
+            const float l = bars->sum_of[0][row] * f[0] + bars->sum_of[1][row] * f[1];
+            if (whole) {
+              const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row that sees nothing: zeros
+              f[0] *= inv;
+              f[1] *= inv;
+            } else if (t == 0) {
+              mine[D * kTreeRows + row] = up;
+              mine[(D + 1) * kTreeRows + row] = l;
+            }
+            T* to = static_cast<T*>(a.out) + (token0 + row / a.group) * a.out_stride + int64_t(head0 + row % a.group) * D;
 #pragma unroll
+            for (int i = t * (D / 64); i < (t + 1) * (D / 64); ++i) {
+              float o[32], x[32];
+#pragma unroll
+              for (int c = 0; c < 32; ++c) x[c] = 0.f;
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                if (it == piece && w != (it & 1)) continue;  // one block: one stream
+                tmem_ld32(lanes + kO + 128 * w + 32 * i, o);
+                tmem_ld_wait();
+                tmem_landed(o);
+#pragma unroll
+                for (int c = 0; c < 32; ++c) x[c] = fmaf(o[c], f[w], x[c]);
+              }
+              if (row < rows) {
+                if (whole) {
+#pragma unroll
+                  for (int c = 0; c < 4; ++c) {
+                    uint4 v;
+                    v.x = pack2<T>(x[8 * c], x[8 * c + 1]);
+                    v.y = pack2<T>(x[8 * c + 2], x[8 * c + 3]);
+                    v.z = pack2<T>(x[8 * c + 4], x[8 * c + 5]);
+                    v.w = pack2<T>(x[8 * c + 6], x[8 * c + 7]);
+                    *reinterpret_cast<uint4*>(to + 32 * i + 8 * c) = v;
+                  }
+                } else {
+#pragma unroll
+                  for (int c = 0; c < 8; ++c)
+                    *reinterpret_cast<float4*>(mine + ((8 * i + c) * kTreeRows + row) * 4) = make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+                }
+              }
+              __syncwarp();  // (the next read of tensor memory takes the whole warp)
+            }
+            tc_fence_before();
+          }
+        } else {
+          const bool works = ok && lane_row % span < rows;
+          float f[2] = {0.f, 0.f};
+          T* to = static_cast<T*>(a.out) + (token0 + place / a.group) * a.out_stride + int64_t(head0 + place % a.group) * D;
+          if (works) {
+            float up = -INFINITY, l = 0.f;
+            for (int r = place; r < kTreeRows; r += span) up = fmaxf(up, fmaxf(bars->tops[0][r], bars->tops[1][r]));
+            const float zero = up == -INFINITY ? 0.f : up;
+            for (int r = place; r < kTreeRows; r += span)
+              l += bars->sum_of[0][r] * exp2_approx((bars->tops[0][r] - zero) * a.scale_log2) +
+                   bars->sum_of[1][r] * exp2_approx((bars->tops[1][r] - zero) * a.scale_log2);
+            f[0] = exp2_approx((bars->tops[0][row] - zero) * a.scale_log2);
+            f[1] = exp2_approx((bars->tops[1][row] - zero) * a.scale_log2);
+            if (whole) {
+              const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row that sees nothing: zeros
+              f[0] *= inv;
+              f[1] *= inv;
+            } else if (t == 0 && copy == 0) {
+              mine[D * kTreeRows + place] = up;
+              mine[(D + 1) * kTreeRows + place] = l;
+            }
+          }
+          // Four columns of a row, where they go.
+          auto put = [&](int column, const float4& x) {
+            if (!works || place >= rows) return;
+            if (whole) {
+              *reinterpret_cast<uint2*>(to + column) = make_uint2(pack2<T>(x.x, x.y), pack2<T>(x.z, x.w));
+            } else {
+              *reinterpret_cast<float4*>(mine + (column / 4 * kTreeRows + place) * 4) = x;
+            }
+          };
+#pragma unroll 1
           for (int i = t * (D / 64); i < (t + 1) * (D / 64); ++i) {
-            float o[32], x[32];
+            float x[32];
 #pragma unroll
             for (int c = 0; c < 32; ++c) x[c] = 0.f;
+            if (works) {
+              __syncwarp();
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              if (it == piece && w != (it & 1)) continue;  // one block: one stream
-              tmem_ld32(lanes + kO + 128 * w + 32 * i, o);
-              tmem_ld_wait();
-              tmem_landed(o);
+              for (int w = 0; w < 2; ++w) {
+                if (it == piece && w != (it & 1)) continue;  // one block: one stream
+                float o[32];
+                tmem_ld32(lanes + kO + 128 * w + 32 * i, o);
+                tmem_ld_wait();
+                tmem_landed(o);
 #pragma unroll
-              for (int c = 0; c < 32; ++c) x[c] = fmaf(o[c], f[w], x[c]);
-            }
-            if (row < rows) {
-              if (whole) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                  uint4 v;
-                  v.x = pack2<T>(x[8 * c], x[8 * c + 1]);
-                  v.y = pack2<T>(x[8 * c + 2], x[8 * c + 3]);
-                  v.z = pack2<T>(x[8 * c + 4], x[8 * c + 5]);
-                  v.w = pack2<T>(x[8 * c + 6], x[8 * c + 7]);
-                  *reinterpret_cast<uint4*>(to + 32 * i + 8 * c) = v;
-                }
-              } else {
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-                  *reinterpret_cast<float4*>(mine + ((8 * i + c) * kTreeRows + row) * 4) = make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+                for (int c = 0; c < 32; ++c) x[c] = fmaf(o[c], f[w], x[c]);
               }
             }
-            __syncwarp();  // (the next read of tensor memory takes the whole warp)
+            // Each copy adds a part of the columns, in the order of the copies.
+            float4* at = meet + t * (8 * kTreeRows);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) at[c * kTreeRows + row] = make_float4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+            warps_sync(3 + t, kTreeRows);
+            for (int c = copy * (8 / C); c < (copy + 1) * (8 / C); ++c) {
+              float4 all = at[c * kTreeRows + place];
+              for (int r = place + span; r < kTreeRows; r += span) {
+                const float4 v = at[c * kTreeRows + r];
+                all.x += v.x;
+                all.y += v.y;
+                all.z += v.z;
+                all.w += v.w;
+              }
+              put(32 * i + 4 * c, all);
+            }
+            warps_sync(3 + t, kTreeRows);
           }
-          tc_fence_before();
+          if (works) tc_fence_before();
         }
         if (!whole) {
           __threadfence();
@@ -636,12 +735,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
   if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(bars->tmem), "r"(512) : "memory");
 }
 
+template <class T, int D, int C>
+cudaError_t launch_tree_copies(const TreeArgs& a, const TreeMaps& maps, cudaStream_t s) {
+  static PerDeviceOnce once;
+  const cudaError_t e = per_device_once(once, [] { return opt_in_smem(tree_kernel<T, D, C>, TreeShape<D, C>::kSmem); });
+  if (e != cudaSuccess) return e;
+  return launch_pdl(tree_kernel<T, D, C>, dim3(unsigned(sm_count())), dim3(kTreeThreads), size_t(TreeShape<D, C>::kSmem), s, a, maps);
+}
 template <class T, int D>
 cudaError_t launch_tree(const TreeArgs& a, const TreeMaps& maps, cudaStream_t s) {
-  static PerDeviceOnce once;
-  const cudaError_t e = per_device_once(once, [] { return opt_in_smem(tree_kernel<T, D>, TreeShape<D>::kSmem); });
-  if (e != cudaSuccess) return e;
-  return launch_pdl(tree_kernel<T, D>, dim3(unsigned(sm_count())), dim3(kTreeThreads), size_t(TreeShape<D>::kSmem), s, a, maps);
+  const int rows = a.tile_tokens * a.group;
+  return rows <= 32 ? launch_tree_copies<T, D, 4>(a, maps, s) : rows <= 64 ? launch_tree_copies<T, D, 2>(a, maps, s) : launch_tree_copies<T, D, 1>(a, maps, s);
 }
 
 // Drafted tokens of a row tile: whole tokens, as many as 128 rows hold.

@@ -105,6 +105,10 @@ CASES = [
     (2, 2, 8, 8, 64, 16, [12000, 9000], "float16", True),
     (2, 9, 100, 1, 64, 16, [300, 41], "bfloat16", True),              # a hundred heads of one key head: a token per row tile
     (3, 11, 45, 5, 128, 32, [260, 0, 513], "float16", True),          # 99 rows
+    (2, 10, 8, 2, 64, 16, [3000, 129], "bfloat16", True),             # 40 rows, twice in the lanes
+    (5, 16, 16, 4, 128, 64, [0, 1, 1700, 64, 4000], "float16", True),  # 64 rows
+    (2, 3, 11, 1, 128, 16, [900, 2500], "bfloat16", False),           # 33 rows
+    (3, 8, 8, 2, 64, 64, [2222, 31, 555], "float16", True),           # 32 rows, four times
     (7, 8, 8, 8, 128, 16, [15, 16, 17, 143, 144, 145, 120], "bfloat16", False),
 ]
 
@@ -219,17 +223,18 @@ def test_captured_calls_follow_the_contexts():
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_rows_that_see_nothing_and_rows_that_see_one_key(dim, dtype):
+@pytest.mark.parametrize("drafted", [64, 24, 16])
+def test_rows_that_see_nothing_and_rows_that_see_one_key(drafted, dim, dtype):
     """Exact zeros and exact copies: a weight of a hidden key that is not zero, however small, would show in both."""
     torch = _torch()
     from fngine_b200 import attention as A
-    q, kc, vc, table, ctx = setup(torch, 2, 64, 4, 2, dim, 16, [0, 0], dtype, 12)
-    mask = torch.tensor([[0 if i % 3 else 1 << i if i < 63 else -(1 << 63) for i in range(64)]] * 2, device="cuda")
-    ws, out = A.attn_tree_workspace(2, 64, 4, 2, dim), torch.full_like(q, float("nan"))
+    q, kc, vc, table, ctx = setup(torch, 2, drafted, 4, 2, dim, 16, [0, 0], dtype, 12)
+    mask = torch.tensor([[0 if i % 3 else 1 << i if i < 63 else -(1 << 63) for i in range(drafted)]] * 2, device="cuda")
+    ws, out = A.attn_tree_workspace(2, drafted, 4, 2, dim), torch.full_like(q, float("nan"))
     A.attn_tree_decode(q, A.KvCache(kc, vc), table, ctx, out, ws, mask=mask)
     torch.cuda.synchronize()
     for s in range(2):
-        for i in range(64):
+        for i in range(drafted):
             v = vc[int(table[s, i // 16]), i % 16].repeat_interleave(2, 0)
             assert torch.equal(out[s, i], v if i % 3 == 0 else torch.zeros_like(v))
     vc[int(table[1, 0]), 6] = float("nan")  # a key that one row sees: NaN in that row
@@ -239,14 +244,15 @@ def test_rows_that_see_nothing_and_rows_that_see_one_key(dim, dtype):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
-def test_not_a_number_reaches_the_rows_that_see_it(dim):
+@pytest.mark.parametrize("drafted", [3, 20, 50])
+def test_not_a_number_reaches_the_rows_that_see_it(drafted, dim):
     """A key of the context that is not a number: every row of its sequence and key head, and no other."""
     torch = _torch()
     from fngine_b200 import attention as A
     for at in range(0, 300, 37):
-        q, kc, vc, table, ctx = setup(torch, 2, 3, 4, 2, dim, 16, [300, 200], "bfloat16", 13)
+        q, kc, vc, table, ctx = setup(torch, 2, drafted, 4, 2, dim, 16, [300, 200], "bfloat16", 13)
         kc[int(table[0, at // 16]), at % 16, 1] = float("nan")
-        ws, out = A.attn_tree_workspace(2, 3, 4, 2, dim), torch.zeros_like(q)
+        ws, out = A.attn_tree_workspace(2, drafted, 4, 2, dim), torch.zeros_like(q)
         A.attn_tree_decode(q, A.KvCache(kc, vc), table, ctx, out, ws)
         torch.cuda.synchronize()
         assert bool(torch.isnan(out[0, :, 2:]).all()) and not bool(torch.isnan(out[0, :, :2]).any()) and not bool(torch.isnan(out[1]).any())
