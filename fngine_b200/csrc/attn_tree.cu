@@ -15,8 +15,8 @@
 // warps, S, O, maxima and sums of their own, which meet where a segment ends: each O is read there by both, half of the columns each.
 // And a warp reaches only its 32 lanes of tensor memory: up to 32 rows lie there four times (up to 64 twice), and each copy takes a part of a
 // block's keys, with zeros for weights of the others, and a maximum, a sum and an O of its own until the segment ends.
-// 32 sequences of up to 16384 keys, four tokens, 32 heads of 128: 274 us = 6.1 TB/s (302 without the copies of rows; head_dim 64 208
-// and 244); eight of 4096 keys, sixteen tokens, 48 heads: 42 us; one token and 1003 keys: 12.
+// 32 sequences of up to 16384 keys, four tokens, 32 heads of 128: 268 us = 6.25 TB/s (302 without the copies of rows; head_dim 64 207
+// and 244); eight of 4096 keys, sixteen tokens, 48 heads: 41 us; one token and 1003 keys: 12.
 // Blocks of context keys come by TMA, a box per run of slots that a page holds (up to 128, the power of two in the page size). The
 // block where the context ends, and all blocks where that power is below kTreeMinBox, come by cp.async, 16 bytes a thread: any slots, and
 // what is not to be read is written as zeros. (cp.async alone moves 4.4 TB/s; TMA gathers of four cache rows took 41 ns each per
@@ -675,34 +675,68 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
               // Piece b of the segment is block b's: the first begins with the segment, the others do not.
               const float* head_piece = a.partial + (2 * size_t(first) + 1) * S::kSlot;
               const float* piece0 = a.partial + 2 * size_t(first) * S::kSlot;
-              float up = __ldcg(head_piece + D * kTreeRows + r);
-#pragma unroll 8
-              for (int b = 1; b <= last - first; ++b) up = fmaxf(up, __ldcg(piece0 + size_t(2 * b) * S::kSlot + D * kTreeRows + r));
-              if (up == -INFINITY) up = 0.f;  // a row that sees nothing
-              T* to = static_cast<T*>(a.out) + (token0 + r / a.group) * a.out_stride + int64_t(head0 + r % a.group) * D;
-              for (int c0 = sub; c0 < D / 4; c0 += 4 * per_row) {
-                float l = 0.f;
-                float4 x[4];
+              // The first pieces, which most segments have no more than, in one go: their weights first, then rounds of 16 loads. (A piece that is
+              // not there is the first one again, with a weight of zero.)
+              constexpr int kFirst = 4;
+              const int pieces = last - first + 1;
+              const float* from[kFirst];
+              float f[kFirst], l = 0.f, up = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+              for (int b = 0; b < kFirst; ++b) {
+                from[b] = b && b < pieces ? piece0 + size_t(2 * b) * S::kSlot : head_piece;
+                f[b] = __ldcg(from[b] + D * kTreeRows + r);
+              }
+              float sums[kFirst];
+#pragma unroll
+              for (int b = 0; b < kFirst; ++b) sums[b] = __ldcg(from[b] + (D + 1) * kTreeRows + r);
+#pragma unroll
+              for (int b = 0; b < kFirst; ++b) up = fmaxf(up, f[b]);
 #pragma unroll 4
-                for (int b = 0; b <= last - first; ++b) {
-                  const float* from = b ? piece0 + size_t(2 * b) * S::kSlot : head_piece;
-                  const float f = exp2_approx((__ldcg(from + D * kTreeRows + r) - up) * a.scale_log2);
-                  l = fmaf(__ldcg(from + (D + 1) * kTreeRows + r), f, l);
+              for (int b = kFirst; b < pieces; ++b) up = fmaxf(up, __ldcg(piece0 + size_t(2 * b) * S::kSlot + D * kTreeRows + r));
+              if (up == -INFINITY) up = 0.f;  // a row that sees nothing
+#pragma unroll
+              for (int b = 0; b < kFirst; ++b) {
+                f[b] = b < pieces ? exp2_approx((f[b] - up) * a.scale_log2) : 0.f;
+                l = fmaf(sums[b], f[b], l);
+              }
+#pragma unroll 4
+              for (int b = kFirst; b < pieces; ++b) {
+                const float* at = piece0 + size_t(2 * b) * S::kSlot + D * kTreeRows + r;
+                l = fmaf(__ldcg(at + kTreeRows), exp2_approx((__ldcg(at) - up) * a.scale_log2), l);
+              }
+              const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+              T* to = static_cast<T*>(a.out) + (token0 + r / a.group) * a.out_stride + int64_t(head0 + r % a.group) * D;
+              auto add = [](float4& x, const float4& o, float w) {
+                x.x = fmaf(o.x, w, x.x);
+                x.y = fmaf(o.y, w, x.y);
+                x.z = fmaf(o.z, w, x.z);
+                x.w = fmaf(o.w, w, x.w);
+              };
+              for (int c0 = sub; c0 < D / 4; c0 += 4 * per_row) {
+                float4 x[4], o[kFirst][4];
+#pragma unroll
+                for (int b = 0; b < kFirst; ++b)
 #pragma unroll
                   for (int e = 0; e < 4; ++e) {
                     const int c = c0 + e * per_row;
-                    if (c < D / 4) {
-                      const float4 o = __ldcg(reinterpret_cast<const float4*>(from + (c * kTreeRows + r) * 4));
-                      x[e].x = fmaf(o.x, f, x[e].x);
-                      x[e].y = fmaf(o.y, f, x[e].y);
-                      x[e].z = fmaf(o.z, f, x[e].z);
-                      x[e].w = fmaf(o.w, f, x[e].w);
-                    }
+                    o[b][e] = __ldcg(reinterpret_cast<const float4*>(from[b] + ((c < D / 4 ? c : c0) * kTreeRows + r) * 4));
+                  }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int b = 0; b < kFirst; ++b)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) add(x[e], o[b][e], f[b]);
+#pragma unroll 2
+                for (int b = kFirst; b < pieces; ++b) {
+                  const float* at = piece0 + size_t(2 * b) * S::kSlot;
+                  const float w = exp2_approx((__ldcg(at + D * kTreeRows + r) - up) * a.scale_log2);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const int c = c0 + e * per_row;
+                    if (c < D / 4) add(x[e], __ldcg(reinterpret_cast<const float4*>(at + (c * kTreeRows + r) * 4)), w);
                   }
                 }
-                const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                   const int c = c0 + e * per_row;
