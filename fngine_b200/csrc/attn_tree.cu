@@ -36,6 +36,7 @@ constexpr int kTreeKeys = 128;           // keys of a block
 constexpr int kTreeMaxDrafted = 64;
 constexpr int kTreeMaxSms = 256;         // partial results are sized for this many blocks
 constexpr int kTreeMinBox = 8;           // slots of the smallest box
+constexpr int kTreeBarBytes = 3 * 1024;  // for barriers and tables
 constexpr float kTreeSlack = 8.f;        // how far (in powers of two) scores may rise above the maximum in use
 
 struct TreeArgs {
@@ -66,7 +67,7 @@ struct TreeShape {
   static constexpr int kHalf = kTreeKeys * 128;  // a tile is D / 64 parts of 128 rows x 128 bytes
   static constexpr int kStages = D == 64 ? 10 : C == 1 ? 5 : 4;
   static constexpr int kMeet = C == 1 ? 0 : 2 * kTreeRows * 32 * 4;  // where copies of rows meet: 32 columns for each stream's warps
-  static constexpr int kSmem = (2 + kStages) * kTileBytes + kMeet + 3072;
+  static constexpr int kSmem = (2 + kStages) * kTileBytes + kMeet + kTreeBarBytes;
   static constexpr int kSlot = (D + 2) * kTreeRows;  // floats of a partial result
 };
 
@@ -86,7 +87,7 @@ struct TreeBars {
   int in_flight;  // copies up to the last one made by TMA
   int last_block;
 };
-static_assert(sizeof(TreeBars) <= 3072, "room behind the ring");
+static_assert(sizeof(TreeBars) <= kTreeBarBytes, "room behind the ring");
 static_assert(TreeShape<128, 1>::kSmem <= 227 * 1024, "all of a multiprocessor's shared memory");
 
 // Walks through the key blocks of the segments in their order.
