@@ -156,7 +156,8 @@ def attn_tree_status(workspace):
 
 
 def attn_tree_decode(q, cache, block_table, contexts, out, workspace, mask=None, scale=None):
-    """fb_attn_tree_decode: q and out [n_seqs][drafted][heads][head_dim], block_table int32 [n_seqs][columns], contexts int32 [n_seqs],
+    """fb_attn_tree_decode_view: q and out [n_seqs][drafted][heads][head_dim], block_table int32 [n_seqs][columns] (some columns of a wider
+    table too: the others are not read), contexts int32 [n_seqs],
     mask int64 or uint64 [n_seqs][drafted] (bit d of token i: it sees drafted token d; None: d <= i), scale 1 / sqrt(head_dim) unless given."""
     n_seqs, drafted, heads, dim = q.shape
     if q.dtype is not cache.dtype or out.dtype is not q.dtype or out.shape != q.shape or dim != cache.head_dim:
@@ -169,20 +170,21 @@ def attn_tree_decode(q, cache, block_table, contexts, out, workspace, mask=None,
         if s[3] != 1 or (heads > 1 and s[2] != dim) or (n_seqs > 1 and s[0] != drafted * token):
             raise ValueError("attn_tree_decode: the tokens of q and out lie at one stride, the heads of a token side by side")
         strides.append(token)
-    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n_seqs or block_table.stride(1) != 1:
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != n_seqs or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
         raise ValueError("attn_tree_decode: block_table int32 [n_seqs][columns]")
-    columns = block_table.stride(0) if n_seqs > 1 else block_table.shape[1]
-    if columns < block_table.shape[1]:
+    columns = block_table.shape[1]
+    table_stride = block_table.stride(0) if n_seqs > 1 else columns
+    if table_stride < columns:
         raise ValueError("attn_tree_decode: rows of block_table overlap")
     if not (q.get_device() == out.get_device() == block_table.get_device() == workspace.get_device() == cache.k.get_device() == dev):
         raise ValueError("attn_tree_decode: not on the current device")
     if mask is not None and mask.dtype is not torch.int64:
         mask = mask.view(torch.int64)
-    st = L.load().fb_attn_tree_decode(q.data_ptr(), strides[0], heads, n_seqs, drafted, cache.ref, block_table.data_ptr(), columns,
-                                      _plain(contexts, (n_seqs,), torch.int32, dev, "contexts"),
-                                      None if mask is None else _plain(mask, (n_seqs, drafted), torch.int64, dev, "mask"),
-                                      dim ** -0.5 if scale is None else scale, out.data_ptr(), strides[1], workspace.data_ptr(),
-                                      workspace.numel(), L.stream())
+    st = L.load().fb_attn_tree_decode_view(q.data_ptr(), strides[0], heads, n_seqs, drafted, cache.ref, block_table.data_ptr(), table_stride, columns,
+                                           _plain(contexts, (n_seqs,), torch.int32, dev, "contexts"),
+                                           None if mask is None else _plain(mask, (n_seqs, drafted), torch.int64, dev, "mask"),
+                                           dim ** -0.5 if scale is None else scale, out.data_ptr(), strides[1], workspace.data_ptr(),
+                                           workspace.numel(), L.stream())
     if st:
         L.check(st, "attn_tree_decode")
 

@@ -48,6 +48,7 @@ struct TreeArgs {
   const uint64_t* mask;
   int64_t out_stride;  // elements between tokens
   int64_t table_stride;
+  int64_t table_columns;
   uint32_t* status;
   int32_t* counters;   // [segments]
   float* partial;      // [2 * blocks]: outputs [D / 4][128][4], maxima [128], sums [128]
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
   TreeBars* bars = reinterpret_cast<TreeBars*>(ring + kStages * S::kTileBytes + S::kMeet);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int parts = a.kv_heads * a.row_tiles;
-  const int64_t room = a.table_stride * a.page_size;  // keys that the table can hold
+  const int64_t room = a.table_columns * a.page_size;  // keys that the table can hold
   pdl_wait_prior();
   if (smem_u32(smem) & 1023u) {  // (tiles and their swizzle start on 1024 bytes)
     if (tid == 0) atomicMax(a.status, uint32_t(FB_STATUS_BAD_WORK));
@@ -838,6 +839,14 @@ int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int3
                             const fb_kv_cache* cache, const int32_t* block_table, int64_t table_stride, const int32_t* contexts,
                             const uint64_t* mask, float scale, void* out, int64_t out_stride, void* workspace,
                             size_t workspace_bytes, void* stream) {
+  return fb_attn_tree_decode_view(q, q_stride, heads, n_seqs, drafted, cache, block_table, table_stride, table_stride, contexts, mask, scale, out,
+                                  out_stride, workspace, workspace_bytes, stream);
+}
+
+int32_t fb_attn_tree_decode_view(const void* q, int64_t q_stride, int32_t heads, int32_t n_seqs, int32_t drafted,
+                                 const fb_kv_cache* cache, const int32_t* block_table, int64_t table_stride, int64_t table_columns,
+                                 const int32_t* contexts, const uint64_t* mask, float scale, void* out, int64_t out_stride,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
   if (!cache) return invalid("attn_tree_decode: null argument");
   const int dim = cache->head_dim, kv = cache->kv_heads;
   if (cache->dtype != FB_DT_BF16 && cache->dtype != FB_DT_F16) return invalid("attn_tree_decode: bf16 or fp16");
@@ -847,8 +856,10 @@ int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int3
   if (!n_seqs) return 0;
   if (!q || !out || !block_table || !contexts || !cache->k || !cache->v) return invalid("attn_tree_decode: null argument");
   if (cache->page_size < 1 || cache->n_pages < 1) return invalid("attn_tree_decode: a cache without pages");
-  if (table_stride < 1) return invalid("attn_tree_decode: a table without columns");
-  if (table_stride > INT32_MAX / 2 / cache->page_size) return invalid("attn_tree_decode: more than 2^30 keys per sequence");
+  if (table_columns < 1) return invalid("attn_tree_decode: a table without columns");
+  if (table_columns > INT32_MAX / 2 / cache->page_size) return invalid("attn_tree_decode: more than 2^30 keys per sequence");
+  if (table_stride < table_columns) return invalid("attn_tree_decode: rows of the table overlap");
+  if (table_stride > INT32_MAX) return invalid("attn_tree_decode: rows of the table lie too far apart");
   if (cache->n_pages > INT32_MAX / cache->page_size) return invalid("attn_tree_decode: a cache of more than 2^31 slots");
   if (int64_t(n_seqs) * drafted > INT32_MAX || q_stride >= int64_t(1) << 38)
     return invalid("attn_tree_decode: q is too large");
@@ -877,6 +888,7 @@ int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int3
   a.mask = mask;
   a.out_stride = out_stride;
   a.table_stride = table_stride;
+  a.table_columns = table_columns;
   uint8_t* base = static_cast<uint8_t*>(workspace);
   a.status = reinterpret_cast<uint32_t*>(base);
   a.partial = reinterpret_cast<float*>(base + 256);

@@ -184,6 +184,8 @@ _SIGNATURES = {
     "fb_attn_tree_workspace_bytes": (C.c_size_t, [_I32, _I32, _I32, _I32, _I32]),
     "fb_attn_tree_decode": (_I32, [_P, _I64, _I32, _I32, _I32, C.POINTER(KvCacheArgs), _P, _I64, _P, _P, C.c_float, _P, _I64,
                                    _P, C.c_size_t, _P]),
+    "fb_attn_tree_decode_view": (_I32, [_P, _I64, _I32, _I32, _I32, C.POINTER(KvCacheArgs), _P, _I64, _I64, _P, _P, C.c_float, _P, _I64,
+                                        _P, C.c_size_t, _P]),
     "fb_dequant_rows": (_I32, [_I32, _P, _I64, _I32, _I32, _P, _P]),
     "fb_quantize_act": (_I32, [_I32, _P, _I32, _I32, _I32, _P, _P]),
     "fb_synth_fill_blocks": (_I32, [_I32, _P, _I64, _I64, C.c_uint64, _P, _P]),

@@ -560,7 +560,7 @@ typedef struct fb_kv_cache {
   int32_t head_dim;
 } fb_kv_cache;
 /* Attention of `drafted` tokens (1..64) per sequence over the cache. Position p of sequence s lies in page block_table[s *
- * table_stride + p / page_size]; positions 0 .. contexts[s] - 1 are the context, which every token sees, and the keys and
+ * table_stride + p / page_size] of the table's table_stride columns; positions 0 .. contexts[s] - 1 are the context, which every token sees, and the keys and
  * values of the drafted tokens follow at contexts[s] .. contexts[s] + drafted - 1 (fb_qk_norm_rope puts them there). Token
  * i sees drafted token d if bit d of mask[s * drafted + i] is set; mask NULL: if d <= i. So one token per sequence is plain
  * decoding, and a shorter tree is padded with tokens whose masks are zero. q and out are [n_seqs * drafted][heads][head_dim] with
@@ -580,6 +580,12 @@ int32_t fb_attn_tree_decode(const void* q, int64_t q_stride, int32_t heads, int3
                             const fb_kv_cache* cache, const int32_t* block_table, int64_t table_stride, const int32_t* contexts,
                             const uint64_t* mask, float scale, void* out, int64_t out_stride, void* workspace,
                             size_t workspace_bytes, void* stream);
+/* The same for a table that is a range of a wider one's columns: rows lie table_stride elements apart and hold table_columns of
+ * this table (1 .. table_stride). What lies between is not read, and a context is brought into 0 .. table_columns * page_size. */
+int32_t fb_attn_tree_decode_view(const void* q, int64_t q_stride, int32_t heads, int32_t n_seqs, int32_t drafted,
+                                 const fb_kv_cache* cache, const int32_t* block_table, int64_t table_stride, int64_t table_columns,
+                                 const int32_t* contexts, const uint64_t* mask, float scale, void* out, int64_t out_stride,
+                                 void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------- parity probes (no reference counterpart)
  * The same device routines the GEMV kernels use, exposed so that dequantized weights and int8

@@ -1,0 +1,84 @@
+"""What the Python entry points of the attention branch hand to the library, and what they refuse before it is called. No GPU: the tensors are
+the CPU's, whose device number stands for the current device's, and the library is a stand-in that notes its arguments."""
+import ctypes as C
+import types
+
+import pytest
+import torch
+
+from fngine_b200 import attention as A
+from fngine_b200 import lib as L
+
+BF16 = torch.bfloat16
+
+
+class Calls:
+    """A library whose functions note their name and arguments and succeed."""
+
+    def __init__(self):
+        self.made = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.made.append((name, args))
+            return 0
+        return call
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    made = Calls()
+    monkeypatch.setattr(L, "load", lambda: made)
+    monkeypatch.setattr(L, "stream", lambda: None)
+    monkeypatch.setattr(A, "_device", lambda: -1)
+    return made
+
+
+def cache_of(pages=9, page=16, kv=2, dim=64, dtype=BF16):
+    """A KvCache of CPU tensors (its constructor wants the GPU's)."""
+    c = types.SimpleNamespace(k=torch.zeros(pages, page, kv, dim, dtype=dtype), v=torch.zeros(pages, page, kv, dim, dtype=dtype), n_pages=pages,
+                              page_size=page, kv_heads=kv, head_dim=dim, dtype=dtype)
+    c.c = L.KvCacheArgs(c.k.data_ptr(), c.v.data_ptr(), pages, page, A._DTYPES[dtype], kv, dim)
+    c.ref = C.byref(c.c)
+    c.k_rows, c.v_rows = c.k.view(-1, kv, dim), c.v.view(-1, kv, dim)
+    return c
+
+
+def tree(table, seqs=3, drafted=2, **change):
+    a = dict(q=torch.zeros(seqs, drafted, 4, 64, dtype=BF16), cache=cache_of(), block_table=table, contexts=torch.zeros(seqs, dtype=torch.int32),
+             out=torch.zeros(seqs, drafted, 4, 64, dtype=BF16), workspace=torch.zeros(1024, dtype=torch.uint8))
+    a.update(change)
+    return A.attn_tree_decode(**a)
+
+
+def test_a_table_of_some_columns_has_a_stride_and_a_width(calls):
+    """Columns of a wider table: the width is the view's, whatever lies beside it, for one sequence as for several."""
+    wide = torch.zeros(3, 100, dtype=torch.int32)
+    for table, seqs, stride, columns in [(wide, 3, 100, 100), (wide[:, :10], 3, 100, 10), (wide[:, 90:], 3, 100, 10), (wide[:, 5:6], 3, 100, 1),
+                                         (wide[1:2, 90:], 1, 10, 10), (wide[:, :10].contiguous(), 3, 10, 10), (wide[:1].expand(3, 100)[:, :100].contiguous(), 3, 100, 100),
+                                         (torch.zeros(1, 3, dtype=torch.int32).T, 3, 1, 1)]:
+        tree(table, seqs)
+        name, args = calls.made.pop()
+        assert name == "fb_attn_tree_decode_view" and args[6:9] == (table.data_ptr(), stride, columns)
+    for table in (wide.T[:3], wide[:2], wide[:, ::2], wide[:1, :10].expand(3, 10), wide.long()):
+        with pytest.raises(ValueError):
+            tree(table)
+    assert not calls.made
+
+
+def test_tree_table_refusals(fb_built):
+    """The library's own checks of a table's stride and width; addresses are made up."""
+    P = 0x100000
+    lib = L.load()
+    size = lib.fb_attn_tree_workspace_bytes(2, 3, 8, 2, 128)
+    c = L.KvCacheArgs(7 * P, 8 * P, 9, 16, L.DT_F16, 2, 128)
+
+    def call(stride, columns, n_seqs=2):
+        st = lib.fb_attn_tree_decode_view(P, 1024, 8, n_seqs, 3, C.byref(c), 2 * P, stride, columns, 3 * P, None, 0.1, 5 * P, 1024, 6 * P, size, None)
+        return st, lib.fb_last_error_string()
+
+    for stride, columns, word in [(4, 0, b"columns"), (4, -1, b"columns"), (4, 5, b"overlap"), (0, 4, b"overlap"), (-4, 4, b"overlap"), (2 ** 31, 4, b"far apart"),
+                                  (2 ** 27, 2 ** 27, b"2^30")]:
+        st, msg = call(stride, columns)
+        assert st == 1 and word in msg, (stride, columns, st, msg)
+    assert call(4, 4, 0)[0] == 0
