@@ -99,9 +99,10 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, eps, rope, positions, q_out, k_out
         L.check(st, "qk_norm_rope")
 
 
-def attn_prefill(q, k, v, cu_seqlens, out, scale=None, status=None):
+def attn_prefill(q, k, v, cu_seqlens, out, scale=None, status=None, padded=False):
     """fb_attn_prefill: q and out [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim], cu_seqlens int32 [n_seqs + 1]; scale
-    1 / sqrt(head_dim) unless given. status: a word (int32 [1]) that a wait which ran out sets."""
+    1 / sqrt(head_dim) unless given. status: a word (int32 [1]) that a wait which ran out sets. Tokens outside of all sequences are left as
+    they were in out; padded (fb_attn_prefill_padded): they get zeros."""
     tokens, heads, dim = q.shape
     kv_heads, dtype = k.shape[1], q.dtype
     if dtype not in _DTYPES:
@@ -114,10 +115,10 @@ def attn_prefill(q, k, v, cu_seqlens, out, scale=None, status=None):
     v_at, v_stride = _heads(v, tokens, kv_heads, dim, dtype, dev, "v")
     o_at, o_stride = _heads(out, tokens, heads, dim, dtype, dev, "out")
     n_seqs = cu_seqlens.shape[0] - 1
-    st = L.load().fb_attn_prefill(L.Qkv(q_at, k_at, v_at, q_stride, k_stride, v_stride, _DTYPES[dtype], heads, kv_heads, dim), tokens,
-                                  _plain(cu_seqlens, (n_seqs + 1,), torch.int32, dev, "cu_seqlens"), n_seqs,
-                                  dim ** -0.5 if scale is None else scale, o_at, o_stride,
-                                  None if status is None else _plain(status, (1,), torch.int32, dev, "status"), L.stream())
+    call = L.load().fb_attn_prefill_padded if padded else L.load().fb_attn_prefill
+    st = call(L.Qkv(q_at, k_at, v_at, q_stride, k_stride, v_stride, _DTYPES[dtype], heads, kv_heads, dim), tokens,
+              _plain(cu_seqlens, (n_seqs + 1,), torch.int32, dev, "cu_seqlens"), n_seqs, dim ** -0.5 if scale is None else scale, o_at, o_stride,
+              None if status is None else _plain(status, (1,), torch.int32, dev, "status"), L.stream())
     if st:
         L.check(st, "attn_prefill")
 
@@ -245,8 +246,8 @@ class AttentionBranch:
 
 def forward_attention_prefill(branch, x, cu_seqlens, positions, X, inj, cache=None, slots=None):
     """The attention branch over packed prompts: projection, norms and rotation, causal attention, projection with the residual write X
-    += inj * y (X fp32 [T][4][hidden], inj [T][4]). x bf16 [T][hidden]. With `cache` the keys and values are put to `slots` for
-    forward_attention_decode."""
+    += inj * y (X fp32 [T][4][hidden], inj [T][4]). x bf16 [T][hidden]. Tokens outside of all sequences (padding) add nothing to X. With
+    `cache` the keys and values are put to `slots` for forward_attention_decode."""
     tokens = branch.check(x, X, inj)
     if not tokens:
         return
@@ -256,7 +257,7 @@ def forward_attention_prefill(branch, x, cu_seqlens, positions, X, inj, cache=No
     if cache is not None:
         kv_store(k, v, cache, slots)
     o = branch.o[:tokens]
-    attn_prefill(q, k, v, cu_seqlens, o)
+    attn_prefill(q, k, v, cu_seqlens, o, padded=True)
     branch.project(o.flatten(1), 1, linear.gr_write(X, inj))
 
 

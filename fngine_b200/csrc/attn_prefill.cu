@@ -41,6 +41,7 @@ struct PfArgs {
   int64_t out_stride;
   float scale_log2;
   int n_seqs, tokens, group;
+  int clear;  // tokens outside of all sequences get zeros
 };
 struct PfMaps {
   CUtensorMap q, k, v;
@@ -72,9 +73,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
   pdl_wait_prior();
 
   // Which sequence and which 256 queries: item blockIdx.y counts the items of the sequences in order, each from its end.
+  // (With `clear` the last blockIdx.y has no item.)
   int start = 0, length = -1, item = -1;
   {
-    int before = 0;
+    const int number = a.clear && blockIdx.y + 1 == gridDim.y ? INT32_MAX : int(blockIdx.y);
+    int before = 0, least = a.tokens, most = 0;
     for (int base = 0; base < a.n_seqs; base += 32) {
       const int s = base + lane;
       int lo = 0, hi = 0;
@@ -85,13 +88,17 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
         hi = hi < lo ? lo : hi > a.tokens ? a.tokens : hi;
       }
       const int n = (hi - lo + kPfQueries - 1) / kPfQueries;
+      if (n) {
+        least = lo < least ? lo : least;
+        most = hi > most ? hi : most;
+      }
       int upto = n;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int other = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += other;
       }
-      const int at = int(blockIdx.y) - before;
+      const int at = number - before;
       const bool mine = n > 0 && at < upto && at >= upto - n;
       const uint32_t who = __ballot_sync(0xffffffffu, mine);
       if (who) {
@@ -103,8 +110,23 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
     }
+    if (item < 0) {  // (block-uniform)
+      // With `clear` the blocks without an item, from `idle` on, share the tokens in front of the first and behind the last sequence, each
+      // for its head. (`before` is the number of items where the ends do not fall.)
+      const int idle = before >= 0 && before < int(gridDim.y) - 1 ? before : int(gridDim.y) - 1;
+      if (!a.clear || int(blockIdx.y) < idle) return;
+      least = __reduce_min_sync(0xffffffffu, least);
+      most = __reduce_max_sync(0xffffffffu, most);
+      most = most < least ? least : most;
+      constexpr int kChunks = D / 8, kRows = kPfThreads / kChunks;
+      const int64_t rest = int64_t(least) + a.tokens - most, step = int64_t(int(gridDim.y) - idle) * kRows;
+      for (int64_t i = int64_t(int(blockIdx.y) - idle) * kRows + tid / kChunks; i < rest; i += step) {
+        const int64_t row = i < least ? i : most + (i - least);
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + row * a.out_stride + int64_t(blockIdx.x) * D + tid % kChunks * 8) = make_uint4(0, 0, 0, 0);
+      }
+      return;
+    }
   }
-  if (item < 0) return;  // (block-uniform)
   const int head = blockIdx.x, kv_head = head / a.group;
   const int row0 = item * kPfQueries;
   const int blocks0 = 2 * item + 1, blocks1 = row0 + kPfRows < length ? 2 * item + 2 : 0;
@@ -392,15 +414,9 @@ cudaError_t launch_pf(const PfArgs& a, const PfMaps& maps, dim3 grid, cudaStream
   return launch_pdl(attn_prefill_kernel<T, D>, grid, dim3(kPfThreads), size_t(PfShape<D>::kSmem), s, a, maps);
 }
 
-}  // namespace
-}  // namespace fb
-
-using namespace fb;
-
-extern "C" {
-
-int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seqlens, int32_t n_seqs, float scale, void* out,
-                        int64_t out_stride, uint32_t* status, void* stream) {
+// The call; clear: tokens outside of all sequences get zeros.
+int32_t attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seqlens, int32_t n_seqs, float scale, void* out, int64_t out_stride,
+                     uint32_t* status, void* stream, bool clear) {
   if (!in) return invalid("attn_prefill: null argument");
   const int dim = in->head_dim;
   if (in->dtype != FB_DT_BF16 && in->dtype != FB_DT_F16) return invalid("attn_prefill: bf16 or fp16");
@@ -408,7 +424,7 @@ int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seql
   if (in->kv_heads < 1 || in->heads < in->kv_heads || in->heads % in->kv_heads || in->heads > 1024)
     return invalid("attn_prefill: heads is a multiple of kv_heads, up to 1024");
   if (tokens < 0 || n_seqs < 0) return invalid("attn_prefill: tokens or n_seqs is negative");
-  if (!tokens || !n_seqs) return 0;
+  if (!tokens || (!n_seqs && !clear)) return 0;
   if (!in->q || !in->k || !in->v || !out || !cu_seqlens) return invalid("attn_prefill: null argument");
   if (in->q_stride < int64_t(in->heads) * dim || in->k_stride < int64_t(in->kv_heads) * dim ||
       in->v_stride < int64_t(in->kv_heads) * dim || out_stride < int64_t(in->heads) * dim)
@@ -421,7 +437,7 @@ int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seql
     return invalid("attn_prefill: cu_seqlens or status is not aligned");
   if (!(scale > 0.f && scale <= 1.0e30f)) return invalid("attn_prefill: scale is not positive and finite");
   const int64_t items = tokens / kPfQueries + int64_t(n_seqs < tokens ? n_seqs : tokens);
-  if (items > 65535) return invalid("attn_prefill: more than 65535 blocks of 256 queries");
+  if (items + clear > 65535) return invalid("attn_prefill: more than 65535 blocks of 256 queries");
   if (!encode_tiled_fn()) {
     set_error("attn_prefill: cuTensorMapEncodeTiled is not available");
     return int32_t(cudaErrorNotSupported);
@@ -441,12 +457,30 @@ int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seql
   a.n_seqs = n_seqs;
   a.tokens = tokens;
   a.group = in->heads / in->kv_heads;
-  const dim3 grid(unsigned(in->heads), unsigned(items));
+  a.clear = clear;
+  const dim3 grid(unsigned(in->heads), unsigned(items + clear));
   cudaStream_t s = as_stream(stream);
   const cudaError_t e = dim == 64 ? (bf ? launch_pf<__nv_bfloat16, 64>(a, maps, grid, s) : launch_pf<__half, 64>(a, maps, grid, s))
                                   : (bf ? launch_pf<__nv_bfloat16, 128>(a, maps, grid, s) : launch_pf<__half, 128>(a, maps, grid, s));
   const int32_t st = check_launch("attn_prefill");
   return st ? st : int32_t(e);
+}
+
+}  // namespace
+}  // namespace fb
+
+using namespace fb;
+
+extern "C" {
+
+int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seqlens, int32_t n_seqs, float scale, void* out,
+                        int64_t out_stride, uint32_t* status, void* stream) {
+  return attn_prefill(in, tokens, cu_seqlens, n_seqs, scale, out, out_stride, status, stream, false);
+}
+
+int32_t fb_attn_prefill_padded(const fb_qkv* in, int32_t tokens, const int32_t* cu_seqlens, int32_t n_seqs, float scale, void* out,
+                               int64_t out_stride, uint32_t* status, void* stream) {
+  return attn_prefill(in, tokens, cu_seqlens, n_seqs, scale, out, out_stride, status, stream, true);
 }
 
 }  // extern "C"

@@ -181,6 +181,7 @@ _SIGNATURES = {
     "fb_linear_q4_decode": (_I32, [_P, _I32, C.POINTER(Q4Weight), C.POINTER(LinearEpilogue), _P]),
     "fb_qk_norm_rope": (_I32, [C.POINTER(Qkv), _I32, C.POINTER(QkNorm), C.POINTER(RopeArgs), C.POINTER(QkvOut), _P]),
     "fb_attn_prefill": (_I32, [C.POINTER(Qkv), _I32, _P, _I32, C.c_float, _P, _I64, _P, _P]),
+    "fb_attn_prefill_padded": (_I32, [C.POINTER(Qkv), _I32, _P, _I32, C.c_float, _P, _I64, _P, _P]),
     "fb_attn_tree_workspace_bytes": (C.c_size_t, [_I32, _I32, _I32, _I32, _I32]),
     "fb_attn_tree_decode": (_I32, [_P, _I64, _I32, _I32, _I32, C.POINTER(KvCacheArgs), _P, _I64, _P, _P, C.c_float, _P, _I64,
                                    _P, C.c_size_t, _P]),

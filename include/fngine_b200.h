@@ -548,6 +548,10 @@ int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm
  * wait ran out. No workspace. out lies apart from q, k and v. head_dim 64 or 128; everything 16-byte aligned, strides multiples of 8 elements. */
 int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seqlens, int32_t n_seqs, float scale, void* out,
                         int64_t out_stride, uint32_t* status, void* stream);
+/* The same, but tokens outside of all sequences (in front of the first, behind the last: a batch padded to a fixed width) get zeros, so
+ * that a projection behind it adds nothing for them. n_seqs 0: all tokens. */
+int32_t fb_attn_prefill_padded(const fb_qkv* in, int32_t tokens, const int32_t* cu_seqlens, int32_t n_seqs, float scale, void* out,
+                               int64_t out_stride, uint32_t* status, void* stream);
 
 /* A paged cache of keys and values: k and v [n_pages][page_size][kv_heads][head_dim], bf16 or fp16, 16-byte aligned. */
 typedef struct fb_kv_cache {

@@ -82,3 +82,26 @@ def test_tree_table_refusals(fb_built):
         st, msg = call(stride, columns)
         assert st == 1 and word in msg, (stride, columns, st, msg)
     assert call(4, 4, 0)[0] == 0
+
+
+def branch_of(monkeypatch, tokens=8, heads=4, kv=2, dim=64, hidden=256):
+    """An AttentionBranch over stand-ins of its projections, which note what they are called with."""
+    made = []
+    monkeypatch.setattr(A.linear, "linear_fp8", lambda x, w, epilogue, work: made.append(w.name))
+    weight = lambda name, n, k: types.SimpleNamespace(name=name, n=n, k=k, codes=torch.zeros(1, dtype=torch.uint8))
+    b = A.AttentionBranch(weight("qkv", (heads + 2 * kv) * dim, hidden), weight("out", hidden, heads * dim), None, None, 1e-6, None, heads, kv, dim, tokens)
+    b.made, b.hidden = made, hidden
+    return b
+
+
+def prompt(b, tokens=4, ends=(0, 2, 4), **more):
+    return A.forward_attention_prefill(b, torch.zeros(tokens, b.hidden, dtype=BF16), torch.tensor(ends, dtype=torch.int32), None,
+                                       torch.zeros(tokens, 4, b.hidden), torch.zeros(tokens, 4), **more)
+
+
+def test_the_branch_asks_for_zeros_where_there_is_no_sequence(calls, monkeypatch):
+    b = branch_of(monkeypatch)
+    prompt(b)
+    assert [name for name, _ in calls.made] == ["fb_qk_norm_rope", "fb_attn_prefill_padded"] and b.made == ["qkv", "out"]
+    A.attn_prefill(b.o, b.o[:, :2], b.o[:, :2].clone(), torch.tensor([0, 8], dtype=torch.int32), b.o.clone())
+    assert calls.made[-1][0] == "fb_attn_prefill"
