@@ -217,7 +217,13 @@ class AttentionBranch:
         device = qkv.codes.device
         self.rows = torch.empty(max_tokens, qkv.n, dtype=torch.bfloat16, device=device)
         self.o = torch.empty(max_tokens, heads, head_dim, dtype=torch.bfloat16, device=device)
+        self.status_word = torch.zeros(1, dtype=torch.int32, device=device)
         self._work = [linear.linear_fp8_workspace(w, max_tokens, device) if isinstance(w, linear.Fp8RowWeight) else None for w in (qkv, out)]
+
+    def status(self):
+        """FB_STATUS_* of the prompts' attention so far (waits for it): not zero once a bounded wait has run out, and the residual streams of that call
+        are not to be used. That of the drafted tokens' is in their workspace (attn_tree_status)."""
+        return int(self.status_word.item())
 
     def parts(self, tokens):
         """q, k and v of the projection's output, [tokens][heads or kv_heads][head_dim]."""
@@ -257,7 +263,7 @@ def forward_attention_prefill(branch, x, cu_seqlens, positions, X, inj, cache=No
     if cache is not None:
         kv_store(k, v, cache, slots)
     o = branch.o[:tokens]
-    attn_prefill(q, k, v, cu_seqlens, o, padded=True)
+    attn_prefill(q, k, v, cu_seqlens, o, status=branch.status_word, padded=True)
     branch.project(o.flatten(1), 1, linear.gr_write(X, inj))
 
 

@@ -105,3 +105,14 @@ def test_the_branch_asks_for_zeros_where_there_is_no_sequence(calls, monkeypatch
     assert [name for name, _ in calls.made] == ["fb_qk_norm_rope", "fb_attn_prefill_padded"] and b.made == ["qkv", "out"]
     A.attn_prefill(b.o, b.o[:, :2], b.o[:, :2].clone(), torch.tensor([0, 8], dtype=torch.int32), b.o.clone())
     assert calls.made[-1][0] == "fb_attn_prefill"
+
+
+def test_the_branch_reports_a_wait_that_ran_out(calls, monkeypatch):
+    """The prompts' attention gets the branch's own status word, a zero until then, and status() reads it."""
+    b = branch_of(monkeypatch)
+    assert b.status() == 0
+    prompt(b)
+    args = dict(calls.made)["fb_attn_prefill_padded"]
+    C.c_int32.from_address(args[7]).value = 1  # as the kernel does
+    assert b.status() == 1
+    assert branch_of(monkeypatch).status() == 0  # a word of its own each

@@ -86,3 +86,4 @@ def test_a_padded_batch_adds_nothing_to_its_padding(kind, tokens):
         assert torch.equal(results[0][:a], before[:a]) and torch.equal(results[0][b:], before[b:])
         assert bool(torch.isfinite(results[0]).all()) and (a == b or bool((results[0][a:b] != before[a:b]).any(2).all()))
         assert not bool(branch.o[:a].any()) and not bool(branch.o[b:tokens].any())
+    assert branch.status() == 0
