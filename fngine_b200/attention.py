@@ -196,6 +196,8 @@ def kv_store(k, v, cache, slots):
     tokens, dev = k.shape[0], _device()
     k_at, k_stride = _heads(k, tokens, cache.kv_heads, cache.head_dim, cache.dtype, dev, "k")
     v_at, v_stride = _heads(v, tokens, cache.kv_heads, cache.head_dim, cache.dtype, dev, "v")
+    if cache.k.get_device() != dev:
+        raise ValueError("kv_store: the cache is not on the current device")
     slot = cache.kv_heads * cache.head_dim
     st = L.load().fb_qk_norm_rope(L.Qkv(None, k_at, v_at, 0, k_stride, v_stride, _DTYPES[cache.dtype], 0, cache.kv_heads, cache.head_dim), tokens,
                                   None, None, L.QkvOut(None, cache.c.k, cache.c.v, 0, slot, slot, _plain(slots, (tokens,), torch.int64, dev, "slots"),

@@ -116,3 +116,27 @@ def test_the_branch_reports_a_wait_that_ran_out(calls, monkeypatch):
     C.c_int32.from_address(args[7]).value = 1  # as the kernel does
     assert b.status() == 1
     assert branch_of(monkeypatch).status() == 0  # a word of its own each
+
+
+class Elsewhere:
+    """A tensor as it is, but on another device."""
+
+    def __init__(self, x):
+        self.x = x
+
+    def __getattr__(self, name):
+        return getattr(self.x, name)
+
+    def get_device(self):
+        return 1
+
+
+def test_kv_store_wants_its_cache_on_the_current_device(calls):
+    k, slots = torch.zeros(3, 2, 64, dtype=BF16), torch.zeros(3, dtype=torch.int64)
+    cache = cache_of()
+    A.kv_store(k, k.clone(), cache, slots)
+    assert [name for name, _ in calls.made] == ["fb_qk_norm_rope"]
+    cache.k, cache.v = Elsewhere(cache.k), Elsewhere(cache.v)
+    with pytest.raises(ValueError, match="cache"):
+        A.kv_store(k, k.clone(), cache, slots)
+    assert len(calls.made) == 1
