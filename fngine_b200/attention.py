@@ -57,6 +57,8 @@ class Rope:
             raise ValueError("positions: int32 [%d axes][%d tokens], contiguous along the tokens" % (self.axes, tokens))
         if positions.get_device() != dev:
             raise ValueError("positions: not on the current device")
+        if self.inv_freq.get_device() != dev:
+            raise ValueError("rope: its frequencies are not on the current device")
         r = L.RopeArgs.from_buffer_copy(self._frozen)
         r.positions = positions.data_ptr()
         if self.axes > 1:

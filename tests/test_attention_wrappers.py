@@ -119,16 +119,18 @@ def test_the_branch_reports_a_wait_that_ran_out(calls, monkeypatch):
 
 
 class Elsewhere:
-    """A tensor as it is, but on another device."""
+    """A tensor as it is, but on a GPU: another device than the current one (of device=-1: the current one)."""
 
-    def __init__(self, x):
-        self.x = x
+    is_cuda = True
+
+    def __init__(self, x, device=1):
+        self.x, self.device_number = x, device
 
     def __getattr__(self, name):
         return getattr(self.x, name)
 
     def get_device(self):
-        return 1
+        return self.device_number
 
 
 def test_kv_store_wants_its_cache_on_the_current_device(calls):
@@ -139,4 +141,14 @@ def test_kv_store_wants_its_cache_on_the_current_device(calls):
     cache.k, cache.v = Elsewhere(cache.k), Elsewhere(cache.v)
     with pytest.raises(ValueError, match="cache"):
         A.kv_store(k, k.clone(), cache, slots)
+    assert len(calls.made) == 1
+
+
+def test_the_rotation_wants_its_frequencies_on_the_current_device(calls):
+    q, k, pos = torch.zeros(3, 4, 64, dtype=BF16), torch.zeros(3, 2, 64, dtype=BF16), torch.zeros(3, dtype=torch.int32)
+    here, there = (A.Rope(Elsewhere(torch.ones(32), d)) for d in (-1, 1))
+    A.qk_norm_rope(q, k, None, None, None, 0.0, here, pos, q, k, None)
+    assert len(calls.made) == 1
+    with pytest.raises(ValueError, match="frequencies"):
+        A.qk_norm_rope(q, k, None, None, None, 0.0, there, pos, q, k, None)
     assert len(calls.made) == 1
