@@ -106,6 +106,7 @@ class Q4GroupWeight:
     def __init__(self, codes, scales, zeros=None):
         assert codes.is_cuda and codes.dtype == torch.uint8 and codes.dim() == 2 and codes.is_contiguous()
         assert scales.is_cuda and scales.dtype in _DTYPES and scales.dim() == 2 and scales.shape[0] == codes.shape[0]
+        assert scales.get_device() == codes.get_device() and (zeros is None or zeros.get_device() == codes.get_device())
         self.codes, self.scales = codes, scales.contiguous()
         self.n, self.k = codes.shape[0], 2 * codes.shape[1]
         assert scales.shape[1] and self.k % scales.shape[1] == 0
