@@ -131,9 +131,13 @@ def linear_q4_decode(x, weight, epilogue):
     swiglu, shared_scale) names. Products are exact and sums fp32."""
     assert x.dtype == torch.bfloat16 and x.is_contiguous() and x.shape[1] == weight.k
     assert x.get_device() == weight.codes.get_device() == torch._C._cuda_getDevice()
-    out, values = epilogue._keep[0], x.shape[0] * weight.n
-    assert out.get_device() == x.get_device() and out.numel() == _VALUES.get(epilogue.kind, 1) * values
-    st = L.load().fb_linear_q4_decode(x.data_ptr(), x.shape[0], weight.ref, ctypes.byref(epilogue), L.stream())
+    (out, inj, gate), tokens = epilogue._keep, x.shape[0]
+    assert out.get_device() == x.get_device() and out.numel() == _VALUES.get(epilogue.kind, 1) * tokens * weight.n
+    assert inj is None or inj.get_device() == x.get_device() and inj.numel() == 4 * tokens
+    if gate is not None:  # gate_logit[t * gate_stride] of the last token, within what the tensor reaches
+        reach = sum((n - 1) * s for n, s in zip(gate.shape, gate.stride()))
+        assert gate.get_device() == x.get_device() and gate.numel() and 0 <= max(tokens - 1, 0) * epilogue.gate_stride <= reach
+    st = L.load().fb_linear_q4_decode(x.data_ptr(), tokens, weight.ref, ctypes.byref(epilogue), L.stream())
     if st:
         L.check(st, "linear_q4_decode")
 

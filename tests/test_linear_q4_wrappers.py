@@ -37,3 +37,26 @@ def test_a_weight_lies_on_one_device():
     for scales, zeros in ((1, None), (0, 1), (1, 1), (1, 0)):
         with pytest.raises(AssertionError):
             linear.Q4GroupWeight(codes(), per_group(torch.float16, device=scales), None if zeros is None else per_group(torch.uint8, device=zeros))
+
+
+def test_epilogue_inputs_of_fewer_tokens_or_another_device(monkeypatch):
+    """inj is [tokens][4]; gate_logit reaches the last token's logit: [tokens][513] from column 512 on, one logit per token, one for all."""
+    made = []
+    monkeypatch.setattr(L, "load", lambda: type("Library", (), {"fb_linear_q4_decode": lambda self, *a: made.append(a) or 0})())
+    monkeypatch.setattr(L, "stream", lambda: None)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    w = linear.Q4GroupWeight(codes(), per_group(torch.float32))
+    gpu = lambda *shape, dtype=torch.float32, device=0: OnGpu(torch.zeros(*shape, dtype=dtype), device)
+    x, T = gpu(5, 256, dtype=torch.bfloat16), 5
+    write = lambda inj: linear.gr_write(gpu(T, 4, 6), inj)
+    scale = lambda gate, stride: linear.shared_scale(gpu(T, 6), gate, stride)
+    logits = torch.zeros(T, 513)
+    good = [write(gpu(T, 4)), scale(OnGpu(logits[:, 512:]), 513), scale(OnGpu(logits.view(-1)[512:]), 513), scale(gpu(T), 1), scale(gpu(1), 0), scale(OnGpu(logits), 513)]
+    for epilogue in good:
+        linear.linear_q4_decode(x, w, epilogue)
+    assert len(made) == len(good)
+    for epilogue in [write(gpu(T - 1, 4)), write(gpu(T + 1, 4)), write(gpu(T, 4, device=1)), scale(OnGpu(logits[:T - 1, 512:]), 513),
+                     scale(OnGpu(logits.view(-1)[513:]), 513), scale(gpu(T - 1), 1), scale(gpu(T), 2), scale(gpu(0), 0), scale(gpu(T), -1), scale(gpu(T, device=1), 1)]:
+        with pytest.raises(AssertionError):
+            linear.linear_q4_decode(x, w, epilogue)
+    assert len(made) == len(good)
