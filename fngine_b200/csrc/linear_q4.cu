@@ -517,6 +517,9 @@ int32_t fb_linear_q4_decode(const void* x_bf16, int32_t tokens, const fb_q4_weig
     return invalid("linear_q4_decode: x, weight codes, scales and zeros must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(epilogue->out) & (kind == FB_EPI_STORE_BF16 || kind == FB_EPI_SWIGLU ? 1 : 3))
     return invalid("linear_q4_decode: out is not aligned to its elements");
+  if ((reinterpret_cast<uintptr_t>(kind == FB_EPI_GR_WRITE ? epilogue->inj : nullptr) |
+       reinterpret_cast<uintptr_t>(kind == FB_EPI_SHARED_SCALE ? epilogue->gate_logit : nullptr)) & 3)
+    return invalid("linear_q4_decode: inj or gate_logit is not aligned to its elements");
   const size_t out_values = size_t(tokens) * size_t(n);
   const size_t out_bytes = kind == FB_EPI_GR_WRITE ? 16 * out_values : kind == FB_EPI_STORE_BF16 ? 2 * out_values
                            : kind == FB_EPI_SWIGLU ? out_values : 4 * out_values;

@@ -468,7 +468,8 @@ int32_t fb_linear_fp8_decode(const void* x_bf16, int32_t tokens, const uint8_t* 
  *   out = epilogue(sum over groups of scale[n][g] * sum_{i in g} (code[n][i] - zero[n][g]) * x[t][i])
  * codes [n][k / 2]: value 2j of a row in the low four bits of byte j, value 2j + 1 in the high ones. scales [n][k / group],
  * fp32, bf16 or fp16. zeros [n][k / group]: one byte per group, of which the low four bits count, or NULL: eight everywhere.
- * group 32, 64 or 128; k % 128 == 0; any n (even for SwiGlu) with n * k / group < 2^31. codes, scales, zeros and x are 16-byte aligned.
+ * group 32, 64 or 128; k % 128 == 0; any n (even for SwiGlu) with n * k / group < 2^31. codes, scales, zeros and x are 16-byte aligned,
+ * out, inj and gate_logit to their elements.
  * x is bf16 [tokens][k], tokens 1..16; the epilogues are those of fb_linear_fp8. Products are exact, but activations below
  * 2^-57 (below 2^7 in a token that has one of 2^63 or more) count as zero; sums are fp32; every output is
  * written once, in an order of additions that the shape fixes: repeated calls are bitwise identical. `out` may not lie in the

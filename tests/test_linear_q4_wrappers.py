@@ -60,3 +60,11 @@ def test_epilogue_inputs_of_fewer_tokens_or_another_device(monkeypatch):
         with pytest.raises(AssertionError):
             linear.linear_q4_decode(x, w, epilogue)
     assert len(made) == len(good)
+
+
+def test_epilogue_inputs_that_are_not_aligned(fb_built):
+    from test_linear_q4_arguments import call
+    lib = L.load()
+    for bad in (dict(kind=L.EPI_GR_WRITE, inj=0x600002), dict(kind=L.EPI_GR_WRITE, inj=0x600001), dict(kind=L.EPI_SHARED_SCALE, gate=0x600002)):
+        st, msg = call(lib, **bad)
+        assert st == 1 and b"inj or gate_logit is not aligned" in msg
