@@ -7,10 +7,11 @@
 // 4-7 is 16 c 2^-133, both exact, and eight codes cost one shift and four ANDs. (As whole bf16 numbers, by an exponent under the bits
 // and a subtraction of 128 + z, they cost eleven instructions, and their issue bound the kernel: 110 us for 248320 x 2560 at 16 tokens.)
 // The activations bring the scale back: they are multiplied by 2^64, those of the codes in bits 4-7 by 2^60, exactly; or by 1 and 1/16
-// in a token that has one of 2^63 or more. Products are exact, the tensor core adds them in fp32; what is below 2^-57 (2^7 in such a
-// token, of more than 2^63) counts as zero. What a zero
-// point takes off, z sum(x) of a group, comes from sums of the activations that are made once:
+// in a token that has one of 2^63 or more. Products are exact, the tensor core adds them in fp32 and keeps subnormal sums, so the smallest
+// step of a sum is 2^-149 here and 2^-80 (2^-16 in such a token) in the activations' own scale: what is far below it is lost. What a zero
+// point takes off, z sum(x) of a group, comes from sums of the activations that are made once, with the same smallest step:
 //   acc += s (P - z X),   P = sum of c x 2^-69 over the group, X = sum of x 2^-69.
+// (P and X of an infinite activation are infinite, or P is NaN: their difference is NaN for every weight of that token.)
 // Nothing is rounded but sums.
 //
 // Bound by the weights' bytes at few tokens and instruction issue at sixteen: 248320 x 2560 in 68 us for one token (4.8 TB/s), 99 for

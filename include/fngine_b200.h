@@ -470,8 +470,9 @@ int32_t fb_linear_fp8_decode(const void* x_bf16, int32_t tokens, const uint8_t* 
  * fp32, bf16 or fp16. zeros [n][k / group]: one byte per group, of which the low four bits count, or NULL: eight everywhere.
  * group 32, 64 or 128; k % 128 == 0; any n (even for SwiGlu) with n * k / group < 2^31. codes, scales, zeros and x are 16-byte aligned,
  * out, inj and gate_logit to their elements.
- * x is bf16 [tokens][k], tokens 1..16; the epilogues are those of fb_linear_fp8. Products are exact, but activations below
- * 2^-57 (below 2^7 in a token that has one of 2^63 or more) count as zero; sums are fp32; every output is
+ * x is bf16 [tokens][k], tokens 1..16; the epilogues are those of fb_linear_fp8. Products are exact, sums are fp32 numbers whose
+ * smallest step is 2^-80 (2^-16 in a token that has an activation of 2^63 or more) instead of 2^-149. An activation that is not finite
+ * makes all outputs of its token NaN, where the formula may give an infinity. Every output is
  * written once, in an order of additions that the shape fixes: repeated calls are bitwise identical. `out` may not lie in the
  * memory of x. No workspace. */
 typedef struct fb_q4_weight {
