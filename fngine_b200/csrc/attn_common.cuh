@@ -50,6 +50,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// Weights are 2^kLift times the formula's (their sum too, so it falls out): fp16 numbers end at 2^-24, and many keys whose weights are below
+// that, one by one nothing, may be a good part of a row in sum. 2^7 and the 2^8 that scores may rise above the maximum in use are 2^15.
+template <class T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.f : 0.f;
 // The larger of m and 32 scores.
 __device__ __forceinline__ float scores_max(const float (&s)[32], float m) {
   float a = max3(m, s[0], s[1]), b = max3(s[2], s[3], s[4]), c = max3(s[5], s[6], s[7]);

@@ -10,7 +10,7 @@
 // The two tiles are half a step apart and take turns with S, which a softmax thread has in registers 70 cycles after it is complete:
 // from then on the other tile's scores are made there, so neither softmax waits for the tensor core.
 // m is the maximum that the exponents refer to, not the latest one: it moves up (and O is multiplied) only when a row's scores
-// rise above it by more than 2^8, which leaves every weight at most 256 and the sum in fp32 range. Normally that is
+// rise above it by more than 2^8, which leaves every weight at most 256 (times 2^7 in fp16) and the sum in fp32 range. Normally that is
 // the first block alone, so O stays in tensor memory untouched.
 // Blocks are handed out longest first (causal: the last queries of a prompt have the most keys).
 // Bound by the exponentials (16 per clock and multiprocessor) and the tensor core, which are near level, and then by power: 8192
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
           }
         }
       }
-      const float base = top * a.scale_log2;
+      const float base = top * a.scale_log2 - kLift<T>;
       const uint64_t minus = pair_of(-base, -base);
       uint64_t part[2] = {0, 0};
       if (j == n - 1) {  // (masked scores stay with the exponential unit: exactly zero)

@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1) tree_kernel(const TreeArgs a,
               }
             }
           }
-          const float base = top == -INFINITY ? 0.f : top * a.scale_log2;
+          const float base = (top == -INFINITY ? 0.f : top * a.scale_log2) - kLift<T>;
           const uint64_t minus = pair_of(-base, -base);
           uint64_t part[2] = {0, 0};
 #pragma unroll 1
