@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
   int start = 0, length = -1, item = -1;
   {
     const int number = a.clear && blockIdx.y + 1 == gridDim.y ? INT32_MAX : int(blockIdx.y);
-    int before = 0, least = a.tokens, most = 0;
+    int before = 0;
     for (int base = 0; base < a.n_seqs; base += 32) {
       const int s = base + lane;
       int lo = 0, hi = 0;
@@ -88,10 +88,6 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
         hi = hi < lo ? lo : hi > a.tokens ? a.tokens : hi;
       }
       const int n = (hi - lo + kPfQueries - 1) / kPfQueries;
-      if (n) {
-        least = lo < least ? lo : least;
-        most = hi > most ? hi : most;
-      }
       int upto = n;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -115,6 +111,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) attn_prefill_kernel(const PfArg
       // for its head. (`before` is the number of items where the ends do not fall.)
       const int idle = before >= 0 && before < int(gridDim.y) - 1 ? before : int(gridDim.y) - 1;
       if (!a.clear || int(blockIdx.y) < idle) return;
+      int least = a.tokens, most = 0;
+      for (int i = lane; i < a.n_seqs; i += 32) {
+        const int lo = a.cu_seqlens[i] < 0 ? 0 : a.cu_seqlens[i], hi = a.cu_seqlens[i + 1] < a.tokens ? a.cu_seqlens[i + 1] : a.tokens;
+        if (lo < hi) {
+          least = lo < least ? lo : least;
+          most = hi > most ? hi : most;
+        }
+      }
       least = __reduce_min_sync(0xffffffffu, least);
       most = __reduce_max_sync(0xffffffffu, most);
       most = most < least ? least : most;
