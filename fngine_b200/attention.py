@@ -91,6 +91,8 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, eps, rope, positions, q_out, k_out
     norm = None
     if q_weight is not None or k_weight is not None:
         w_dtype = (k_weight if q_weight is None else q_weight).dtype
+        if w_dtype not in _WEIGHT_DTYPES:
+            raise ValueError("qk_norm_rope: weights are fp32, bf16 or fp16")
         norm = L.QkNorm(None if q_weight is None else _plain(q_weight, (dim,), w_dtype, dev, "q_weight"),
                         None if k_weight is None else _plain(k_weight, (dim,), w_dtype, dev, "k_weight"), _WEIGHT_DTYPES[w_dtype], eps)
     s_at = None if slots is None else _plain(slots, (tokens,), torch.int64, dev, "slots")

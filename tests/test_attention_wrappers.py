@@ -152,3 +152,35 @@ def test_the_rotation_wants_its_frequencies_on_the_current_device(calls):
     with pytest.raises(ValueError, match="frequencies"):
         A.qk_norm_rope(q, k, None, None, None, 0.0, there, pos, q, k, None)
     assert len(calls.made) == 1
+
+
+def rotate(**change):
+    q, k = torch.zeros(3, 4, 64, dtype=BF16), torch.zeros(3, 2, 64, dtype=BF16)
+    a = dict(q=q, k=k, v=None, q_weight=None, k_weight=None, eps=0.0, rope=None, positions=None, q_out=q, k_out=k, v_out=None)
+    a.update(change)
+    return A.qk_norm_rope(**a)
+
+
+def test_each_refusal_of_the_norms_and_rotation_is_its_own(calls):
+    """The arguments without a fault reach the library; each fault by itself has its own message."""
+    q, k, one = torch.zeros(3, 4, 64, dtype=BF16), torch.zeros(3, 2, 64, dtype=BF16), torch.ones(64)
+    rope = A.Rope(Elsewhere(torch.ones(32), -1))
+    axes = A.Rope(Elsewhere(torch.ones(32), -1), sections=(8, 24))
+    pos = torch.zeros(3, dtype=torch.int32)
+    good = [dict(), dict(q_weight=one), dict(k_weight=one.half()), dict(v=k, v_out=k), dict(slots=torch.zeros(3, dtype=torch.int64)), dict(rope=rope, positions=pos),
+            dict(rope=rope, positions=pos[None]), dict(rope=axes, positions=pos[None].expand(2, 3)), dict(k_out=torch.zeros(9, 2, 64, dtype=BF16), slots=torch.zeros(3, dtype=torch.int64))]
+    for change in good:
+        rotate(**change)
+    assert [name for name, _ in calls.made] == ["fb_qk_norm_rope"] * len(good)
+    for change, word in [(dict(q=q.float()), "bf16 or fp16"), (dict(k=k.half()), "^k: "), (dict(k=k[:2]), "^k: "), (dict(q_out=q[:, :3]), "^q_out: "),
+                         (dict(k_out=k[:2]), "another number"), (dict(q=q.transpose(0, 1).contiguous().transpose(0, 1)), "side by side"), (dict(v=k), "together"),
+                         (dict(v_out=k), "together"), (dict(v=k.half(), v_out=k), "^v: "), (dict(v=k, v_out=q), "^v_out: "), (dict(q_weight=torch.ones(63)), "^q_weight: "),
+                         (dict(q_weight=one, k_weight=one.half()), "^k_weight: "), (dict(k_weight=torch.ones(128)[::2]), "^k_weight: "),
+                         (dict(q_weight=one.double()), "weights are"), (dict(slots=torch.zeros(3, dtype=torch.int32)), "^slots: "), (dict(slots=torch.zeros(2, dtype=torch.int64)), "^slots: "),
+                         (dict(rope=rope, positions=pos[:2]), "^positions: "), (dict(rope=rope, positions=pos.long()), "^positions: "), (dict(rope=axes, positions=pos), "^positions: "),
+                         (dict(rope=rope, positions=torch.zeros(6, dtype=torch.int32)[::2]), "^positions: "),
+                         (dict(rope=rope, positions=Elsewhere(pos)), "positions: not on"), (dict(q=Elsewhere(q)), "^q: not on"), (dict(k_out=Elsewhere(k)), "^k_out: not on"),
+                         (dict(q_weight=Elsewhere(one)), "^q_weight: not on"), (dict(slots=Elsewhere(torch.zeros(3, dtype=torch.int64))), "^slots: not on")]:
+        with pytest.raises(ValueError, match=word):
+            rotate(**change)
+    assert len(calls.made) == len(good)
