@@ -183,7 +183,7 @@ def attn_tree_decode(q, cache, block_table, contexts, out, workspace, mask=None,
         raise ValueError("attn_tree_decode: rows of block_table overlap")
     if not (q.get_device() == out.get_device() == block_table.get_device() == workspace.get_device() == cache.k.get_device() == dev):
         raise ValueError("attn_tree_decode: not on the current device")
-    if mask is not None and mask.dtype is not torch.int64:
+    if mask is not None and mask.dtype is torch.uint64:
         mask = mask.view(torch.int64)
     st = L.load().fb_attn_tree_decode_view(q.data_ptr(), strides[0], heads, n_seqs, drafted, cache.ref, block_table.data_ptr(), table_stride, columns,
                                            _plain(contexts, (n_seqs,), torch.int32, dev, "contexts"),

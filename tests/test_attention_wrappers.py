@@ -184,3 +184,32 @@ def test_each_refusal_of_the_norms_and_rotation_is_its_own(calls):
         with pytest.raises(ValueError, match=word):
             rotate(**change)
     assert len(calls.made) == len(good)
+
+
+def test_masks_are_64_bit_words(calls):
+    """Words of another size are not taken two or eight at a time."""
+    table = torch.zeros(3, 4, dtype=torch.int32)
+    for mask in (None, torch.ones(3, 2, dtype=torch.int64), torch.ones(3, 2, dtype=torch.uint64)):
+        tree(table, mask=mask)
+    assert len(calls.made) == 3 and [c[1][10] is None for c in calls.made] == [True, False, False]
+    for mask in (torch.ones(3, 4, dtype=torch.int32), torch.ones(3, 16, dtype=torch.bool), torch.ones(3, 2, dtype=torch.float64), torch.ones(3, 3, dtype=torch.int64),
+                 torch.ones(3, 4, dtype=torch.int64)[:, ::2]):
+        with pytest.raises(ValueError, match="^mask"):
+            tree(table, mask=mask)
+    assert len(calls.made) == 3
+
+
+def test_each_refusal_of_the_tree_is_its_own(calls):
+    table, q = torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, 2, 4, 64, dtype=BF16)
+    tree(table)
+    for change, word in [(dict(q=q.half()), "cache's type"), (dict(out=q.half()), "cache's type"), (dict(out=q[:, :1]), "cache's type"), (dict(cache=cache_of(dim=128)), "cache's type"),
+                         (dict(q=q.transpose(1, 2).contiguous().transpose(1, 2)), "one stride"), (dict(out=torch.zeros(3, 4, 4, 64, dtype=BF16)[:, ::3]), "one stride"),
+                         (dict(block_table=table.long()), "block_table"), (dict(block_table=table[:2]), "block_table"), (dict(contexts=torch.zeros(2, dtype=torch.int32)), "^contexts"),
+                         (dict(contexts=torch.zeros(3, dtype=torch.int64)), "^contexts"), (dict(q=Elsewhere(q)), "current device"),
+                         (dict(workspace=Elsewhere(torch.zeros(8, dtype=torch.uint8))), "current device")]:
+        with pytest.raises(ValueError, match=word):
+            a = dict(table=table)
+            if "block_table" in change:
+                a = dict(table=change.pop("block_table"))
+            tree(**a, **change)
+    assert len(calls.made) == 1
