@@ -135,8 +135,10 @@ def linear_q4_decode(x, weight, epilogue):
     assert out.get_device() == x.get_device() and out.numel() == _VALUES.get(epilogue.kind, 1) * tokens * weight.n
     assert inj is None or inj.get_device() == x.get_device() and inj.numel() == 4 * tokens
     if gate is not None:  # gate_logit[t * gate_stride] of the last token, within what the tensor reaches
-        reach = sum((n - 1) * s for n, s in zip(gate.shape, gate.stride()))
-        assert gate.get_device() == x.get_device() and gate.numel() and 0 <= max(tokens - 1, 0) * epilogue.gate_stride <= reach
+        assert gate.get_device() == x.get_device() and gate.numel()
+        if tokens > 1:
+            strides = gate.stride()
+            assert 0 <= (tokens - 1) * epilogue.gate_stride <= sum(map(int.__mul__, gate.shape, strides)) - sum(strides)
     st = L.load().fb_linear_q4_decode(x.data_ptr(), tokens, weight.ref, ctypes.byref(epilogue), L.stream())
     if st:
         L.check(st, "linear_q4_decode")
