@@ -32,7 +32,7 @@ struct QkArgs {
   const int64_t* slots;
   int64_t n_slots;
   float eps;
-  int weight_dtype, heads, kv_heads, half, adjacent;
+  int weight_dtype, half, adjacent;
   int rows;              // heads of all tensors
   int tiles, shortest, longer;  // tiles of `shortest` tokens, the first `longer` of them with one more
   int first[3];          // first row of q, k, v
@@ -336,8 +336,6 @@ int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm
   a.n_slots = out->n_slots;
   if (a.slots && (reinterpret_cast<uintptr_t>(a.slots) & 7)) return invalid("qk_norm_rope: slots are not aligned");
   if (a.slots && a.n_slots <= 0) return invalid("qk_norm_rope: slots without n_slots");
-  a.heads = in->heads;
-  a.kv_heads = in->kv_heads;
   // Tiles of up to kQkTile tokens where every block gets a step of one; the passes over a token's heads go to as many blocks as it takes to
   // give each multiprocessor's blocks two tiles (the angles are made once more in each). Tiles as even as they come: all blocks end together.
   const int per_pass = kQkThreads / (dim / 8), passes = (a.rows + per_pass - 1) / per_pass, room = kQkBlocks * sm_count();
