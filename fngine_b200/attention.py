@@ -218,6 +218,10 @@ class AttentionBranch:
     def __init__(self, qkv, out, q_weight, k_weight, eps, rope, heads, kv_heads, head_dim, max_tokens):
         if qkv.n != (heads + 2 * kv_heads) * head_dim or out.k != heads * head_dim:
             raise ValueError("AttentionBranch: the projections do not fit the heads")
+        if head_dim not in (64, 128):
+            raise ValueError("AttentionBranch: head_dim 64 or 128")
+        if qkv.codes.get_device() != out.codes.get_device():
+            raise ValueError("AttentionBranch: the projections are not on one device")
         self.qkv, self.out, self.q_weight, self.k_weight, self.eps, self.rope = qkv, out, q_weight, k_weight, eps, rope
         self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
         device = qkv.codes.device

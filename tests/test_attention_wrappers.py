@@ -213,3 +213,14 @@ def test_each_refusal_of_the_tree_is_its_own(calls):
                 a = dict(table=change.pop("block_table"))
             tree(**a, **change)
     assert len(calls.made) == 1
+
+
+def test_a_branch_refuses_projections_that_its_calls_could_not_use(monkeypatch):
+    """Another head_dim than attention takes, projections on two devices: before any buffer is made."""
+    assert branch_of(monkeypatch, dim=128).head_dim == 128
+    for dim in (32, 96, 256):
+        with pytest.raises(ValueError, match="head_dim"):
+            branch_of(monkeypatch, dim=dim)
+    here, there = (types.SimpleNamespace(n=512, k=256, codes=Elsewhere(torch.zeros(1, dtype=torch.uint8), d)) for d in (0, 1))
+    with pytest.raises(ValueError, match="one device"):
+        A.AttentionBranch(here, there, None, None, 1e-6, None, 4, 2, 64, 8)
