@@ -67,7 +67,7 @@ __device__ __forceinline__ float scores_max(const float (&s)[32], float m) {
 }
 // 2^x of a pair on the multiply-add pipe: x = n + f with n whole and |f| <= 1/2 (adding 1.5 * 2^23 rounds to whole numbers and leaves
 // n in the low bits), a polynomial of degree four for 2^f (minimax by Remez exchange, relative error 2.7e-6), n into the exponent.
-// Below -126 it stays at 2^-126, so not for scores that are masked. NaN does not stay NaN: the row's maximum has to show it.
+// Below -126 it stays at 2^-126, so not for scores that are masked (and a score of minus infinity keeps that weight). NaN does not stay NaN: the row's maximum has to show it.
 __device__ __forceinline__ void exp2_poly(uint64_t x2, float& x, float& y) {
   float a, b;
   unpair(x2, a, b);
@@ -87,8 +87,9 @@ __device__ __forceinline__ void exp2_poly(uint64_t x2, float& x, float& y) {
   x = __uint_as_float(__float_as_uint(a) + (__float_as_uint(n0) << 23));
   y = __uint_as_float(__float_as_uint(b) + (__float_as_uint(n1) << 23));
 }
-// 32 weights 2^(scale s - base) as pairs of T (rounded to the type of v: half a step of each weight, averaged over the keys) and, before
-// that rounding, added to `sum` (a pair of partial sums). MIXED: two of sixteen pairs by exp2_poly, which takes work off the exponential
+// 32 weights 2^(scale s - base) as pairs of T and, before the rounding to it, added to `sum` (a pair of partial sums). The products take weights
+// of v's type: half a step of each, which costs an output of values with mean zero about as much as its own rounding does (bf16, rms against
+// 64 bits: 0.0016 with weights in 32 bits, 0.0020 for 8192 tokens). MIXED: two of sixteen pairs by exp2_poly, which takes work off the exponential
 // unit (eight cycles per warp and instruction, 2048 of some 2600 cycles that two softmax warps of a scheduler have for a block of keys)
 // at nine instructions a pair: 8192 tokens 624 us with none, 616 with two, 619 with four, 653 with six.
 template <class T, bool MIXED>

@@ -14,7 +14,7 @@
 // (P and X of an infinite activation are infinite, or P is NaN: their difference is NaN for every weight of that token.)
 // Nothing is rounded but sums.
 //
-// Bound by the weights' bytes at few tokens and instruction issue at sixteen: 248320 x 2560 in 68 us for one token (4.8 TB/s), 99 for
+// Bound by the weights' bytes at few tokens and instruction issue at sixteen: 248320 x 2560 in 69 us for one token (4.8 TB/s), 99 for
 // sixteen. The weights are the only large operand, so the kernel is built around their stream. A warp takes 16 MT rows (the M
 // side of mma.sync m16n8k16, the tokens are the N side) through K in steps of 128: its own ring of cp.async stages in
 // shared memory, no barrier between warps. ldmatrix gives lane (g, t) of a quad eight consecutive codes of row g. The activations lie
