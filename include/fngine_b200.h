@@ -547,7 +547,8 @@ int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm
  * of all sequences are left as they were. A sequence's result does not depend on what lies beside it; its own keys and values are to
  * be finite. Softmax statistics and sums are fp32, the weights are rounded to the type of v; repeated calls are bitwise
  * identical. cu_seqlens is read on the device. `status` (one device word, may be NULL) is set to FB_STATUS_PIPELINE_TIMEOUT when a bounded
- * wait ran out, and left as it was otherwise: rows of out are then missing. No workspace. out lies apart from q, k and v. head_dim 64 or 128; everything 16-byte aligned, strides multiples of 8 elements. */
+ * wait ran out, and left as it was otherwise: rows of out are then missing. No workspace. out lies apart from q, k and v. head_dim 64 or 128; everything 16-byte aligned, strides multiples of 8 elements;
+ * tokens / 256 + min(n_seqs, tokens) below 65535. */
 int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seqlens, int32_t n_seqs, float scale, void* out,
                         int64_t out_stride, uint32_t* status, void* stream);
 /* The same, but tokens outside of all sequences (in front of the first, behind the last: a batch padded to a fixed width) get zeros, so
