@@ -547,7 +547,8 @@ int32_t fb_qk_norm_rope(const fb_qkv* in, int32_t tokens, const fb_qk_norm* norm
  * of all sequences are left as they were. A sequence's result does not depend on what lies beside it; its own keys and values are to
  * be finite. Softmax statistics and sums are fp32, the weights are rounded to the type of v; repeated calls are bitwise
  * identical. cu_seqlens is read on the device. `status` (one device word, may be NULL) is set to FB_STATUS_PIPELINE_TIMEOUT when a bounded
- * wait ran out, and left as it was otherwise: rows of out are then missing. No workspace. out lies apart from q, k and v. head_dim 64 or 128; everything 16-byte aligned, strides multiples of 8 elements;
+ * wait ran out (rows of out are missing then) and left as it was otherwise. No workspace. out lies apart from q, k and v. head_dim 64 or 128;
+ * everything 16-byte aligned, strides multiples of 8 elements;
  * tokens / 256 + min(n_seqs, tokens) below 65535. */
 int32_t fb_attn_prefill(const fb_qkv* in, int32_t tokens, const int32_t* cu_seqlens, int32_t n_seqs, float scale, void* out,
                         int64_t out_stride, uint32_t* status, void* stream);
@@ -567,8 +568,8 @@ typedef struct fb_kv_cache {
   int32_t head_dim;
 } fb_kv_cache;
 /* Attention of `drafted` tokens (1..64) per sequence over the cache. Position p of sequence s lies in page block_table[s *
- * table_stride + p / page_size] of the table's table_stride columns; positions 0 .. contexts[s] - 1 are the context, which every token sees, and the keys and
- * values of the drafted tokens follow at contexts[s] .. contexts[s] + drafted - 1 (fb_qk_norm_rope puts them there). Token
+ * table_stride + p / page_size] of the table's table_stride columns; positions 0 .. contexts[s] - 1 are the context, which every token
+ * sees, and the keys and values of the drafted tokens follow at contexts[s] .. contexts[s] + drafted - 1 (fb_qk_norm_rope puts them there). Token
  * i sees drafted token d if bit d of mask[s * drafted + i] is set; mask NULL: if d <= i. So one token per sequence is plain
  * decoding, and a shorter tree is padded with tokens whose masks are zero. q and out are [n_seqs * drafted][heads][head_dim] with
  * strides between tokens; query head h reads key head h / (heads / kv_heads).
